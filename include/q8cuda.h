@@ -172,7 +172,9 @@ int q8_rope_inv_freq(const q8_config* cfg, float* out);
  * (src/llama_common.mojo:299-342) with the page table of a paged cache.
  * qkv [T, ldqkv] f32 holds q | k | v per token; q (and k) are rotated in place.
  * k_pages / v_pages: [num_pages, n_kv, page, hd] f32.  pos[T], seq[T] int32;
- * block_table [n_seq, max_pages] int32.  q_norm / k_norm may be NULL. */
+ * block_table [n_seq, max_pages] int32.  q_norm / k_norm may be NULL.  With
+ * k_pages, v_pages, seq and block_table all NULL the rows are only rotated (for a
+ * cache of another kind, q8op_kv8_append). */
 int q8op_rope_kv_append(float* qkv, int64_t ldqkv, int64_t T, const int32_t* pos,
                         const int32_t* seq, int n_heads, int n_kv, int hd,
                         const float* inv_freq, const uint16_t* q_norm,
@@ -209,6 +211,146 @@ int q8op_argmax(const float* logits, int64_t rows, int64_t n, int64_t ld, int32_
  * per-device op scratch (28 bytes per logit).  exp() is CUDA's expf. */
 int q8op_sample(const float* logits, int64_t rows, int64_t n, int64_t ld, float temp, float top_p,
                 const float* u, int32_t* out, void* stream);
+
+/* ------------------------------------------------- 8-bit paged KV cache, op level
+ * No counterpart in the reference, whose cache is f32 (k_rope_qk_copy2,
+ * src/llama_common.mojo:299-342).  Pages of one layer: int8 codes
+ * [num_pages, n_kv, page, head_dim] and one f32 scale per Q8_KV8_BLOCK
+ * consecutive tokens of a kv head, [num_pages, n_kv, page / Q8_KV8_BLOCK], for
+ * k and for v; the value is code * scale.  page is a multiple of
+ * Q8_KV8_BLOCK, head_dim 64 or 128, the code arrays 16-byte aligned.
+ *
+ * The rows of a call are packed: rows seq_start[b] .. seq_start[b + 1] - 1
+ * belong to sequence b (seq_start [S + 1], not decreasing) and are its last
+ * positions, ctx[b] - n .. ctx[b] - 1, where ctx[b] counts the sequence's
+ * positions with the call's rows among them.  Rows from seq_start[S] on are
+ * padding: nothing is read or written for them.  Rows that would lie before
+ * position 0 have no position.  block_table [S, max_pages] int32 holds the
+ * page of each `page` positions; an entry outside [0, num_pages), or a position
+ * past the table, is a page that is not there.  All of these are device
+ * memory.  Nothing is allocated and no scratch is shared: calls on different
+ * streams are independent as long as their tensors are. */
+#define Q8_KV8_BLOCK 16
+typedef struct q8_kv8_pages {
+  int8_t* k;
+  int8_t* v;
+  float* k_scale;
+  float* v_scale;
+  int64_t num_pages;
+  int32_t n_kv, page, head_dim;
+} q8_kv8_pages;
+
+/* Writes the rows' k and v (rotated, dtype Q8_F32 / Q8_BF16 / Q8_F16, rows of
+ * n_kv * head_dim elements ldk / ldv apart) into the pages.  The scale of a
+ * block becomes max|x| / 127 of its new tokens, rounded to f32, or stays where
+ * the block has earlier tokens and their scale is larger; codes that stay
+ * become round(code * old / new), new ones round(x / scale), both of the exact
+ * quotient, ties to even, within +-127.  A block whose first token is new
+ * starts over.  NaN is stored as 0; infinities as +-127, and they do not
+ * enter the scale.  Rows whose page is not there are left out.  The table may
+ * not lead two of the call's rows to the same place. */
+int q8op_kv8_append(const void* k, int64_t ldk, const void* v, int64_t ldv, int dtype, int64_t rows,
+                    const int32_t* seq_start, const int32_t* ctx, int64_t S, const q8_kv8_pages* kv,
+                    const int32_t* block_table, int max_pages, void* stream);
+
+/* The cached values of the rows' positions as f32 [rows, n_kv, head_dim]
+ * (the inverse of the append, as q8op_dequant is of q8op_pack).  Rows without
+ * a page or a position read as zeros. */
+int q8op_kv8_read(const q8_kv8_pages* kv, const int32_t* seq_start, const int32_t* ctx, int64_t S,
+                  const int32_t* block_table, int max_pages, float* k, float* v, int64_t rows, void* stream);
+
+/* Causal GQA attention over the 8-bit cache: q8op_attention for packed rows.
+ * q, out: rows of n_heads * head_dim elements of `dtype`, ldq / ldo apart.  A
+ * row attends to the positions 0 .. its own of its sequence; positions whose
+ * page is not there are masked (pages freed behind a window, say), and a row
+ * that sees no position gives zeros.  Scores, softmax statistics and sums are
+ * f32. */
+int q8op_kv8_attention(const void* q, int64_t ldq, int dtype, int64_t rows, const int32_t* seq_start,
+                       const int32_t* ctx, int64_t S, int n_heads, const q8_kv8_pages* kv,
+                       const int32_t* block_table, int max_pages, void* out, int64_t ldo, void* stream);
+
+/* ---------------------------------------------------- page tables, op level
+ * Device-side state of a paged cache of either kind (the reference has one
+ * sequence and no pages): block_table [S, max_pages] int32, contiguous, -1
+ * where there is no page; ctx [S] int32, the sequences' lengths; refs
+ * [num_pages] int32, how many table entries hold a page, 0: free.  Pages taken
+ * are always the lowest free ones, so equal states give equal results.  At
+ * most 8192 sequences; calls on one state must be ordered by the caller. */
+
+/* Shortens sequence s to new_len[s] (device, [S]) positions and lets go of
+ * every page behind them, pages reserved in advance included; 0 frees the
+ * sequence, a length not below ctx[s] only drops reserved pages, a negative
+ * one leaves the sequence alone. */
+int q8op_kv_truncate(int32_t* block_table, int64_t S, int max_pages, int32_t* ctx, int32_t* refs,
+                     int64_t num_pages, int page, const int32_t* new_len, void* stream);
+
+/* Sequence dst[i] becomes sequence src[i] as it was before the call, sharing
+ * the pages of its positions (reserved pages are not shared); what dst[i] held
+ * is let go of.  All n pairs (device, int32) happen at once, so a beam search
+ * may permute its beams.  A pair with a number outside [0, S) is left out; of
+ * pairs with the same dst the last one counts. */
+int q8op_kv_fork(int32_t* block_table, int64_t S, int max_pages, int32_t* ctx, int32_t* refs, int64_t num_pages,
+                 int page, const int32_t* src, const int32_t* dst, int64_t n, void* stream);
+
+/* Makes room for n_new[s] (device, [S]; <= 0: none) more positions of every
+ * sequence: missing pages are taken, and a page that is shared and will be
+ * written is replaced by a new one, of which src[s] / dst[s] give the pair to
+ * copy (q8op_kv_copy_pages; -1: none).  When all sharers of a page write, the
+ * first of them keeps it.  Requests are served in the order of (sequence,
+ * position).  ctx grows by n_new.  All or nothing: when the pool or a table row
+ * is too small, nothing changes, and src / dst are -1.  status [3]: Q8_OK or
+ * Q8_ERR_KV_FULL, pages wanted (of the rows that fit their table), pages free
+ * after the call.  src, dst [S], status and work [num_pages] are int32 device
+ * memory, work being scratch. */
+int q8op_kv_reserve(int32_t* block_table, int64_t S, int max_pages, int32_t* ctx, int32_t* refs, int64_t num_pages,
+                    int page, const int32_t* n_new, int32_t* src, int32_t* dst, int32_t* status, int32_t* work,
+                    void* stream);
+
+/* Renumbers the pages so that those in use are the first ones: the k-th used
+ * page above the number of used pages becomes the k-th free one below it.
+ * src / dst [num_pages / 2] int32 give the copies to make, -1 behind the last;
+ * work [num_pages] int32 is scratch.  The table has to hold every counted
+ * entry. */
+int q8op_kv_compact(int32_t* block_table, int64_t S, int max_pages, int32_t* refs, int64_t num_pages, int32_t* src,
+                    int32_t* dst, int32_t* work, void* stream);
+
+/* Copies page src[i] to page dst[i] (device, int32, n of them) in each of up
+ * to 64 pools: pools / page_bytes are host arrays of their device addresses
+ * and of the bytes of one page.  A pair with a number outside [0, num_pages) is
+ * left out; so is one whose dst is also a source of the call, or the dst of
+ * another pair, since such a result would depend on the order. */
+int q8op_kv_copy_pages(void* const* pools, const int64_t* page_bytes, int n_pools, int64_t num_pages,
+                       const int32_t* src, const int32_t* dst, int64_t n, void* stream);
+
+/* ------------------------------------------- speculative decoding, op level */
+
+/* The distribution that q8op_sample draws from at top_p = 1 (sample(),
+ * src/sample.mojo:15-59): p = w / sum w, w = exp((l - max) / temp) where
+ * l >= max - 16, else 0.  temp <= 0: 1 at the first maximum.  NaN and -inf
+ * count as never; a row without any other logit gives 1 at index 0.  logits
+ * [rows, ld] f32 with n used columns, out [rows, ldo] f32. */
+int q8op_probs(const float* logits, int64_t rows, int64_t n, int64_t ld, float temp, float* out, int64_t ldo,
+               void* stream);
+
+/* Verification of drafted tokens (speculative sampling).  The rows
+ * seq_start[b] .. seq_start[b + 1] - 1 of p [rows, ldp] are the target model's
+ * distributions behind the tokens ids [rows] it was fed: a sequence's last
+ * known token, then its drafts, so the draft behind row r is ids[r + 1].  q
+ * [q_rows, ldq] holds the draft model's distributions in the same order
+ * without a row for the last one of a sequence (NULL: the drafts were certain).
+ * u [rows]: uniform draws in [0, 1).  The draft x behind row r is kept while
+ * u[r] * q_r(x) < p_r(x).  The next token is then drawn from max(p - q, 0) at
+ * the first refused row, or from the last row's p: the first index whose
+ * cumulative weight exceeds u[last row] times the whole (from p itself when
+ * max(p - q, 0) is all zero).  n_accepted [S]: drafts kept.  tokens [rows]:
+ * the kept drafts, the next token, then -1, from seq_start[b] on.  Sums are 64
+ * bits.  NaN and negative weights count as 0; a draft outside [0, n), or
+ * whose row of q is not among the q_rows, is refused; a row without any weight
+ * gives token 0.  Rows from seq_start[S] on
+ * are left as they are.  No counterpart in the reference. */
+int q8op_verify(const float* p, int64_t ldp, const float* q, int64_t ldq, int64_t q_rows, const int32_t* ids,
+                const int32_t* seq_start, int64_t rows, int64_t S, int64_t n, const float* u, int32_t* n_accepted,
+                int32_t* tokens, void* stream);
 
 /* ================================================================ model level */
 

@@ -27,6 +27,11 @@ class q8_config(C.Structure):
                 ("tied", C.c_int32), ("weight_dtype", C.c_int32)]
 
 
+class q8_kv8_pages(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("num_pages", C.c_int64), ("n_kv", C.c_int32), ("page", C.c_int32), ("head_dim", C.c_int32)]
+
+
 class Q8Error(RuntimeError):
     """Raised on a non-zero status; ``.status`` holds the code."""
 
@@ -66,6 +71,16 @@ SIGNATURES = {
     "q8op_attention": [_P, _I64, _I64, _P, _P, _I32, _I32, _I32, _P, _P, _I32, _P, _I32, _P, _I64, _P],
     "q8op_argmax": [_P, _I64, _I64, _I64, _P, _P],
     "q8op_sample": [_P, _I64, _I64, _I64, _F, _F, _P, _P, _P],
+    "q8op_kv8_append": [_P, _I64, _P, _I64, _I32, _I64, _P, _P, _I64, _P, _P, _I32, _P],
+    "q8op_kv8_read": [_P, _P, _P, _I64, _P, _I32, _P, _P, _I64, _P],
+    "q8op_kv8_attention": [_P, _I64, _I32, _I64, _P, _P, _I64, _I32, _P, _P, _I32, _P, _I64, _P],
+    "q8op_kv_truncate": [_P, _I64, _I32, _P, _P, _I64, _I32, _P, _P],
+    "q8op_kv_fork": [_P, _I64, _I32, _P, _P, _I64, _I32, _P, _P, _I64, _P],
+    "q8op_kv_reserve": [_P, _I64, _I32, _P, _P, _I64, _I32, _P, _P, _P, _P, _P, _P],
+    "q8op_kv_compact": [_P, _I64, _I32, _P, _I64, _P, _P, _P, _P],
+    "q8op_kv_copy_pages": [_P, _P, _I32, _I64, _P, _P, _I64, _P],
+    "q8op_probs": [_P, _I64, _I64, _I64, _F, _P, _I64, _P],
+    "q8op_verify": [_P, _I64, _P, _I64, _I64, _P, _P, _I64, _I64, _I64, _P, _P, _P, _P],
     "q8_create": [C.POINTER(q8_config), _I32, _I32, _I32, _I32, _I32, _I32, _P, C.POINTER(_P)],
     "q8_destroy": [_P],
     "q8_nccl_unique_id": [_P],

@@ -161,6 +161,11 @@ __global__ void __launch_bounds__(256) k_rope_kv(float* __restrict__ qkv, int64_
     for (int j = 0; j < J; ++j) base[lane + 32 * j] = v[j];
     return;
   }
+  if (!kp) {  // rotation only
+#pragma unroll
+    for (int j = 0; j < J; ++j) base[lane + 32 * j] = v[j];
+    return;
+  }
   const int kvh = h - nh;
   const int pg = bt[(int64_t)seq[t] * max_pages + p / page];
   const int64_t off = (((int64_t)pg * nkv + kvh) * page + (p % page)) * HD;
@@ -632,7 +637,10 @@ extern "C" int q8op_rope_kv_append(float* qkv, int64_t ldqkv, int64_t T, const i
                                    int n_heads, int n_kv, int hd, const float* inv_freq, const uint16_t* q_norm,
                                    const uint16_t* k_norm, float eps, float* k_pages, float* v_pages, int page,
                                    const int32_t* block_table, int max_pages, void* stream) {
-  Q8_CHECK_ARG(qkv && pos && seq && inv_freq && k_pages && v_pages && block_table, "q8op_rope_kv_append: null");
+  const bool only = !k_pages && !v_pages && !block_table && !seq;  // rotation without an append
+  Q8_CHECK_ARG(qkv && pos && inv_freq && (only || (seq && k_pages && v_pages && block_table)),
+               "q8op_rope_kv_append: null");
+  if (only) page = max_pages = 1;
   Q8_CHECK_ARG(n_heads > 0 && n_kv > 0 && page > 0 && max_pages > 0 && ldqkv >= (int64_t)(n_heads + 2 * n_kv) * hd,
                "q8op_rope_kv_append: bad shape");
   return rope_kv_launch(qkv, ldqkv, T, pos, seq, n_heads, n_kv, hd, inv_freq, q_norm, k_norm, eps, k_pages,

@@ -7,6 +7,13 @@ Names follow the reference kernels they replace: ``pack_q8`` (quantize.py:31),
 :299), ``attention`` (k_scores/k_softmax_rows/k_att_out, :402-473),
 ``argmax`` (k_argmax, :493).  Tensors are torch CUDA tensors (torch provides
 device memory and the stream); every kernel is in libq8cuda.so.
+
+Without a counterpart in the reference: the 8-bit paged cache (``KV8Pages``,
+``kv8_append``, ``kv8_read``, ``kv8_attention``), the page tables of either cache
+(``kv_truncate``, ``kv_fork``, ``kv_reserve``, ``kv_compact``, ``kv_copy_pages``) and
+speculative decoding (``probs``, ``verify``).  include/q8cuda.h says what each
+does; these run on the device of their tensors, on torch's current stream
+there, and may be captured into CUDA graphs.
 """
 from __future__ import annotations
 
@@ -129,6 +136,14 @@ def rope_inv_freq(cfg) -> torch.Tensor:
     return torch.from_numpy(out)
 
 
+def rope(qkv, pos, n_heads, n_kv, hd, inv_freq, q_norm=None, k_norm=None, eps=1e-6):
+    """(QK-norm and) RoPE of the q and k heads of q|k|v rows, in place, without an append."""
+    _need_cuda(qkv, pos, inv_freq, q_norm, k_norm)
+    check(lib().q8op_rope_kv_append(_p(qkv), qkv.stride(0), qkv.shape[0], _p(pos), None, n_heads, n_kv, hd,
+                                    _p(inv_freq), _p(q_norm), _p(k_norm), eps, None, None, 0, None, 0,
+                                    _stream(qkv)))
+
+
 def rope_kv_append(qkv, pos, seq, n_heads, n_kv, hd, inv_freq, q_norm, k_norm, eps, k_pages, v_pages, page,
                    block_table):
     _need_cuda(qkv, pos, seq, inv_freq, k_pages, v_pages, block_table)
@@ -156,6 +171,275 @@ def argmax(logits: torch.Tensor) -> torch.Tensor:
     check(lib().q8op_argmax(_p(logits), logits.shape[0], logits.shape[1], logits.stride(0), _p(out),
                             _stream(logits)))
     return out
+
+
+# ------------------------------------------------------------------ 8-bit paged cache
+KV8_BLOCK = 16  # tokens of a kv head that share a scale (Q8_KV8_BLOCK)
+
+
+def _tensor(t, what, dtype, shape=None, device=None):
+    """A contiguous CUDA tensor of ``dtype`` (and shape, and device)."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError(f"{what}: libq8cuda ops take CUDA tensors")
+    if t.dtype != dtype:
+        raise ValueError(f"{what}: {dtype} wanted, got {t.dtype}")
+    if not t.is_contiguous():
+        raise ValueError(f"{what}: must be contiguous")
+    if shape is not None and tuple(t.shape) != shape:
+        raise ValueError(f"{what}: shape {shape} wanted, got {tuple(t.shape)}")
+    if device is not None and t.device != device:
+        raise ValueError(f"{what}: is on {t.device}, other tensors of the call on {device}")
+
+
+def _call(fn, dev: torch.device, *args):
+    """fn(*args, stream) on torch's current stream of ``dev``."""
+    if torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev):
+            check(fn(*args, torch.cuda.current_stream(dev).cuda_stream))
+    else:
+        check(fn(*args, torch.cuda.current_stream(dev).cuda_stream))
+
+
+class KV8Pages:
+    """One layer's pages of the 8-bit cache: int8 codes k, v [num_pages, n_kv, page, head_dim]
+    and f32 scales k_scale, v_scale [num_pages, n_kv, page / 16]; a value is code * scale."""
+
+    __slots__ = ("k", "v", "k_scale", "v_scale", "num_pages", "n_kv", "page", "head_dim", "_c", "_ref")
+
+    def __init__(self, k, v, k_scale, v_scale):
+        _tensor(k, "KV8Pages k", torch.int8)
+        if k.dim() != 4 or k.shape[2] == 0 or k.shape[2] % KV8_BLOCK or k.shape[3] not in (64, 128):
+            raise ValueError(f"KV8Pages k: [pages, n_kv, page (a multiple of {KV8_BLOCK}), head_dim (64 or 128)] "
+                             f"wanted, got {tuple(k.shape)}")
+        pages, kv, page, hd = k.shape
+        _tensor(v, "KV8Pages v", torch.int8, tuple(k.shape), k.device)
+        for t, what in ((k_scale, "KV8Pages k_scale"), (v_scale, "KV8Pages v_scale")):
+            _tensor(t, what, torch.float32, (pages, kv, page // KV8_BLOCK), k.device)
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.num_pages, self.n_kv, self.page, self.head_dim = pages, kv, page, hd
+        self._c = _lib.q8_kv8_pages(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages, kv,
+                                    page, hd)
+        self._ref = C.addressof(self._c)
+
+    @classmethod
+    def empty(cls, num_pages: int, n_kv: int, page: int = 64, head_dim: int = 128, device="cuda") -> "KV8Pages":
+        """Zeroed pages."""
+        shape = (num_pages, n_kv, page, head_dim)
+        scales = (num_pages, n_kv, page // KV8_BLOCK)
+        return cls(torch.zeros(shape, dtype=torch.int8, device=device),
+                   torch.zeros(shape, dtype=torch.int8, device=device),
+                   torch.zeros(scales, dtype=torch.float32, device=device),
+                   torch.zeros(scales, dtype=torch.float32, device=device))
+
+    @property
+    def device(self) -> torch.device:
+        return self.k.device
+
+    def tensors(self) -> list:
+        """The four pools, as kv_copy_pages takes them."""
+        return [self.k, self.v, self.k_scale, self.v_scale]
+
+
+def _packed(what, seq_start, ctx, pages, block_table):
+    """Checks what every call on packed rows takes; returns (S, max_pages, device)."""
+    if not isinstance(pages, KV8Pages):
+        raise ValueError(f"{what}: pages must be a KV8Pages")
+    dev = pages.k.device
+    if ctx.dim() != 1 or block_table.dim() != 2:
+        raise ValueError(f"{what}: ctx [S] and block_table [S, max_pages] wanted")
+    S, width = block_table.shape
+    _tensor(seq_start, f"{what}: seq_start", torch.int32, (S + 1,), dev)
+    _tensor(ctx, f"{what}: ctx", torch.int32, (S,), dev)
+    _tensor(block_table, f"{what}: block_table", torch.int32, None, dev)
+    return S, width, dev
+
+
+def _rows_of(t, what, width, dev):
+    """[T, width] or [T, heads, head_dim] rows with contiguous elements: (row count, row stride)."""
+    if not t.is_cuda or t.device != dev:
+        raise ValueError(f"{what}: is on {t.device}, the pages are on {dev}")
+    if t.dtype not in _DT:
+        raise ValueError(f"{what}: f32, bf16 or f16 rows wanted, got {t.dtype}")
+    st, sh = t.stride(), t.shape
+    if t.dim() == 2 and sh[1] == width and (st[1] == 1 or width == 1):
+        return sh[0], st[0] if sh[0] > 1 else max(st[0], width)
+    if t.dim() == 3 and sh[1] * sh[2] == width and st[2] == 1 and (st[1] == sh[2] or sh[1] == 1):
+        return sh[0], st[0] if sh[0] > 1 else max(st[0], width)
+    raise ValueError(f"{what}: rows of {width} contiguous elements wanted, got shape {tuple(sh)}, strides {st}")
+
+
+def kv8_append(k, v, seq_start, ctx, pages: KV8Pages, block_table) -> None:
+    """Write the packed rows' (rotated) k and v, the last positions of their sequences, into
+    the 8-bit pages (q8op_kv8_append).  ctx counts them already."""
+    S, width, dev = _packed("kv8_append", seq_start, ctx, pages, block_table)
+    w = pages.n_kv * pages.head_dim
+    T, ldk = _rows_of(k, "kv8_append: k", w, dev)
+    Tv, ldv = _rows_of(v, "kv8_append: v", w, dev)
+    if T != Tv or k.dtype != v.dtype:
+        raise ValueError("kv8_append: k and v must have the same rows and type")
+    _call(lib().q8op_kv8_append, dev, k.data_ptr(), ldk, v.data_ptr(), ldv, _DT[k.dtype], T, seq_start.data_ptr(),
+          ctx.data_ptr(), S, pages._ref, block_table.data_ptr(), width)
+
+
+def kv8_read(seq_start, ctx, pages: KV8Pages, block_table, rows: int):
+    """(k, v) f32 [rows, n_kv, head_dim]: the cached values at the packed rows' positions
+    (rows behind the last sequence are not written)."""
+    S, width, dev = _packed("kv8_read", seq_start, ctx, pages, block_table)
+    if rows < 0:
+        raise ValueError("kv8_read: rows < 0")
+    shape = (rows, pages.n_kv, pages.head_dim)
+    k, v = torch.empty(shape, device=dev), torch.empty(shape, device=dev)
+    _call(lib().q8op_kv8_read, dev, pages._ref, seq_start.data_ptr(), ctx.data_ptr(), S, block_table.data_ptr(),
+          width, k.data_ptr(), v.data_ptr(), rows)
+    return k, v
+
+
+def kv8_attention(q, seq_start, ctx, n_heads: int, pages: KV8Pages, block_table, out=None) -> torch.Tensor:
+    """Causal GQA attention of packed rows over the 8-bit cache (q8op_kv8_attention).  Returns
+    [T, n_heads * head_dim] of q's type; ``out`` may be given (its padding rows are left alone)."""
+    S, width, dev = _packed("kv8_attention", seq_start, ctx, pages, block_table)
+    w = n_heads * pages.head_dim
+    T, ldq = _rows_of(q, "kv8_attention: q", w, dev)
+    if out is None:
+        out = torch.empty((T, w), dtype=q.dtype, device=dev)
+        ldo = w
+    else:
+        To, ldo = _rows_of(out, "kv8_attention: out", w, dev)
+        if To != T or out.dtype != q.dtype:
+            raise ValueError("kv8_attention: out must have q's rows and type")
+    _call(lib().q8op_kv8_attention, dev, q.data_ptr(), ldq, _DT[q.dtype], T, seq_start.data_ptr(), ctx.data_ptr(), S,
+          n_heads, pages._ref, block_table.data_ptr(), width, out.data_ptr(), ldo)
+    return out
+
+
+# ------------------------------------------------------------------ page tables
+def _state(what, block_table, ctx, refs):
+    if block_table.dim() != 2 or refs.dim() != 1:
+        raise ValueError(f"{what}: block_table [S, max_pages] and refs [num_pages] wanted")
+    dev = block_table.device
+    _tensor(block_table, f"{what}: block_table", torch.int32)
+    if ctx is not None:
+        _tensor(ctx, f"{what}: ctx", torch.int32, (block_table.shape[0],), dev)
+    _tensor(refs, f"{what}: refs", torch.int32, None, dev)
+    return block_table.shape[0], block_table.shape[1], refs.shape[0], dev
+
+
+def kv_truncate(block_table, ctx, refs, page: int, new_len) -> None:
+    """Shorten (0: free) the sequences to new_len [S] positions, in place; negative: leave alone."""
+    S, width, pages, dev = _state("kv_truncate", block_table, ctx, refs)
+    _tensor(new_len, "kv_truncate: new_len", torch.int32, (S,), dev)
+    _call(lib().q8op_kv_truncate, dev, block_table.data_ptr(), S, width, ctx.data_ptr(), refs.data_ptr(), pages,
+          page, new_len.data_ptr())
+
+
+def kv_fork(block_table, ctx, refs, page: int, src, dst) -> None:
+    """Sequences dst [n] become sequences src [n] as they were before the call, sharing their pages."""
+    S, width, pages, dev = _state("kv_fork", block_table, ctx, refs)
+    n = src.numel()
+    _tensor(src, "kv_fork: src", torch.int32, (n,), dev)
+    _tensor(dst, "kv_fork: dst", torch.int32, (n,), dev)
+    _call(lib().q8op_kv_fork, dev, block_table.data_ptr(), S, width, ctx.data_ptr(), refs.data_ptr(), pages, page,
+          src.data_ptr(), dst.data_ptr(), n)
+
+
+def kv_reserve(block_table, ctx, refs, page: int, n_new):
+    """Make room for n_new [S] more positions, in place; ctx grows by them.  Returns (src, dst,
+    status): the page copies to make before writing (kv_copy_pages), and [0 or Q8_ERR_KV_FULL,
+    pages wanted, pages free], all on the device.  When the pool is too small nothing changes."""
+    S, width, pages, dev = _state("kv_reserve", block_table, ctx, refs)
+    _tensor(n_new, "kv_reserve: n_new", torch.int32, (S,), dev)
+    got = torch.empty(2 * S + 3 + pages, dtype=torch.int32, device=dev)  # src, dst, status, scratch
+    at = got.data_ptr()
+    _call(lib().q8op_kv_reserve, dev, block_table.data_ptr(), S, width, ctx.data_ptr(), refs.data_ptr(), pages, page,
+          n_new.data_ptr(), at, at + 4 * S, at + 8 * S, at + 8 * S + 12)
+    return got[:S], got[S:2 * S], got[2 * S:2 * S + 3]
+
+
+def kv_compact(block_table, refs):
+    """Renumber the pages so that those in use come first, in place.  Returns (src, dst)
+    [num_pages / 2], the page copies to make (kv_copy_pages), -1 behind the last."""
+    S, width, pages, dev = _state("kv_compact", block_table, None, refs)
+    half = pages // 2
+    got = torch.empty(2 * half + pages, dtype=torch.int32, device=dev)
+    at = got.data_ptr()
+    _call(lib().q8op_kv_compact, dev, block_table.data_ptr(), S, width, refs.data_ptr(), pages, at, at + 4 * half,
+          at + 8 * half)
+    return got[:half], got[half:2 * half]
+
+
+def kv_copy_pages(pools, src, dst) -> None:
+    """pool[dst[i]] = pool[src[i]] in every pool (contiguous, pages first); pairs with a
+    negative number are left out, and so are pairs whose result would depend on the order."""
+    if not pools:
+        return
+    dev, num_pages = pools[0].device, pools[0].shape[0]
+    n = src.numel()
+    _tensor(src, "kv_copy_pages: src", torch.int32, (n,), dev)
+    _tensor(dst, "kv_copy_pages: dst", torch.int32, (n,), dev)
+    for t in pools:
+        _tensor(t, "kv_copy_pages: pool", t.dtype, None, dev)
+        if t.dim() < 2 or t.shape[0] != num_pages or t.numel() == 0:
+            raise ValueError("kv_copy_pages: pools of the same number of pages wanted")
+    for at in range(0, len(pools), 64):
+        part = pools[at:at + 64]
+        k = len(part)
+        _call(lib().q8op_kv_copy_pages, dev, (C.c_void_p * k)(*[t.data_ptr() for t in part]),
+              (C.c_int64 * k)(*[t.numel() // num_pages * t.element_size() for t in part]), k, num_pages,
+              src.data_ptr(), dst.data_ptr(), n)
+
+
+# ------------------------------------------------------------------ speculative decoding
+def _matrix(t, what, dev=None):
+    """f32 [rows, n] with contiguous columns: (rows, n, row stride)."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError(f"{what}: libq8cuda ops take CUDA tensors")
+    if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] == 0 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"{what}: f32 [rows, n] with contiguous columns wanted")
+    if dev is not None and t.device != dev:
+        raise ValueError(f"{what}: is on {t.device}, other tensors of the call on {dev}")
+    rows, n = t.shape
+    return rows, n, t.stride(0) if rows > 1 else max(t.stride(0), n)
+
+
+def probs(logits: torch.Tensor, temp: float, out: torch.Tensor = None) -> torch.Tensor:
+    """The distributions that sampling at ``temp`` and top_p = 1 draws from (q8op_probs)."""
+    rows, n, ld = _matrix(logits, "probs: logits")
+    dev = logits.device
+    if out is None:
+        out = torch.empty((rows, n), device=dev)
+    ro, no, ldo = _matrix(out, "probs: out", dev)
+    if (ro, no) != (rows, n):
+        raise ValueError("probs: out must have the shape of logits")
+    _call(lib().q8op_probs, dev, logits.data_ptr(), rows, n, ld, temp, out.data_ptr(), ldo)
+    return out
+
+
+def verify(p, q, ids, seq_start, u):
+    """Verify drafted tokens against the target's distributions p [T, n] (q8op_verify): q is the
+    drafts' [drafts, n] or None (certain drafts), ids [T] the tokens fed, u [T] uniform draws.
+    Returns (n_accepted [S], tokens [T]: kept drafts, the next token, -1)."""
+    rows, n, ldp = _matrix(p, "verify: p")
+    dev = p.device
+    S = seq_start.numel() - 1
+    if S < 0:
+        raise ValueError("verify: seq_start [S + 1] wanted")
+    _tensor(seq_start, "verify: seq_start", torch.int32, (S + 1,), dev)
+    _tensor(ids, "verify: ids", torch.int32, (rows,), dev)
+    _tensor(u, "verify: u", torch.float32, (rows,), dev)
+    q_rows, ldq, qp = 0, 0, None
+    if q is not None:
+        if q.shape[0] == 0:  # no row has a draft
+            ldq, qp = n, p.data_ptr()
+        else:
+            q_rows, nq, ldq = _matrix(q, "verify: q", dev)
+            if nq != n:
+                raise ValueError("verify: q must have p's columns")
+            qp = q.data_ptr()
+    n_accepted = torch.empty(S, dtype=torch.int32, device=dev)
+    tokens = torch.empty(rows, dtype=torch.int32, device=dev)
+    _call(lib().q8op_verify, dev, p.data_ptr(), ldp, qp, ldq, q_rows, ids.data_ptr(), seq_start.data_ptr(), rows, S,
+          n, u.data_ptr(), n_accepted.data_ptr(), tokens.data_ptr())
+    return n_accepted, tokens
 
 
 def device_status() -> None:
