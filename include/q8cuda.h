@@ -218,7 +218,7 @@ int q8op_sample(const float* logits, int64_t rows, int64_t n, int64_t ld, float 
  * [num_pages, n_kv, page, head_dim] and one f32 scale per Q8_KV8_BLOCK
  * consecutive tokens of a kv head, [num_pages, n_kv, page / Q8_KV8_BLOCK], for
  * k and for v; the value is code * scale.  page is a multiple of
- * Q8_KV8_BLOCK, head_dim 64 or 128, the code arrays 16-byte aligned.
+ * Q8_KV8_BLOCK, head_dim 64 or 128, the code arrays 32-byte aligned.
  *
  * The rows of a call are packed: rows seq_start[b] .. seq_start[b + 1] - 1
  * belong to sequence b (seq_start [S + 1], not decreasing) and are its last
@@ -228,8 +228,8 @@ int q8op_sample(const float* logits, int64_t rows, int64_t n, int64_t ld, float 
  * position 0 have no position.  block_table [S, max_pages] int32 holds the
  * page of each `page` positions; an entry outside [0, num_pages), or a position
  * past the table, is a page that is not there.  All of these are device
- * memory.  Nothing is allocated and no scratch is shared: calls on different
- * streams are independent as long as their tensors are. */
+ * memory.  Nothing is allocated and no scratch is shared inside the library:
+ * calls on different streams are independent as long as their tensors are. */
 #define Q8_KV8_BLOCK 16
 typedef struct q8_kv8_pages {
   int8_t* k;
@@ -264,10 +264,13 @@ int q8op_kv8_read(const q8_kv8_pages* kv, const int32_t* seq_start, const int32_
  * row attends to the positions 0 .. its own of its sequence; positions whose
  * page is not there are masked (pages freed behind a window, say), and a row
  * that sees no position gives zeros.  Scores, softmax statistics and sums are
- * f32. */
+ * f32.  work: device scratch of q8op_kv8_attention_workspace() bytes, 16-byte
+ * aligned (NULL where that is 0); calls that overlap need a scratch each. */
+size_t q8op_kv8_attention_workspace(int dtype, int64_t rows, int64_t S, int n_heads, int n_kv, int head_dim);
 int q8op_kv8_attention(const void* q, int64_t ldq, int dtype, int64_t rows, const int32_t* seq_start,
                        const int32_t* ctx, int64_t S, int n_heads, const q8_kv8_pages* kv,
-                       const int32_t* block_table, int max_pages, void* out, int64_t ldo, void* stream);
+                       const int32_t* block_table, int max_pages, void* out, int64_t ldo, void* work,
+                       size_t work_bytes, void* stream);
 
 /* ---------------------------------------------------- page tables, op level
  * Device-side state of a paged cache of either kind (the reference has one

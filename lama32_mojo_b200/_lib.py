@@ -73,7 +73,8 @@ SIGNATURES = {
     "q8op_sample": [_P, _I64, _I64, _I64, _F, _F, _P, _P, _P],
     "q8op_kv8_append": [_P, _I64, _P, _I64, _I32, _I64, _P, _P, _I64, _P, _P, _I32, _P],
     "q8op_kv8_read": [_P, _P, _P, _I64, _P, _I32, _P, _P, _I64, _P],
-    "q8op_kv8_attention": [_P, _I64, _I32, _I64, _P, _P, _I64, _I32, _P, _P, _I32, _P, _I64, _P],
+    "q8op_kv8_attention": [_P, _I64, _I32, _I64, _P, _P, _I64, _I32, _P, _P, _I32, _P, _I64, _P, C.c_size_t, _P],
+    "q8op_kv8_attention_workspace": [_I32, _I64, _I64, _I32, _I32, _I32],
     "q8op_kv_truncate": [_P, _I64, _I32, _P, _P, _I64, _I32, _P, _P],
     "q8op_kv_fork": [_P, _I64, _I32, _P, _P, _I64, _I32, _P, _P, _I64, _P],
     "q8op_kv_reserve": [_P, _I64, _I32, _P, _P, _I64, _I32, _P, _P, _P, _P, _P, _P],
@@ -101,7 +102,8 @@ SIGNATURES = {
     "q8_profile": [_P, _I32, C.POINTER(C.c_char_p), C.POINTER(C.c_double), C.POINTER(C.c_double),
                    C.POINTER(_I32), C.POINTER(_I32)],
 }
-_RESTYPE = {"q8_last_error": C.c_char_p, "q8_status_string": C.c_char_p, "q8_version": C.c_char_p}
+_RESTYPE = {"q8_last_error": C.c_char_p, "q8_status_string": C.c_char_p, "q8_version": C.c_char_p,
+            "q8op_kv8_attention_workspace": C.c_size_t}
 
 _lib = None
 

@@ -18,7 +18,9 @@ int kv8_check(const char* what, const q8_kv8_pages* kv, const int32_t* seq_start
                "%s: page size %d is not a multiple of %d", what, kv->page, KV8_BLOCK);
   Q8_CHECK_ARG(kv->num_pages > 0 && kv->num_pages < ((int64_t)1 << 31) && kv->n_kv > 0 && kv->n_kv <= 65535,
                "%s: bad pages (%lld pages, %d kv heads)", what, (long long)kv->num_pages, kv->n_kv);
-  Q8_CHECK_ARG((((uintptr_t)kv->k | (uintptr_t)kv->v) & 15) == 0, "%s: codes must be 16-byte aligned", what);
+  Q8_CHECK_ARG(kv->num_pages * kv->n_kv * (kv->page / KV8_BLOCK) < ((int64_t)1 << 31), "%s: 2^31 blocks or more",
+               what);
+  Q8_CHECK_ARG((((uintptr_t)kv->k | (uintptr_t)kv->v) & 31) == 0, "%s: codes must be 32-byte aligned", what);
   Q8_CHECK_ARG(S >= 0 && S <= (1 << 20) && rows >= 0 && rows <= (1 << 24) && max_pages > 0,
                "%s: bad shape (%lld sequences, %lld rows, %d table columns)", what, (long long)S, (long long)rows,
                max_pages);

@@ -12,6 +12,11 @@ sum_d |q_d k_jd| / sqrt(hd) of the row,
     that moves every p by the factor exp(+-smag E'), so o by 2 smag E' mag;
   * p is kept in two 11-bit halves (f32 rows) or one (16-bit rows, 2^-11), the
     sums are f32 over at most a few hundred steps: 2^-18 mag covers them;
+  * the weights p_j sv_j are f16 numbers lifted so that the largest lies just
+    below 2^15; the f16 grid is never finer than 2^-24, so each is off by up to
+    2^-25 / 2^14 = 2^-39 of the largest, however small it is, times a code of at
+    most 127: positions * 2^-39 * 127 * max_j p_j sv_j.  (mag does not cover this
+    where the positions that carry the weight have the code 0.)
   * the result is rounded to its type: eps / 2 of its value.
 """
 import math
@@ -81,6 +86,13 @@ class HostCache:
             assert np.array_equal(a, t.cpu().numpy())
         for a, t in zip(self.s, (pages.k_scale, pages.v_scale)):
             assert np.array_equal(a, t.cpu().numpy())
+
+    def scale_of(self, which, table_row, upto, h):
+        """f64 [upto]: the scale of each position of a kv head (0: no page)."""
+        j = [table_row[p // self.page] if p // self.page < len(table_row) else -1 for p in range(upto)]
+        n = self.c[0].shape[0]
+        return np.array([float(self.s[which][e, h, p % self.page // B]) if 0 <= e < n else 0.0
+                         for p, e in enumerate(j)])
 
     def values(self, which, table_row, upto):
         """f64 [upto, kv, hd] and which positions have a page."""
@@ -257,7 +269,8 @@ def reference(host, q, ns, ctx, table, heads):
                     mag = p @ np.abs(v)
                     E = 2.0 ** -21 + (hd // 16 + 3 + 2) * 2.0 ** -23
                     out[t + i, h] = p @ v
-                    tol[t + i, h] = mag * (2 * smag * E + 2.0 ** -18)
+                    wmax = (p * host.scale_of(1, table[b], e, h // G)[see]).max()
+                    tol[t + i, h] = mag * (2 * smag * E + 2.0 ** -18) + len(p) * 127 * 2.0 ** -39 * wmax
                     tol16 = mag * 2.0 ** -11
                     reference.tol16[t + i, h] = tol16
         t += n

@@ -28,7 +28,7 @@ def test_kv8_entries_refuse():
         return L.q8op_kv8_append(k, ld, k, ld, dtype, rows, starts, ctx, S, kv or pages(), table, width, None)
 
     def attend(q=ONE, ld=256, dtype=0, rows=1, heads=4, kv=None, width=1, out=ONE, S=1):
-        return L.q8op_kv8_attention(q, ld, dtype, rows, ONE, ONE, S, heads, kv or pages(), ONE, width, out, ld, None)
+        return L.q8op_kv8_attention(q, ld, dtype, rows, ONE, ONE, S, heads, kv or pages(), ONE, width, out, ld, ONE, 1 << 30, None)
 
     refused(append(k=None), "rows need")
     refused(append(ld=127), "rows need")
