@@ -254,8 +254,8 @@ int q8op_kv8_append(const void* k, int64_t ldk, const void* v, int64_t ldv, int 
                     const int32_t* block_table, int max_pages, void* stream);
 
 /* The cached values of the rows' positions as f32 [rows, n_kv, head_dim]
- * (the inverse of the append, as q8op_dequant is of q8op_pack).  Rows without
- * a page or a position read as zeros. */
+ * (the inverse of the append, as q8op_dequant is of q8op_pack), k and v 16-byte
+ * aligned.  Rows without a page or a position read as zeros. */
 int q8op_kv8_read(const q8_kv8_pages* kv, const int32_t* seq_start, const int32_t* ctx, int64_t S,
                   const int32_t* block_table, int max_pages, float* k, float* v, int64_t rows, void* stream);
 

@@ -4,6 +4,7 @@
 #include "q8_kv8.cuh"
 
 #include <math.h>
+#include <type_traits>
 
 namespace q8 {
 
@@ -28,25 +29,26 @@ int kv8_check(const char* what, const q8_kv8_pages* kv, const int32_t* seq_start
 }
 
 // round(x / s), ties to even, within +-127: the quotient of the real numbers,
-// not of their f32 rounding.  r - |x - r s| stays exact: x - r s is a multiple
-// of the smaller ulp of x and s and at most about s, so the FMA does not round.
-// s > 0; x finite.
+// not of their f32 rounding.  The estimate r is off by one at most, next to a
+// tie; x - r s is exact there: a multiple of the smaller ulp of x and s and at
+// most about s / 2.  s > 0; an infinite x gives +-127.
 __device__ __forceinline__ int kv8_code(float x, float s) {
   float r = rintf(__fdiv_rn(x, s));
-  if (!(fabsf(r) <= 127.f)) return x < 0.f ? -127 : 127;  // a scale below the normal range
-  const float d = fmaf(-r, s, x);
-  const float two = 2.f * fabsf(d);
-  if (two > s || (two == s && ((int)r & 1))) r += d > 0.f ? 1.f : -1.f;
-  return max(-127, min(127, (int)r));
+  const float d = fmaf(-r, s, x), two = fabsf(d) * 2.f;
+  if (two >= s && (two > s || ((int)r & 1))) r += d > 0.f ? 1.f : -1.f;
+  return (int)fminf(fmaxf(r, -127.f), 127.f);
 }
 
-// round(c s0 / s1) for a code that stays while its block's scale grows; the
-// products fit 64-bit floats exactly.
-__device__ __forceinline__ int kv8_rescale(int c, float s0, float s1) {
-  int r = (int)rintf((float)c * __fdiv_rn(s0, s1));
-  const double d = (double)c * (double)s0 - (double)r * (double)s1;
-  const double two = 2.0 * fabs(d);
-  if (two > (double)s1 || (two == (double)s1 && (r & 1))) r += d > 0.0 ? 1 : -1;
+// round(c s0 / s1), ties to even, for a code that stays while its block's scale
+// grows; ratio = s0 / s1 rounded.  c ratio is off by less than 127 2^-23, so
+// only next to a tie the exact products (64 bits hold them) have to decide.
+__device__ __forceinline__ int kv8_rescale(int c, float ratio, float s0, float s1) {
+  const float y = (float)c * ratio;
+  int r = __float2int_rn(y);
+  if (fabsf(fabsf(y - (float)r) - 0.5f) < 0x1p-14f) {
+    const double d = (double)c * (double)s0 - (double)r * (double)s1, two = 2.0 * fabs(d);
+    if (two > (double)s1 || (two == (double)s1 && (r & 1))) r += d > 0.0 ? 1 : -1;
+  }
   return r;
 }
 
@@ -54,26 +56,60 @@ __device__ __forceinline__ int kv8_rescale(int c, float s0, float s1) {
 struct Kv8Rows {
   const void* x;
   int64_t ld;
+  bool aligned;  // to 16 bytes
 };
 
-// One warp per (block of 16 positions, kv head, k or v); lane l holds dims
-// l*HD/32 .. of every new token of the block.  Slots number the touched
-// blocks: sequence b's start at starts[b]/16 + 2b, which leaves room for the
-// n/16 + 2 blocks that n rows can touch.
+__device__ __forceinline__ float kv8_f32(float x) { return x; }
+__device__ __forceinline__ float kv8_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float kv8_f32(__half x) { return __half2float(x); }
+
+// the larger of top and |w|, by pairs for 16-bit elements; NaN is the largest
+template <typename T>
+__device__ __forceinline__ unsigned kv8_max(unsigned top, unsigned w) {
+  if constexpr (sizeof(T) == 4) {
+    return max(top, w & 0x7fffffffu);
+  } else {
+    typedef typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type T2;
+    w &= 0x7fff7fffu;
+    const T2 m = __hmax2_nan(*reinterpret_cast<T2*>(&top), *reinterpret_cast<T2*>(&w));
+    return *reinterpret_cast<const unsigned*>(&m);
+  }
+}
+
+// two floats in a register pair, and their packed fused multiply-add
+__device__ __forceinline__ uint64_t kv8_two(float a, float b) {
+  return (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a);
+}
+__device__ __forceinline__ uint64_t kv8_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+
+// One warp per (block of 16 positions, kv head, k or v).  A lane takes 16 bytes
+// of a row, the warp as many rows as fit; the rows are read twice, for the
+// scale and for the codes (the second time from the caches), which takes half
+// the registers of keeping them and leaves room for twice the warps.  Slots
+// number the touched blocks: sequence b's start at starts[b]/16 + 2b, which
+// leaves room for the n/16 + 2 blocks that n rows can touch.  Bytes: the rows
+// once, a quarter or half of that in codes.
+//
+// Codes, two at a time in packed f32 operations: m = fma(x, 1/s, 1.5 2^23) rounds to the whole number nearest to the
+// estimated quotient and holds it in its low byte; r = m - 1.5 2^23.  The
+// estimate is 2 ulps off at most, so r is right, or by one off next to a tie;
+// d = x - r s, which is exact, tells: r moves towards x where |d| > s / 2, or
+// where it is s / 2 and r odd (m's last bit).  Blocks with numbers that are not
+// finite, or scales far outside the usual ones, go the long way (kv8_code).
 template <typename T, int HD>
-__global__ void __launch_bounds__(256) k_kv8_append(Kv8Rows kr, Kv8Rows vr, int rows, const int32_t* __restrict__ starts,
-                                                    const int32_t* __restrict__ ctx, int S, q8_kv8_pages kv,
-                                                    const int32_t* __restrict__ table, int max_pages) {
-  constexpr int E = HD / 32;
-  const int slot = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int before = 0;
-  for (int b = threadIdx.x; b < S; b += blockDim.x) before += min(max(starts[b], 0), rows) / KV8_BLOCK + 2 * b <= slot;
-  __shared__ int s_cnt;
-  if (threadIdx.x == 0) s_cnt = 0;
-  __syncthreads();
-  if (before) atomicAdd(&s_cnt, before);
-  __syncthreads();
-  const int b = s_cnt - 1;
+__global__ void __launch_bounds__(128, 10) k_kv8_append(Kv8Rows kr, Kv8Rows vr, int rows,
+                                                        const int32_t* __restrict__ starts,
+                                                        const int32_t* __restrict__ ctx, int S, q8_kv8_pages kv,
+                                                        const int32_t* __restrict__ table, int max_pages) {
+  constexpr int E = 16 / sizeof(T), LPR = HD / E, RPI = 32 / LPR;
+  const int slot = blockIdx.x, lane = threadIdx.x & 31;
+  const int unit = blockIdx.y * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (unit >= 2 * kv.n_kv) return;
+  const int b = kv8_find_warp(starts, S, rows, KV8_BLOCK, 2, slot);
   if (b < 0) return;
   const Kv8Seq sq = kv8_seq(starts, ctx, b, rows);
   if (sq.n <= 0) return;
@@ -82,101 +118,164 @@ __global__ void __launch_bounds__(256) k_kv8_append(Kv8Rows kr, Kv8Rows vr, int 
   const int64_t lo = max(blk * KV8_BLOCK, first);
   const int64_t hi = min((blk + 1) * KV8_BLOCK, sq.pos0 + sq.n);
   if (lo >= hi) return;
-  const int pg = kv8_page(table + (int64_t)b * max_pages, max_pages, kv.num_pages, kv.page, lo);
-  if (pg < 0) return;
   const int in = (int)(lo % KV8_BLOCK), cnt = (int)(hi - lo);
   const int row = sq.row0 + (int)(lo - sq.pos0);
-  const int unit = blockIdx.y * (blockDim.x >> 5) + warp;
-  if (unit >= 2 * kv.n_kv) return;
-  const int h = unit >> 1;
+  const int h = unit >> 1, tk = lane / LPR, el = (lane % LPR) * E;
   const bool isv = unit & 1;
   const Kv8Rows src = isv ? vr : kr;
-  const int64_t cell = (int64_t)pg * kv.n_kv + h;
-  const int tok0 = (int)((blk * KV8_BLOCK) % kv.page);
-  int8_t* codes = (isv ? kv.v : kv.k) + (cell * kv.page + tok0) * HD + lane * E;
-  float* scale = (isv ? kv.v_scale : kv.k_scale) + cell * (kv.page / KV8_BLOCK) + tok0 / KV8_BLOCK;
-  const T* x = (const T*)src.x + (int64_t)row * src.ld + h * HD + lane * E;
-  float v[KV8_BLOCK][E];
-  float high = 0.f;
+  const T* x = (const T*)src.x + (int64_t)row * src.ld + h * HD + el;
+  union Piece {
+    uint4 w;
+    uint32_t u[4];
+    T e[E];
+    __device__ Piece() {}
+  };
+  auto load = [&](Piece& v, int t) {
+    if (src.aligned) {
+      v.w = *reinterpret_cast<const uint4*>(x + (int64_t)t * src.ld);
+    } else {
 #pragma unroll
-  for (int i = 0; i < KV8_BLOCK; ++i) {
-#pragma unroll
-    for (int e = 0; e < E; ++e) v[i][e] = i < cnt ? kv8_load(x + (int64_t)i * src.ld + e) : 0.f;
-  }
-#pragma unroll
-  for (int i = 0; i < KV8_BLOCK; ++i)
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      if (v[i][e] != v[i][e]) v[i][e] = 0.f;  // NaN
-      const float a = fabsf(v[i][e]);
-      if (a != INFINITY) high = fmaxf(high, a);
+      for (int e = 0; e < E; ++e) v.e[e] = x[(int64_t)t * src.ld + e];
     }
-  high = warp_max(high);
+  };
+  const int pg = kv8_page(table + (int64_t)b * max_pages, max_pages, kv.num_pages, kv.page, lo);
+  if (pg < 0) return;
+  const int64_t cell = (int64_t)pg * kv.n_kv + h;
+  const int tok0 = (int)((uint32_t)(blk * KV8_BLOCK) % (uint32_t)kv.page);
+  int8_t* codes = (isv ? kv.v : kv.k) + (cell * kv.page + tok0) * HD + el;
+  float* scale = (isv ? kv.v_scale : kv.k_scale) + cell * (kv.page / KV8_BLOCK) + tok0 / KV8_BLOCK;
   const float old = in > 0 ? *scale : 0.f;
-  const float s = fmaxf(old, __fdiv_rn(high, 127.f));
-  __syncwarp();
-  if (s != old && in > 0) {
-    for (int i = 0; i < in; ++i)
+  // the largest |x| by its bits, which order as the numbers do; non-finite ones lie above
+  unsigned top = 0u;
+#pragma unroll 4
+  for (int t = tk; t < cnt; t += RPI) {
+    Piece v;
+    load(v, t);
 #pragma unroll
-      for (int e = 0; e < E; ++e)
-        codes[i * HD + e] = old > 0.f ? (int8_t)kv8_rescale(codes[i * HD + e], old, s) : (int8_t)0;
+    for (int e = 0; e < 4; ++e)
+      top = kv8_max<T>(top, v.u[e]);
+  }
+  if (sizeof(T) == 2) {
+    const unsigned short bits = (unsigned short)max(top & 0xffffu, top >> 16);
+    top = __float_as_uint(kv8_f32(*reinterpret_cast<const T*>(&bits)));
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  const bool finite = top < 0x7f800000u;
+  if (!finite) {  // NaN counts as 0, and infinities do not enter the scale
+    top = 0u;
+#pragma unroll 1
+    for (int t = tk; t < cnt; t += RPI)
+#pragma unroll 1
+      for (int e = 0; e < E; ++e) {
+        const unsigned a = __float_as_uint(kv8_f32(x[(int64_t)t * src.ld + e])) & 0x7fffffffu;
+        if (a < 0x7f800000u) top = max(top, a);
+      }
+    top = __reduce_max_sync(0xffffffffu, top);
+  }
+  const float s = fmaxf(old, __fdiv_rn(__uint_as_float(top), 127.f));
+  union Codes {
+    int8_t c[E];
+    typename std::conditional<E == 8, uint2, uint32_t>::type w;
+  };
+  using Word = decltype(Codes::w);
+  if (s != old && in > 0) {
+    const float ratio = __fdiv_rn(old, s);
+#pragma unroll 4
+    for (int t = tk; t < in; t += RPI) {
+      Codes k;
+      k.w = *reinterpret_cast<const Word*>(codes + t * HD);
+#pragma unroll
+      for (int e = 0; e < E; ++e) k.c[e] = (int8_t)kv8_rescale(k.c[e], ratio, old, s);
+      *reinterpret_cast<Word*>(codes + t * HD) = k.w;
+    }
   }
   if (lane == 0) *scale = s;
+  const bool plain = finite && s > 0x1p-100f && s < 0x1p100f;
+  if (!plain) {
+#pragma unroll 1
+    for (int t = tk; t < cnt; t += RPI)
+#pragma unroll 1
+      for (int e = 0; e < E; ++e) {
+        const float a = kv8_f32(x[(int64_t)t * src.ld + e]);
+        int c = 0;
+        if (a == a) c = s > 0.f ? kv8_code(a, s) : fabsf(a) == INFINITY ? (a < 0.f ? -127 : 127) : 0;
+        codes[(in + t) * HD + e] = (int8_t)c;
+      }
+    return;
+  }
+  const float inv = 1.f / s;
+  const int half_up = __float_as_int(s * 0.5f) + 1;  // the next number above s / 2
+  const uint64_t inv2 = kv8_two(inv, inv), s2 = kv8_two(s, s), magic = kv8_two(12582912.f, 12582912.f),
+                 minus = kv8_two(-1.f, -1.f);
+#pragma unroll 2
+  for (int t = tk; t < cnt; t += RPI) {
+    Piece v;
+    load(v, t);
+    uint32_t w[E / 4];
 #pragma unroll
-  for (int i = 0; i < KV8_BLOCK; ++i) {
-    if (i >= cnt) break;
+    for (int e = 0; e < E; e += 4) {
+      uint32_t c[4];
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const float a = v[i][e];
-      int c = 0;
-      if (fabsf(a) == INFINITY) c = a < 0.f ? -127 : 127;
-      else if (s > 0.f) c = kv8_code(a, s);
-      codes[(in + i) * HD + e] = (int8_t)c;
+      for (int j = 0; j < 4; j += 2) {
+        const uint64_t a = kv8_two(kv8_f32(v.e[e + j]), kv8_f32(v.e[e + j + 1]));
+        const uint64_t m = kv8_fma2(a, inv2, magic), d = kv8_fma2(kv8_fma2(m, minus, magic), s2, a);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float di = __uint_as_float((uint32_t)(d >> (32 * i)));
+          float mi = __uint_as_float((uint32_t)(m >> (32 * i)));
+          const float edge = __int_as_float(half_up - (__float_as_int(mi) & 1));
+          if (fabsf(di) >= edge) mi += copysignf(1.f, di);
+          c[j + i] = __float_as_uint(mi);
+        }
+      }
+      w[e / 4] = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
     }
+    if constexpr (E == 8) *reinterpret_cast<uint2*>(codes + (in + t) * HD) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint32_t*>(codes + (in + t) * HD) = w[0];
   }
 }
 
-// One CTA per row of the call; rows without a page read as zeros.
+// One warp per row of the call; rows without a page read as zeros.
 template <int HD>
 __global__ void __launch_bounds__(256) k_kv8_read(int rows, const int32_t* __restrict__ starts,
                                                   const int32_t* __restrict__ ctx, int S, q8_kv8_pages kv,
                                                   const int32_t* __restrict__ table, int max_pages,
                                                   float* __restrict__ ko, float* __restrict__ vo) {
-  const int t = blockIdx.x;
-  int before = 0;
-  for (int b = threadIdx.x; b < S; b += blockDim.x) before += min(max(starts[b], 0), rows) <= t;
-  __shared__ int s_cnt;
-  if (threadIdx.x == 0) s_cnt = 0;
-  __syncthreads();
-  if (before) atomicAdd(&s_cnt, before);
-  __syncthreads();
-  const int b = s_cnt - 1;
+  const int t = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (t >= rows) return;
+  const int b = kv8_find_warp(starts, S, rows, 1, 0, t);
   if (b < 0) return;
   const Kv8Seq sq = kv8_seq(starts, ctx, b, rows);
   if (t >= sq.row0 + sq.n) return;  // behind the last sequence
   const int64_t p = sq.pos0 + (t - sq.row0);
   const int pg = kv8_page(table + (int64_t)b * max_pages, max_pages, kv.num_pages, kv.page, p);
-  const int tok = pg < 0 ? 0 : (int)(p % kv.page);
-  for (int i = threadIdx.x; i < 2 * kv.n_kv * HD; i += blockDim.x) {
-    const bool isv = i >= kv.n_kv * HD;
-    const int j = isv ? i - kv.n_kv * HD : i;
-    const int h = j / HD, d = j % HD;
-    float r = 0.f;
+  const int tok = pg < 0 ? 0 : (int)((uint32_t)p % (uint32_t)kv.page);
+  const int64_t cell = (int64_t)max(pg, 0) * kv.n_kv, step = (int64_t)kv.page * HD;
+  const int64_t code0 = cell * step + (int64_t)tok * HD, scale0 = cell * (kv.page / KV8_BLOCK) + tok / KV8_BLOCK;
+  const int64_t o0 = (int64_t)t * kv.n_kv * HD;
+#pragma unroll 4
+  for (int i = lane * 4; i < kv.n_kv * HD; i += 128) {
+    const int h = i / HD, d = i % HD;
+    float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
     if (pg >= 0) {
-      const int64_t cell = (int64_t)pg * kv.n_kv + h;
-      r = (float)(isv ? kv.v : kv.k)[(cell * kv.page + tok) * HD + d] *
-          (isv ? kv.v_scale : kv.k_scale)[cell * (kv.page / KV8_BLOCK) + tok / KV8_BLOCK];
+      const int64_t at = code0 + h * step + d;
+      const char4 ck = *reinterpret_cast<const char4*>(kv.k + at), cv = *reinterpret_cast<const char4*>(kv.v + at);
+      const int64_t si = scale0 + (int64_t)h * (kv.page / KV8_BLOCK);
+      const float sk = kv.k_scale[si], sv = kv.v_scale[si];
+      k = make_float4(ck.x * sk, ck.y * sk, ck.z * sk, ck.w * sk);
+      v = make_float4(cv.x * sv, cv.y * sv, cv.z * sv, cv.w * sv);
     }
-    (isv ? vo : ko)[(int64_t)t * kv.n_kv * HD + j] = r;
+    *reinterpret_cast<float4*>(ko + o0 + i) = k;
+    *reinterpret_cast<float4*>(vo + o0 + i) = v;
   }
 }
 
 template <typename T>
 static int append_run(const Kv8Rows& k, const Kv8Rows& v, int rows, const int32_t* starts, const int32_t* ctx, int S,
                       const q8_kv8_pages& kv, const int32_t* table, int max_pages, cudaStream_t st) {
-  const dim3 grid(rows / KV8_BLOCK + 2 * S, ceil_div(2 * kv.n_kv, 8));
-  if (kv.head_dim == 64) k_kv8_append<T, 64><<<grid, 256, 0, st>>>(k, v, rows, starts, ctx, S, kv, table, max_pages);
-  else k_kv8_append<T, 128><<<grid, 256, 0, st>>>(k, v, rows, starts, ctx, S, kv, table, max_pages);
+  const dim3 grid(rows / KV8_BLOCK + 2 * S, ceil_div(2 * kv.n_kv, 4));
+  if (kv.head_dim == 64) k_kv8_append<T, 64><<<grid, 128, 0, st>>>(k, v, rows, starts, ctx, S, kv, table, max_pages);
+  else k_kv8_append<T, 128><<<grid, 128, 0, st>>>(k, v, rows, starts, ctx, S, kv, table, max_pages);
   return launch_check("k_kv8_append");
 }
 
@@ -193,7 +292,9 @@ extern "C" int q8op_kv8_append(const void* k, int64_t ldk, const void* v, int64_
   const int64_t width = (int64_t)kv->n_kv * kv->head_dim;
   Q8_CHECK_ARG(k && v && ldk >= width && ldv >= width, "q8op_kv8_append: k and v rows need %lld elements",
                (long long)width);
-  const Kv8Rows kr{k, ldk}, vr{v, ldv};
+  const int64_t size = dtype == Q8_F32 ? 4 : 2;
+  const Kv8Rows kr{k, ldk, (((uintptr_t)k | (uintptr_t)(ldk * size)) & 15) == 0},
+      vr{v, ldv, (((uintptr_t)v | (uintptr_t)(ldv * size)) & 15) == 0};
   cudaStream_t st = (cudaStream_t)stream;
   if (dtype == Q8_F32)
     return append_run<float>(kr, vr, (int)rows, seq_start, ctx, (int)S, *kv, block_table, max_pages, st);
@@ -207,11 +308,11 @@ extern "C" int q8op_kv8_read(const q8_kv8_pages* kv, const int32_t* seq_start, c
                              void* stream) {
   Q8_TRY(kv8_check("q8op_kv8_read", kv, seq_start, ctx, S, rows, block_table, max_pages));
   if (rows == 0 || S == 0) return Q8_OK;
-  Q8_CHECK_ARG(k && v, "q8op_kv8_read: null output");
+  Q8_CHECK_ARG(k && v && (((uintptr_t)k | (uintptr_t)v) & 15) == 0, "q8op_kv8_read: null or unaligned output");
   cudaStream_t st = (cudaStream_t)stream;
   if (kv->head_dim == 64)
-    k_kv8_read<64><<<(int)rows, 256, 0, st>>>((int)rows, seq_start, ctx, (int)S, *kv, block_table, max_pages, k, v);
+    k_kv8_read<64><<<ceil_div(rows, 8), 256, 0, st>>>((int)rows, seq_start, ctx, (int)S, *kv, block_table, max_pages, k, v);
   else
-    k_kv8_read<128><<<(int)rows, 256, 0, st>>>((int)rows, seq_start, ctx, (int)S, *kv, block_table, max_pages, k, v);
+    k_kv8_read<128><<<ceil_div(rows, 8), 256, 0, st>>>((int)rows, seq_start, ctx, (int)S, *kv, block_table, max_pages, k, v);
   return launch_check("k_kv8_read");
 }

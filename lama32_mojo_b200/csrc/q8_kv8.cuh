@@ -34,15 +34,19 @@ __device__ __forceinline__ Kv8Seq kv8_seq(const int32_t* starts, const int32_t* 
 // Page of position p, or -1.
 __device__ __forceinline__ int kv8_page(const int32_t* table_row, int max_pages, int64_t num_pages, int page,
                                         int64_t p) {
-  const int64_t j = p / page;
-  if (p < 0 || j >= max_pages) return -1;
+  if (p < 0) return -1;
+  const uint32_t j = (uint32_t)p / (uint32_t)page;  // a position is below ctx, an int32
+  if (j >= (uint32_t)max_pages) return -1;
   const int e = table_row[j];
   return e >= 0 && e < num_pages ? e : -1;
 }
 
-template <typename T>
-__device__ __forceinline__ float kv8_load(const T* p) {
-  return (float)*p;
+// Sequence of slot g, slots of sequence b starting at starts[b] / per + more b,
+// by one warp; -1: before the first.
+__device__ __forceinline__ int kv8_find_warp(const int32_t* starts, int S, int rows, int per, int more, int slot) {
+  int n = 0;
+  for (int b = threadIdx.x & 31; b < S; b += 32) n += min(max(starts[b], 0), rows) / per + more * b <= slot;
+  return __reduce_add_sync(0xffffffffu, n) - 1;
 }
 
 int kv8_check(const char* what, const q8_kv8_pages* kv, const int32_t* seq_start, const int32_t* ctx, int64_t S,

@@ -12,9 +12,19 @@
 // one of a hundred draws.
 #include "q8_kernels.h"
 
+#include <algorithm>
+#include <cooperative_groups.h>
 #include <math.h>
 
+namespace cg = cooperative_groups;
+
 namespace q8 {
+
+constexpr int VF_THREADS = 512;
+constexpr int VF_WARPS = VF_THREADS / 32;
+constexpr int VF_MAX_CLUSTER = 16;
+constexpr int VF_Q = 10;                           // four-logit pieces that a thread of k_probs holds
+constexpr int VF_SLICE = VF_THREADS * 4 * VF_Q;    // logits of a row per CTA, at most
 
 __device__ __forceinline__ void vf_best(float& bv, int& bi, float ov, int oi) {
   if (ov > bv || (ov == bv && oi < bi)) {
@@ -23,18 +33,82 @@ __device__ __forceinline__ void vf_best(float& bv, int& bi, float ov, int oi) {
   }
 }
 
-__global__ void __launch_bounds__(1024) k_probs(const float* __restrict__ logits, int n, int64_t ld, float temp,
-                                                float* __restrict__ out, int64_t ldo) {
-  __shared__ float s_v[32];
-  __shared__ int s_i[32];
-  __shared__ double s_d[32];
-  const float* x = logits + (int64_t)blockIdx.x * ld;
-  float* y = out + (int64_t)blockIdx.x * ldo;
+__device__ __forceinline__ uint32_t vf_map(const void* p, int rank) {
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ float vf_peer(const float* p, int rank) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(vf_map(p, rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ int vf_peer(const int* p, int rank) {
+  int v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(vf_map(p, rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ double vf_peer(const double* p, int rank) {
+  double v;
+  asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(vf_map(p, rank)) : "memory");
+  return v;
+}
+
+// Sum over the warp, the same order on every lane.
+__device__ __forceinline__ double vf_warp_sum(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// A cluster of CTAs per row, each with a slice of it in registers: logits are
+// read once and probabilities written once (8 bytes a logit), the maximum and
+// the sum are exchanged through distributed shared memory.
+//
+// (l - max) / temp log2(e) is taken as y + z, y the f32 product with c = ch + cl
+// and z what it lost, so that the exponent's rounding does not grow with it:
+// w = 2^y (1 + z ln 2).  Four weights are added in 32 bits, those sums in 64.
+__global__ void __launch_bounds__(VF_THREADS, 2) k_probs(const float* __restrict__ logits, int n, int64_t ld,
+                                                         float temp, float ch, float cl, float* __restrict__ out,
+                                                         int64_t ldo, int per) {
+  __shared__ float s_v[VF_WARPS], s_top;
+  __shared__ int s_i[VF_WARPS], s_arg;
+  __shared__ double s_d[VF_WARPS], s_sum;
+  const cg::cluster_group cluster = cg::this_cluster();
+  const int nc = cluster.num_blocks(), rank = cluster.block_rank(), row = blockIdx.x / nc;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int lo = min(n, rank * per), cnt = min(n, lo + per) - lo;
+  const float* src = logits + (int64_t)row * ld + lo;
+  float* dst = out + (int64_t)row * ldo + lo;
+  const int at = threadIdx.x * 4;  // piece k: at + k * 4 * VF_THREADS
+  const bool wide = ((uintptr_t)src & 15) == 0;
+  float v[VF_Q][4];
+#pragma unroll
+  for (int k = 0; k < VF_Q; ++k) {
+    const int i = at + k * 4 * VF_THREADS;
+    if (wide && i + 4 <= cnt) {
+      const float4 f = __ldcs(reinterpret_cast<const float4*>(src + i));
+      v[k][0] = f.x, v[k][1] = f.y, v[k][2] = f.z, v[k][3] = f.w;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[k][e] = i + e < cnt ? src[i + e] : -INFINITY;
+    }
+  }
+  const bool greedy = !(temp > 0.f);
   float bv = -INFINITY;
   int bi = 0x7fffffff;
-  for (int i = threadIdx.x; i < n; i += blockDim.x)
-    if (x[i] > -INFINITY) vf_best(bv, bi, x[i], i);
+#pragma unroll
+  for (int k = 0; k < VF_Q; ++k)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) bv = fmaxf(bv, v[k][e]);  // a NaN is passed over
+  if (greedy && bv > -INFINITY) {
+#pragma unroll
+    for (int k = VF_Q - 1; k >= 0; --k)
+#pragma unroll
+      for (int e = 3; e >= 0; --e)
+        if (v[k][e] == bv) bi = lo + at + k * 4 * VF_THREADS + e;
+  }
+#pragma unroll
   for (int o = 16; o > 0; o >>= 1)
     vf_best(bv, bi, __shfl_xor_sync(0xffffffffu, bv, o), __shfl_xor_sync(0xffffffffu, bi, o));
   if (lane == 0) {
@@ -42,56 +116,111 @@ __global__ void __launch_bounds__(1024) k_probs(const float* __restrict__ logits
     s_i[w] = bi;
   }
   __syncthreads();
-  for (int k = 0; k < 32; ++k) vf_best(bv, bi, s_v[k], s_i[k]);
-  if (bi == 0x7fffffff) bi = 0;  // nothing above -inf: as q8op_argmax
-  if (!(temp > 0.f) || bv == -INFINITY) {
-    for (int i = threadIdx.x; i < n; i += blockDim.x) y[i] = i == bi ? 1.f : 0.f;
+  if (w == 0) {
+    bv = lane < VF_WARPS ? s_v[lane] : -INFINITY;
+    bi = lane < VF_WARPS ? s_i[lane] : 0x7fffffff;
+#pragma unroll
+    for (int o = VF_WARPS / 2; o > 0; o >>= 1)
+      vf_best(bv, bi, __shfl_xor_sync(0xffffffffu, bv, o), __shfl_xor_sync(0xffffffffu, bi, o));
+    if (lane == 0) {
+      s_top = bv;
+      s_arg = bi;
+    }
+  }
+  cluster.sync();
+  bv = lane < nc ? vf_peer(&s_top, lane) : -INFINITY;
+  bi = lane < nc ? vf_peer(&s_arg, lane) : 0x7fffffff;
+#pragma unroll
+  for (int o = VF_MAX_CLUSTER / 2; o > 0; o >>= 1)
+    vf_best(bv, bi, __shfl_xor_sync(0xffffffffu, bv, o), __shfl_xor_sync(0xffffffffu, bi, o));
+  bv = __shfl_sync(0xffffffffu, bv, 0);
+  bi = __shfl_sync(0xffffffffu, bi, 0);
+  if (greedy || bv == -INFINITY) {
+    if (bi == 0x7fffffff) bi = 0;  // nothing above -inf: as q8op_argmax
+    for (int i = threadIdx.x; i < cnt; i += VF_THREADS) dst[i] = lo + i == bi ? 1.f : 0.f;
+    cluster.sync();
     return;
   }
   const float low = bv - 16.f;
-  auto weight = [&](float l) {
-    if (!(l >= low)) return 0.f;
-    return l == bv ? 1.f : expf((l - bv) / temp);
-  };
   double sum = 0.0;
-  for (int i = threadIdx.x; i < n; i += blockDim.x) sum += (double)weight(x[i]);
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+#pragma unroll
+  for (int k = 0; k < VF_Q; ++k) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float l = v[k][e], d = l == bv ? 0.f : l - bv;  // inf - inf is 0 here
+      const float y = d * ch, z = fmaf(d, cl, fmaf(d, ch, -y));
+      float p;
+      asm("ex2.approx.f32 %0, %1;" : "=f"(p) : "f"(y));
+      v[k][e] = l >= low && y > -160.f ? fmaf(p, z * 0.69314718f, p) : 0.f;  // below 2^-149; z is no number at -inf
+    }
+    sum += (double)((v[k][0] + v[k][1]) + (v[k][2] + v[k][3]));
+  }
+  sum = vf_warp_sum(sum);
   if (lane == 0) s_d[w] = sum;
   __syncthreads();
-  sum = 0.0;
-  for (int k = 0; k < 32; ++k) sum += s_d[k];
+  if (threadIdx.x == 0) {
+    sum = 0.0;
+    for (int k = 0; k < VF_WARPS; ++k) sum += s_d[k];
+    s_sum = sum;
+  }
+  cluster.sync();
+  sum = vf_warp_sum(lane < nc ? vf_peer(&s_sum, lane) : 0.0);
   const float inv = (float)(1.0 / sum);
-  for (int i = threadIdx.x; i < n; i += blockDim.x) y[i] = weight(x[i]) * inv;
+  const bool wide_out = ((uintptr_t)dst & 15) == 0;
+#pragma unroll
+  for (int k = 0; k < VF_Q; ++k) {
+    const int i = at + k * 4 * VF_THREADS;
+    if (wide_out && i + 4 <= cnt) {
+      __stcs(reinterpret_cast<float4*>(dst + i),
+             make_float4(v[k][0] * inv, v[k][1] * inv, v[k][2] * inv, v[k][3] * inv));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (i + e < cnt) dst[i + e] = v[k][e] * inv;
+    }
+  }
+  cluster.sync();  // nobody leaves while its sum is read
 }
 
-// One CTA per sequence.
-__global__ void __launch_bounds__(1024) k_verify(const float* __restrict__ p, int64_t ldp, const float* __restrict__ q,
-                                                 int64_t ldq, int q_rows, const int32_t* __restrict__ ids,
-                                                 const int32_t* __restrict__ starts, int rows, int S, int n,
-                                                 const float* __restrict__ u, int32_t* __restrict__ taken,
-                                                 int32_t* __restrict__ tokens) {
-  __shared__ double s_d[1024];
-  __shared__ int s_i[32];
-  __shared__ int s_stop, s_filled;
-  const int b = blockIdx.x, lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+// A cluster of CTAs per sequence; all of them find the refused row, then each
+// adds up a slice of its weights, in segments of 128 per warp, so that the
+// drawn index is found in one segment: p and q rows are read once.
+constexpr int VF_SEG = 128;
+
+__global__ void __launch_bounds__(VF_THREADS) k_verify(const float* __restrict__ p, int64_t ldp,
+                                                       const float* __restrict__ q, int64_t ldq, int q_rows,
+                                                       const int32_t* __restrict__ ids,
+                                                       const int32_t* __restrict__ starts, int rows, int n,
+                                                       const float* __restrict__ u, int32_t* __restrict__ taken,
+                                                       int32_t* __restrict__ tokens, int per) {
+  extern __shared__ double s_seg[];  // the slice's segments, in order
+  __shared__ double s_sum;
+  __shared__ int s_stop, s_filled, s_last;
+  const cg::cluster_group cluster = cg::this_cluster();
+  const int nc = cluster.num_blocks(), rank = cluster.block_rank(), b = blockIdx.x / nc;
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   const int r0 = min(max(starts[b], 0), rows), r1 = min(max(starts[b + 1], r0), rows);
   if (r1 <= r0) {
-    if (threadIdx.x == 0) taken[b] = 0;
+    if (rank == 0 && threadIdx.x == 0) taken[b] = 0;
     return;
   }
+  const float draw = u[r1 - 1];
   // q has no row for a sequence's last row: row r's is r - (sequences with rows before b)
   int filled = 0;
-  for (int k = threadIdx.x; k < b; k += blockDim.x)
-    filled += min(max(starts[k + 1], 0), rows) > min(max(starts[k], 0), rows);
+  if (q)
+    for (int k = threadIdx.x; k < b; k += VF_THREADS)
+      filled += min(max(starts[k + 1], 0), rows) > min(max(starts[k], 0), rows);
   if (threadIdx.x == 0) {
     s_stop = r1 - 1;
     s_filled = 0;
+    s_last = -1;
   }
   __syncthreads();
-  if (filled) atomicAdd(&s_filled, filled);
+  filled = __reduce_add_sync(0xffffffffu, filled);
+  if (lane == 0 && filled) atomicAdd(&s_filled, filled);
   __syncthreads();
   const int q0 = -s_filled;  // r + q0: the row of q
-  for (int r = r0 + threadIdx.x; r < r1 - 1; r += blockDim.x) {
+  for (int r = r0 + threadIdx.x; r < r1 - 1; r += VF_THREADS) {
     const int x = ids[r + 1];
     bool keep = false;
     if (x >= 0 && x < n && (!q || r + q0 < q_rows)) {
@@ -104,87 +233,201 @@ __global__ void __launch_bounds__(1024) k_verify(const float* __restrict__ p, in
   const int stop = s_stop;
   const float* pr = p + (int64_t)stop * ldp;
   const float* qr = q && stop < r1 - 1 && stop + q0 < q_rows ? q + (int64_t)(stop + q0) * ldq : nullptr;
-  const int gone = !q && stop < r1 - 1 ? ids[stop + 1] : -1;
-  const int per = (n + blockDim.x - 1) / blockDim.x;
-  const int lo = min(n, (int)threadIdx.x * per), hi = min(n, lo + per);
-  bool rest = true;  // weights of the residual; false: of p itself
-  auto weight = [&](int i) {
-    double a = (double)pr[i];
-    if (rest && qr) a -= (double)qr[i];
-    if (rest && i == gone) a = 0.0;
-    return a > 0.0 ? a : 0.0;
+  int gone = !q && stop < r1 - 1 ? ids[stop + 1] : -1;
+  const int lo = min(n, rank * per), hi = min(n, lo + per);
+  const int segs = (hi - lo + VF_SEG - 1) / VF_SEG;
+  const bool wide = (((uintptr_t)pr | (uintptr_t)qr) & 15) == 0;  // lo is a multiple of VF_SEG
+  // the lane's four weights of a segment
+  auto weights = [&](int seg, double (&v)[4]) {
+    const int i = lo + seg * VF_SEG + lane * 4;
+    float a[4] = {0.f, 0.f, 0.f, 0.f}, c[4] = {0.f, 0.f, 0.f, 0.f};
+    if (wide && i + 4 <= hi) {
+      const float4 f = *reinterpret_cast<const float4*>(pr + i);
+      a[0] = f.x, a[1] = f.y, a[2] = f.z, a[3] = f.w;
+      if (qr) {
+        const float4 h = *reinterpret_cast<const float4*>(qr + i);
+        c[0] = h.x, c[1] = h.y, c[2] = h.z, c[3] = h.w;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (i + e < hi) {
+          a[e] = pr[i + e];
+          if (qr) c[e] = qr[i + e];
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const double d = (double)a[e] - (double)c[e];
+      v[e] = d > 0.0 && i + e != gone ? d : 0.0;
+    }
   };
-  double before = 0.0, total = 0.0, mine = 0.0;
-  for (int pass = 0; pass < 2; ++pass) {
-    mine = 0.0;
-    for (int i = lo; i < hi; ++i) mine += weight(i);
-    __syncthreads();
-    s_d[threadIdx.x] = mine;
-    __syncthreads();
-    before = total = 0.0;
-    for (int k = 0; k < (int)blockDim.x; ++k) {
-      if (k == (int)threadIdx.x) before = total;
-      total += s_d[k];
+  double total = 0.0, before = 0.0;
+  for (;;) {
+    int last = -1;
+#pragma unroll 4
+    for (int s = wid; s < segs; s += VF_WARPS) {
+      double v[4];
+      weights(s, v);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (v[e] > 0.0) last = lo + s * VF_SEG + lane * 4 + e;
+      const double sum = vf_warp_sum((v[0] + v[1]) + (v[2] + v[3]));
+      if (lane == 0) s_seg[s] = sum;
     }
-    if (total > 0.0 || !rest) break;
-    rest = false;  // p == q: the refusal was a rounding's
-  }
-  // first index whose cumulative weight exceeds u total; if rounding leaves
-  // none, the last index with a weight
-  const double r = (double)u[r1 - 1] * total;
-  int first = 0x7fffffff, last = -1;
-  double cum = before;
-  for (int i = lo; i < hi; ++i) {
-    const double a = weight(i);
-    if (!(a > 0.0)) continue;
-    cum += a;
-    last = i;
-    if (first == 0x7fffffff && cum > r) first = i;
-  }
-  first = __reduce_min_sync(0xffffffffu, first);
-  last = __reduce_max_sync(0xffffffffu, last);
-  __shared__ int s_l[32];
-  if (lane == 0) {
-    s_i[wid] = first;
-    s_l[wid] = last;
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int k = 0; k < 32; ++k) {
-      first = min(first, s_i[k]);
-      last = max(last, s_l[k]);
+    last = __reduce_max_sync(0xffffffffu, last);
+    if (lane == 0 && last >= 0) atomicMax(&s_last, last);
+    __syncthreads();
+    // running sums of the segments by one warp, a stretch of them per lane
+    if (wid == 0) {
+      const int each = (segs + 31) / 32;
+      double mine = 0.0;
+      for (int k = lane * each; k < min(segs, (lane + 1) * each); ++k) s_seg[k] = mine += s_seg[k];
+      double up = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double y = __shfl_up_sync(0xffffffffu, up, o);
+        if (lane >= o) up += y;
+      }
+      double base = __shfl_up_sync(0xffffffffu, up, 1);
+      if (lane == 0) base = 0.0;
+      for (int k = lane * each; k < min(segs, (lane + 1) * each); ++k) s_seg[k] += base;
+      __syncwarp();
+      if (lane == 0) s_sum = segs ? s_seg[segs - 1] : 0.0;
     }
-    taken[b] = stop - r0;
-    tokens[stop] = first != 0x7fffffff ? first : max(last, 0);
+    cluster.sync();
+    total = before = 0.0;
+    for (int k = 0; k < nc; ++k) {
+      if (k == rank) before = total;
+      total += vf_peer(&s_sum, k);
+    }
+    if (total > 0.0 || !(qr || gone >= 0)) break;
+    // p <= q everywhere: the refusal was a rounding's, p itself is drawn from
+    cluster.sync();
+    qr = nullptr;
+    gone = -1;
   }
-  for (int i = r0 + threadIdx.x; i < r1; i += blockDim.x)
-    if (i != stop) tokens[i] = i < stop ? ids[i + 1] : -1;
+  // the first index whose cumulative weight exceeds u total lies in the CTA
+  // that reaches beyond it; if rounding leaves none, the last index with a weight
+  const double r = (double)draw * total;
+  if (wid == 0) {
+    const bool mine = before <= r && before + s_sum > r;
+    if (mine) {
+      // first segment that reaches beyond r
+      int a = 0, z = segs - 1;
+      while (a < z) {
+        const int mid = (a + z) / 2;
+        if (before + s_seg[mid] > r) z = mid;
+        else a = mid + 1;
+      }
+      double v[4], cum = 0.0;
+      weights(a, v);
+      cum = ((v[0] + v[1]) + v[2]) + v[3];
+      double up = cum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double y = __shfl_up_sync(0xffffffffu, up, o);
+        if (lane >= o) up += y;
+      }
+      double base = __shfl_up_sync(0xffffffffu, up, 1);
+      if (lane == 0) base = 0.0;
+      base += before + (a ? s_seg[a - 1] : 0.0);
+      int first = 0x7fffffff, last = -1;
+      double run = 0.0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        run += v[e];
+        if (!(v[e] > 0.0)) continue;
+        last = lo + a * VF_SEG + lane * 4 + e;
+        if (first == 0x7fffffff && base + run > r) first = last;
+      }
+      first = __reduce_min_sync(0xffffffffu, first);
+      last = __reduce_max_sync(0xffffffffu, last);
+      if (lane == 0) tokens[stop] = first != 0x7fffffff ? first : last;
+    }
+    if (rank == 0 && !(r < total)) {
+      const int last = __reduce_max_sync(0xffffffffu, lane < nc ? vf_peer(&s_last, lane) : -1);
+      if (lane == 0) tokens[stop] = max(last, 0);
+    }
+  }
+  if (rank == nc - 1) {
+    if (threadIdx.x == 0) taken[b] = stop - r0;
+    for (int i = r0 + threadIdx.x; i < r1; i += VF_THREADS)
+      if (i != stop) tokens[i] = i < stop ? ids[i + 1] : -1;
+  }
+  cluster.sync();  // nobody leaves while its sums are read
+}
+
+// CTAs per row: what `least` asks for, more while the GPU has room and a CTA keeps 2048 entries.
+static int vf_cluster(int64_t rows, int64_t n, int64_t least, int64_t room) {
+  int c = 1;
+  while (c < VF_MAX_CLUSTER && (c < least || (rows * c * 2 <= room && n / c > 4096))) c *= 2;
+  return c;
+}
+
+template <typename... KArgs, typename... Args>
+static int vf_launch(const char* what, void (*kern)(KArgs...), int64_t rows, int c, size_t smem, int most,
+                     cudaStream_t st, Args... args) {
+  static_assert(sizeof...(KArgs) == sizeof...(Args), "a kernel of this file");
+  static bool ready[64] = {false};  // of this kernel: the two have parameters of their own
+  int dev = 0;
+  Q8_CUDA(cudaGetDevice(&dev));
+  if (!ready[dev & 63]) {
+    Q8_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+    Q8_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    ready[dev & 63] = true;
+  }
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {(unsigned)c, 1, 1};
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(rows * c));
+  cfg.blockDim = dim3(VF_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
+  if (e != cudaSuccess) {
+    set_error("launch %s: %s", what, cudaGetErrorString(e));
+    return Q8_ERR_CUDA;
+  }
+  return Q8_OK;
 }
 
 }  // namespace q8
 
 using namespace q8;
 
+constexpr int64_t VF_PROBS_MAX = (int64_t)VF_MAX_CLUSTER * VF_SLICE;  // 327,680
+constexpr int64_t VF_VERIFY_MAX = (int64_t)VF_MAX_CLUSTER * 20000 * VF_SEG;
+
 extern "C" int q8op_probs(const float* logits, int64_t rows, int64_t n, int64_t ld, float temp, float* out,
                           int64_t ldo, void* stream) {
-  Q8_CHECK_ARG(rows >= 0 && rows <= (1 << 24) && n >= 1 && n <= (1 << 28) && ld >= n && ldo >= n,
-               "q8op_probs: bad shape");
+  Q8_CHECK_ARG(rows >= 0 && rows <= (1 << 24) && n >= 1 && n <= VF_PROBS_MAX && ld >= n && ldo >= n,
+               "q8op_probs: bad shape (%lld rows of %lld, at most %lld)", (long long)rows, (long long)n,
+               (long long)VF_PROBS_MAX);
   Q8_CHECK_ARG(!isnan(temp), "q8op_probs: temp must not be NaN");
   if (rows == 0) return Q8_OK;
   Q8_CHECK_ARG(logits && out, "q8op_probs: null pointer");
-  k_probs<<<(int)rows, 1024, 0, (cudaStream_t)stream>>>(logits, (int)n, ld, temp, out, ldo);
-  return launch_check("k_probs");
+  const int c = vf_cluster(rows, n, (n + VF_SLICE - 1) / VF_SLICE, 2 * num_sms());
+  const int per = (int)((n + c - 1) / c + 3) & ~3;
+  const double scale = std::min(1.4426950408889634 / (double)temp, 3e38);  // a subnormal temp: still no 0 x infinity
+  const float ch = (float)scale, cl = (float)(scale - (double)ch);
+  return vf_launch("k_probs", k_probs, rows, c, 0, 0, (cudaStream_t)stream, logits, (int)n, ld, temp, ch, cl, out,
+                   ldo, per);
 }
 
 extern "C" int q8op_verify(const float* p, int64_t ldp, const float* q, int64_t ldq, int64_t q_rows,
                            const int32_t* ids, const int32_t* seq_start, int64_t rows, int64_t S, int64_t n,
                            const float* u, int32_t* n_accepted, int32_t* tokens, void* stream) {
-  Q8_CHECK_ARG(rows >= 0 && rows <= (1 << 24) && S >= 0 && S <= (1 << 20) && n >= 1 && n <= (1 << 28) && ldp >= n &&
-                   (!q || (ldq >= n && q_rows >= 0 && q_rows <= (1 << 24))),
+  Q8_CHECK_ARG(rows >= 0 && rows <= (1 << 24) && S >= 0 && S <= (1 << 20) && n >= 1 && n <= VF_VERIFY_MAX &&
+                   ldp >= n && (!q || (ldq >= n && q_rows >= 0 && q_rows <= (1 << 24))),
                "q8op_verify: bad shape");
   if (S == 0) return Q8_OK;
   Q8_CHECK_ARG(seq_start && n_accepted && (rows == 0 || (p && ids && u && tokens)), "q8op_verify: null pointer");
-  k_verify<<<(int)S, 1024, 0, (cudaStream_t)stream>>>(p, ldp, q, ldq, (int)q_rows, ids, seq_start, (int)rows, (int)S, (int)n, u,
-                                                      n_accepted, tokens);
-  return launch_check("k_verify");
+  const int c = vf_cluster(S, n, 1, 2 * num_sms());
+  const int per = (int)(((n + c - 1) / c + VF_SEG - 1) / VF_SEG * VF_SEG);
+  return vf_launch("k_verify", k_verify, S, c, (size_t)(per / VF_SEG) * 8, 20001 * 8, (cudaStream_t)stream, p, ldp, q,
+                   ldq, (int)q_rows, ids, seq_start, (int)rows, (int)n, u, n_accepted, tokens, per);
 }

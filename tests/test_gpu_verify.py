@@ -76,7 +76,7 @@ def test_probs_special_rows(cuda):
     rows[7, [4, 9]] = 3.0
     rows[8] = 3e38
     rows[8, 1::2] = -3e38
-    for temp in (1.0, 0.05, 0.0, 50.0):
+    for temp in (1.0, 0.05, 0.0, 50.0, 1e-30, 1e-44):
         check_probs(rows, temp, cuda)
 
 

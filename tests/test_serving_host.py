@@ -51,6 +51,7 @@ def test_kv8_entries_refuse():
     refused(attend(dtype=-1), "dtype")
     assert append(rows=0) == attend(rows=0) == append(S=0) == attend(S=0) == _lib.Q8_OK
     refused(L.q8op_kv8_read(pages(), ONE, ONE, 1, ONE, 1, None, ONE, 1, None), "null")
+    refused(L.q8op_kv8_read(pages(), ONE, ONE, 1, ONE, 1, ONE + 4, ONE, 1, None), "unaligned")
     refused(L.q8op_kv8_read(pages(), ONE, None, 1, ONE, 1, ONE, ONE, 1, None), "null")
 
 
