@@ -289,17 +289,35 @@ struct PoolList {
 // A pair is left out when its destination is a source of the call, or the
 // destination of another pair: what such copies leave would depend on their
 // order.  Every CTA marks the call's page numbers in bitmaps (sources,
-// destinations, destinations seen twice), then takes its share of the pairs.
-__global__ void __launch_bounds__(512) k_pg_copy(PoolList pools, int num_pages, const int32_t* __restrict__ src,
-                                                 const int32_t* __restrict__ dst, int n) {
+// destinations, destinations seen twice), lists the pairs that remain, and
+// takes its share of their 16 KB pieces: 64 bytes of a piece per thread, all
+// loaded before the first is stored.
+constexpr int PG_COPY_THREADS = 256;
+constexpr int PG_PIECE = PG_COPY_THREADS * 64;
+constexpr int PG_LIST = 2048;  // pairs per pass
+
+__global__ void __launch_bounds__(PG_COPY_THREADS) k_pg_copy(PoolList pools, int num_pages,
+                                                             const int32_t* __restrict__ src,
+                                                             const int32_t* __restrict__ dst, int n) {
   extern __shared__ unsigned bits[];
-  const int words = (min(num_pages, PG_WINDOW) + 31) / 32;
+  __shared__ int2 s_list[PG_LIST];
+  __shared__ int s_at[PG_MAX_POOLS + 1];  // first piece of each pool within a page
+  __shared__ int s_warp[PG_COPY_THREADS / 32];
+  const int words = (min(num_pages, PG_WINDOW) + 31) / 32, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   unsigned *is_src = bits, *is_dst = bits + words, *twice = bits + 2 * words;
+  if (threadIdx.x == 0) {
+    int at = 0;
+    for (int k = 0; k < pools.n; ++k) {
+      s_at[k] = at;
+      at += (int)((pools.bytes[k] + PG_PIECE - 1) / PG_PIECE);
+    }
+    s_at[pools.n] = at;
+  }
   for (int w0 = 0; w0 < num_pages; w0 += PG_WINDOW) {
     __syncthreads();
-    for (int i = threadIdx.x; i < 3 * words; i += blockDim.x) bits[i] = 0u;
+    for (int i = threadIdx.x; i < 3 * words; i += PG_COPY_THREADS) bits[i] = 0u;
     __syncthreads();
-    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+    for (int i = threadIdx.x; i < n; i += PG_COPY_THREADS) {
       const int a = src[i], b = dst[i];
       if (a < 0 || a >= num_pages || b < 0 || b >= num_pages) continue;
       const int ra = a - w0, rb = b - w0;
@@ -310,22 +328,53 @@ __global__ void __launch_bounds__(512) k_pg_copy(PoolList pools, int num_pages, 
       }
     }
     __syncthreads();
-    for (int i = blockIdx.x; i < n; i += gridDim.x) {
-      const int a = src[i], b = dst[i];
-      if (a < 0 || a >= num_pages || b < 0 || b >= num_pages) continue;
-      const int rb = b - w0;
-      if (rb < 0 || rb >= PG_WINDOW || ((is_src[rb >> 5] | twice[rb >> 5]) >> (rb & 31) & 1)) continue;
-      for (int k = 0; k < pools.n; ++k) {
-        const int64_t bytes = pools.bytes[k];
-        const uint8_t* from = pools.base[k] + a * bytes;
-        uint8_t* to = pools.base[k] + b * bytes;
-        if (((uintptr_t)pools.base[k] | bytes) % 16 == 0) {
-          for (int64_t o = threadIdx.x; o < bytes / 16; o += blockDim.x)
-            reinterpret_cast<uint4*>(to)[o] = reinterpret_cast<const uint4*>(from)[o];
+    for (int p0 = 0; p0 < n; p0 += PG_LIST) {
+      int listed = 0;
+      for (int i0 = p0; i0 < min(n, p0 + PG_LIST); i0 += PG_COPY_THREADS) {
+        const int i = i0 + threadIdx.x;
+        int a = -1, b = -1;
+        if (i < n) a = src[i], b = dst[i];
+        const int rb = b - w0;
+        bool ok = a >= 0 && a < num_pages && b >= 0 && b < num_pages && rb >= 0 && rb < PG_WINDOW;
+        if (ok) ok = !((is_src[rb >> 5] | twice[rb >> 5]) >> (rb & 31) & 1);
+        const unsigned m = __ballot_sync(0xffffffffu, ok);
+        if (lane == 0) s_warp[warp] = __popc(m);
+        __syncthreads();
+        int at = listed;
+        for (int k = 0; k < PG_COPY_THREADS / 32; ++k) {
+          if (k < warp) at += s_warp[k];
+          listed += s_warp[k];
+        }
+        if (ok) s_list[at + __popc(m & ((1u << lane) - 1u))] = make_int2(a, b);
+        __syncthreads();
+      }
+      const int per = s_at[pools.n];
+      for (int64_t u = blockIdx.x; u < (int64_t)listed * per; u += gridDim.x) {
+        const int2 pair = s_list[u / per];
+        const int c = (int)(u % per);
+        int k = 0;
+        while (c >= s_at[k + 1]) ++k;
+        const int64_t bytes = pools.bytes[k], o = (int64_t)(c - s_at[k]) * PG_PIECE;
+        const uint8_t* from = pools.base[k] + pair.x * bytes + o;
+        uint8_t* to = pools.base[k] + pair.y * bytes + o;
+        const int len = (int)min((int64_t)PG_PIECE, bytes - o);
+        if ((((uintptr_t)pools.base[k] | bytes) & 15) == 0) {
+          uint4 v[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int at = (i * PG_COPY_THREADS + threadIdx.x) * 16;
+            if (at < len) v[i] = __ldcs(reinterpret_cast<const uint4*>(from + at));
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int at = (i * PG_COPY_THREADS + threadIdx.x) * 16;
+            if (at < len) __stcs(reinterpret_cast<uint4*>(to + at), v[i]);
+          }
         } else {
-          for (int64_t o = threadIdx.x; o < bytes; o += blockDim.x) to[o] = from[o];
+          for (int i = threadIdx.x; i < len; i += PG_COPY_THREADS) to[i] = from[i];
         }
       }
+      __syncthreads();  // the list is used again
     }
   }
 }
@@ -342,11 +391,11 @@ static int pg_check(const char* what, const void* table, int64_t S, int max_page
   return Q8_OK;
 }
 
-// Opt-in above 48 KB: always the kernel's own largest size, so that two threads
+// Opt-in above 48 KB (the kernels' static arrays included): always the kernel's own largest size, so that two threads
 // that call at once ask for the same.
 template <typename K>
 static int pg_smem(K kern, size_t bytes, int most) {
-  if (bytes > 48 * 1024) Q8_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+  if (bytes > 24 * 1024) Q8_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
   return Q8_OK;
 }
 
@@ -414,14 +463,17 @@ extern "C" int q8op_kv_copy_pages(void* const* pools, const int64_t* page_bytes,
   Q8_CHECK_ARG(pools && page_bytes && src && dst, "q8op_kv_copy_pages: null pointer");
   PoolList l{};
   l.n = n_pools;
+  int64_t pieces = 0;
   for (int i = 0; i < n_pools; ++i) {
     Q8_CHECK_ARG(pools[i] && page_bytes[i] > 0, "q8op_kv_copy_pages: pool %d is null or empty", i);
     l.base[i] = (uint8_t*)pools[i];
     l.bytes[i] = page_bytes[i];
+    pieces += (page_bytes[i] + PG_PIECE - 1) / PG_PIECE;
   }
+  Q8_CHECK_ARG(pieces < ((int64_t)1 << 30), "q8op_kv_copy_pages: pages of more than 16 TB");
   const size_t smem = (size_t)((std::min<int64_t>(num_pages, PG_WINDOW) + 31) / 32) * 12;
   Q8_TRY(pg_smem(k_pg_copy, smem, PG_WINDOW / 32 * 12));
-  const int grid = (int)std::min<int64_t>(n, 2 * num_sms());
-  k_pg_copy<<<grid, 512, smem, (cudaStream_t)stream>>>(l, (int)num_pages, src, dst, (int)n);
+  const int grid = (int)std::min<int64_t>(n * pieces, 6 * num_sms());
+  k_pg_copy<<<grid, PG_COPY_THREADS, smem, (cudaStream_t)stream>>>(l, (int)num_pages, src, dst, (int)n);
   return launch_check("k_pg_copy");
 }

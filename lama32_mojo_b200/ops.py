@@ -177,49 +177,61 @@ def argmax(logits: torch.Tensor) -> torch.Tensor:
 KV8_BLOCK = 16  # tokens of a kv head that share a scale (Q8_KV8_BLOCK)
 
 
-def _tensor(t, what, dtype, shape=None, device=None):
-    """A contiguous CUDA tensor of ``dtype`` (and shape, and device)."""
+def _tensor(t, what, dtype, shape, dev: int) -> None:
+    """Raises unless ``t`` is a contiguous tensor of ``dtype`` (and shape) on CUDA device ``dev``."""
+    try:
+        if t.dtype is dtype and t.get_device() == dev and t.is_contiguous() and (shape is None or t.shape == shape):
+            return
+    except AttributeError:
+        pass
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f"{what}: libq8cuda ops take CUDA tensors")
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise ValueError(f"{what}: {dtype} wanted, got {t.dtype}")
+    if t.get_device() != dev:
+        raise ValueError(f"{what}: is on {t.device}, other tensors of the call on cuda:{dev}")
     if not t.is_contiguous():
         raise ValueError(f"{what}: must be contiguous")
-    if shape is not None and tuple(t.shape) != shape:
-        raise ValueError(f"{what}: shape {shape} wanted, got {tuple(t.shape)}")
-    if device is not None and t.device != device:
-        raise ValueError(f"{what}: is on {t.device}, other tensors of the call on {device}")
+    raise ValueError(f"{what}: shape {tuple(shape)} wanted, got {tuple(t.shape)}")
 
 
-def _call(fn, dev: torch.device, *args):
-    """fn(*args, stream) on torch's current stream of ``dev``."""
-    if torch.cuda.current_device() != dev.index:
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else \
+    (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+
+
+def _call(fn, dev: int, *args) -> None:
+    """fn(*args, stream) on torch's current stream of device ``dev``."""
+    if torch.cuda.current_device() != dev:
         with torch.cuda.device(dev):
-            check(fn(*args, torch.cuda.current_stream(dev).cuda_stream))
-    else:
-        check(fn(*args, torch.cuda.current_stream(dev).cuda_stream))
+            check(fn(*args, _raw_stream(dev)))
+        return
+    status = fn(*args, _raw_stream(dev))
+    if status:
+        check(status)
 
 
 class KV8Pages:
     """One layer's pages of the 8-bit cache: int8 codes k, v [num_pages, n_kv, page, head_dim]
     and f32 scales k_scale, v_scale [num_pages, n_kv, page / 16]; a value is code * scale."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "num_pages", "n_kv", "page", "head_dim", "_c", "_ref")
+    __slots__ = ("k", "v", "k_scale", "v_scale", "num_pages", "n_kv", "page", "head_dim", "_c", "_ref", "_dev")
 
     def __init__(self, k, v, k_scale, v_scale):
-        _tensor(k, "KV8Pages k", torch.int8)
+        dev = k.get_device()
+        _tensor(k, "KV8Pages k", torch.int8, None, max(dev, 0))
         if k.dim() != 4 or k.shape[2] == 0 or k.shape[2] % KV8_BLOCK or k.shape[3] not in (64, 128):
             raise ValueError(f"KV8Pages k: [pages, n_kv, page (a multiple of {KV8_BLOCK}), head_dim (64 or 128)] "
                              f"wanted, got {tuple(k.shape)}")
         pages, kv, page, hd = k.shape
-        _tensor(v, "KV8Pages v", torch.int8, tuple(k.shape), k.device)
+        _tensor(v, "KV8Pages v", torch.int8, k.shape, dev)
         for t, what in ((k_scale, "KV8Pages k_scale"), (v_scale, "KV8Pages v_scale")):
-            _tensor(t, what, torch.float32, (pages, kv, page // KV8_BLOCK), k.device)
+            _tensor(t, what, torch.float32, (pages, kv, page // KV8_BLOCK), dev)
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.num_pages, self.n_kv, self.page, self.head_dim = pages, kv, page, hd
         self._c = _lib.q8_kv8_pages(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages, kv,
                                     page, hd)
         self._ref = C.addressof(self._c)
+        self._dev = dev
 
     @classmethod
     def empty(cls, num_pages: int, n_kv: int, page: int = 64, head_dim: int = 128, device="cuda") -> "KV8Pages":
@@ -244,26 +256,26 @@ def _packed(what, seq_start, ctx, pages, block_table):
     """Checks what every call on packed rows takes; returns (S, max_pages, device)."""
     if not isinstance(pages, KV8Pages):
         raise ValueError(f"{what}: pages must be a KV8Pages")
-    dev = pages.k.device
-    if ctx.dim() != 1 or block_table.dim() != 2:
-        raise ValueError(f"{what}: ctx [S] and block_table [S, max_pages] wanted")
+    dev = pages._dev
+    if block_table.dim() != 2:
+        raise ValueError(f"{what}: block_table [S, max_pages] wanted")
     S, width = block_table.shape
-    _tensor(seq_start, f"{what}: seq_start", torch.int32, (S + 1,), dev)
-    _tensor(ctx, f"{what}: ctx", torch.int32, (S,), dev)
-    _tensor(block_table, f"{what}: block_table", torch.int32, None, dev)
+    _tensor(seq_start, what + ": seq_start", torch.int32, (S + 1,), dev)
+    _tensor(ctx, what + ": ctx", torch.int32, (S,), dev)
+    _tensor(block_table, what + ": block_table", torch.int32, None, dev)
     return S, width, dev
 
 
-def _rows_of(t, what, width, dev):
+def _rows_of(t, what, width, dev: int):
     """[T, width] or [T, heads, head_dim] rows with contiguous elements: (row count, row stride)."""
-    if not t.is_cuda or t.device != dev:
-        raise ValueError(f"{what}: is on {t.device}, the pages are on {dev}")
+    if t.get_device() != dev:
+        raise ValueError(f"{what}: is on {t.device}, the pages are on cuda:{dev}")
     if t.dtype not in _DT:
         raise ValueError(f"{what}: f32, bf16 or f16 rows wanted, got {t.dtype}")
     st, sh = t.stride(), t.shape
-    if t.dim() == 2 and sh[1] == width and (st[1] == 1 or width == 1):
+    if len(sh) == 2 and sh[1] == width and (st[1] == 1 or width == 1):
         return sh[0], st[0] if sh[0] > 1 else max(st[0], width)
-    if t.dim() == 3 and sh[1] * sh[2] == width and st[2] == 1 and (st[1] == sh[2] or sh[1] == 1):
+    if len(sh) == 3 and sh[1] * sh[2] == width and st[2] == 1 and (st[1] == sh[2] or sh[1] == 1):
         return sh[0], st[0] if sh[0] > 1 else max(st[0], width)
     raise ValueError(f"{what}: rows of {width} contiguous elements wanted, got shape {tuple(sh)}, strides {st}")
 
@@ -287,8 +299,7 @@ def kv8_read(seq_start, ctx, pages: KV8Pages, block_table, rows: int):
     S, width, dev = _packed("kv8_read", seq_start, ctx, pages, block_table)
     if rows < 0:
         raise ValueError("kv8_read: rows < 0")
-    shape = (rows, pages.n_kv, pages.head_dim)
-    k, v = torch.empty(shape, device=dev), torch.empty(shape, device=dev)
+    k, v = torch.empty((2, rows, pages.n_kv, pages.head_dim), dtype=torch.float32, device=pages.k.device).unbind(0)
     _call(lib().q8op_kv8_read, dev, pages._ref, seq_start.data_ptr(), ctx.data_ptr(), S, block_table.data_ptr(),
           width, k.data_ptr(), v.data_ptr(), rows)
     return k, v
@@ -301,16 +312,15 @@ def kv8_attention(q, seq_start, ctx, n_heads: int, pages: KV8Pages, block_table,
     w = n_heads * pages.head_dim
     T, ldq = _rows_of(q, "kv8_attention: q", w, dev)
     if out is None:
-        out = torch.empty((T, w), dtype=q.dtype, device=dev)
-        ldo = w
+        out, ldo = q.new_empty((T, w)), w
     else:
         To, ldo = _rows_of(out, "kv8_attention: out", w, dev)
         if To != T or out.dtype != q.dtype:
             raise ValueError("kv8_attention: out must have q's rows and type")
     nbytes = lib().q8op_kv8_attention_workspace(_DT[q.dtype], T, S, n_heads, pages.n_kv, pages.head_dim)
-    work = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    work = torch.empty(nbytes, dtype=torch.uint8, device=q.device).data_ptr() if nbytes else None
     _call(lib().q8op_kv8_attention, dev, q.data_ptr(), ldq, _DT[q.dtype], T, seq_start.data_ptr(), ctx.data_ptr(), S,
-          n_heads, pages._ref, block_table.data_ptr(), width, out.data_ptr(), ldo, _p(work), nbytes)
+          n_heads, pages._ref, block_table.data_ptr(), width, out.data_ptr(), ldo, work, nbytes)
     return out
 
 
@@ -318,12 +328,13 @@ def kv8_attention(q, seq_start, ctx, n_heads: int, pages: KV8Pages, block_table,
 def _state(what, block_table, ctx, refs):
     if block_table.dim() != 2 or refs.dim() != 1:
         raise ValueError(f"{what}: block_table [S, max_pages] and refs [num_pages] wanted")
-    dev = block_table.device
-    _tensor(block_table, f"{what}: block_table", torch.int32)
+    dev = block_table.get_device()
+    S, width = block_table.shape
+    _tensor(block_table, what + ": block_table", torch.int32, None, max(dev, 0))
     if ctx is not None:
-        _tensor(ctx, f"{what}: ctx", torch.int32, (block_table.shape[0],), dev)
-    _tensor(refs, f"{what}: refs", torch.int32, None, dev)
-    return block_table.shape[0], block_table.shape[1], refs.shape[0], dev
+        _tensor(ctx, what + ": ctx", torch.int32, (S,), dev)
+    _tensor(refs, what + ": refs", torch.int32, None, dev)
+    return S, width, refs.shape[0], dev
 
 
 def kv_truncate(block_table, ctx, refs, page: int, new_len) -> None:
@@ -350,11 +361,11 @@ def kv_reserve(block_table, ctx, refs, page: int, n_new):
     pages wanted, pages free], all on the device.  When the pool is too small nothing changes."""
     S, width, pages, dev = _state("kv_reserve", block_table, ctx, refs)
     _tensor(n_new, "kv_reserve: n_new", torch.int32, (S,), dev)
-    got = torch.empty(2 * S + 3 + pages, dtype=torch.int32, device=dev)  # src, dst, status, scratch
+    got = refs.new_empty(2 * S + 3 + pages)
     at = got.data_ptr()
     _call(lib().q8op_kv_reserve, dev, block_table.data_ptr(), S, width, ctx.data_ptr(), refs.data_ptr(), pages, page,
           n_new.data_ptr(), at, at + 4 * S, at + 8 * S, at + 8 * S + 12)
-    return got[:S], got[S:2 * S], got[2 * S:2 * S + 3]
+    return got.split_with_sizes((S, S, 3, pages))[:3]  # the rest is scratch
 
 
 def kv_compact(block_table, refs):
@@ -362,11 +373,11 @@ def kv_compact(block_table, refs):
     [num_pages / 2], the page copies to make (kv_copy_pages), -1 behind the last."""
     S, width, pages, dev = _state("kv_compact", block_table, None, refs)
     half = pages // 2
-    got = torch.empty(2 * half + pages, dtype=torch.int32, device=dev)
+    got = refs.new_empty(2 * half + pages)
     at = got.data_ptr()
     _call(lib().q8op_kv_compact, dev, block_table.data_ptr(), S, width, refs.data_ptr(), pages, at, at + 4 * half,
           at + 8 * half)
-    return got[:half], got[half:2 * half]
+    return got.split_with_sizes((half, half, pages))[:2]  # the rest is scratch
 
 
 def kv_copy_pages(pools, src, dst) -> None:
@@ -374,44 +385,45 @@ def kv_copy_pages(pools, src, dst) -> None:
     negative number are left out, and so are pairs whose result would depend on the order."""
     if not pools:
         return
-    dev, num_pages = pools[0].device, pools[0].shape[0]
-    n = src.numel()
-    _tensor(src, "kv_copy_pages: src", torch.int32, (n,), dev)
+    dev, num_pages, n = pools[0].get_device(), pools[0].shape[0], src.numel()
+    _tensor(src, "kv_copy_pages: src", torch.int32, (n,), max(dev, 0))
     _tensor(dst, "kv_copy_pages: dst", torch.int32, (n,), dev)
+    addr, size = [], []
     for t in pools:
         _tensor(t, "kv_copy_pages: pool", t.dtype, None, dev)
         if t.dim() < 2 or t.shape[0] != num_pages or t.numel() == 0:
             raise ValueError("kv_copy_pages: pools of the same number of pages wanted")
-    for at in range(0, len(pools), 64):
-        part = pools[at:at + 64]
-        k = len(part)
-        _call(lib().q8op_kv_copy_pages, dev, (C.c_void_p * k)(*[t.data_ptr() for t in part]),
-              (C.c_int64 * k)(*[t.numel() // num_pages * t.element_size() for t in part]), k, num_pages,
-              src.data_ptr(), dst.data_ptr(), n)
+        addr.append(t.data_ptr())
+        size.append(t.nbytes // num_pages)
+    for at in range(0, len(addr), 64):
+        k = min(64, len(addr) - at)
+        _call(lib().q8op_kv_copy_pages, dev, (C.c_void_p * k)(*addr[at:at + k]), (C.c_int64 * k)(*size[at:at + k]), k,
+              num_pages, src.data_ptr(), dst.data_ptr(), n)
 
 
 # ------------------------------------------------------------------ speculative decoding
-def _matrix(t, what, dev=None):
+def _matrix(t, what, dev: int):
     """f32 [rows, n] with contiguous columns: (rows, n, row stride)."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f"{what}: libq8cuda ops take CUDA tensors")
-    if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] == 0 or (t.shape[1] > 1 and t.stride(1) != 1):
+    sh, st = t.shape, t.stride()
+    if t.dtype is not torch.float32 or len(sh) != 2 or sh[1] == 0 or (sh[1] > 1 and st[1] != 1):
         raise ValueError(f"{what}: f32 [rows, n] with contiguous columns wanted")
-    if dev is not None and t.device != dev:
-        raise ValueError(f"{what}: is on {t.device}, other tensors of the call on {dev}")
-    rows, n = t.shape
-    return rows, n, t.stride(0) if rows > 1 else max(t.stride(0), n)
+    if t.get_device() != dev:
+        raise ValueError(f"{what}: is on {t.device}, other tensors of the call on cuda:{dev}")
+    return sh[0], sh[1], st[0] if sh[0] > 1 else max(st[0], sh[1])
 
 
 def probs(logits: torch.Tensor, temp: float, out: torch.Tensor = None) -> torch.Tensor:
     """The distributions that sampling at ``temp`` and top_p = 1 draws from (q8op_probs)."""
-    rows, n, ld = _matrix(logits, "probs: logits")
-    dev = logits.device
+    dev = logits.get_device()
+    rows, n, ld = _matrix(logits, "probs: logits", dev)
     if out is None:
-        out = torch.empty((rows, n), device=dev)
-    ro, no, ldo = _matrix(out, "probs: out", dev)
-    if (ro, no) != (rows, n):
-        raise ValueError("probs: out must have the shape of logits")
+        out, ldo = logits.new_empty((rows, n)), n
+    else:
+        ro, no, ldo = _matrix(out, "probs: out", dev)
+        if (ro, no) != (rows, n):
+            raise ValueError("probs: out must have the shape of logits")
     _call(lib().q8op_probs, dev, logits.data_ptr(), rows, n, ld, temp, out.data_ptr(), ldo)
     return out
 
@@ -420,8 +432,8 @@ def verify(p, q, ids, seq_start, u):
     """Verify drafted tokens against the target's distributions p [T, n] (q8op_verify): q is the
     drafts' [drafts, n] or None (certain drafts), ids [T] the tokens fed, u [T] uniform draws.
     Returns (n_accepted [S], tokens [T]: kept drafts, the next token, -1)."""
-    rows, n, ldp = _matrix(p, "verify: p")
-    dev = p.device
+    dev = p.get_device()
+    rows, n, ldp = _matrix(p, "verify: p", dev)
     S = seq_start.numel() - 1
     if S < 0:
         raise ValueError("verify: seq_start [S + 1] wanted")
@@ -437,8 +449,7 @@ def verify(p, q, ids, seq_start, u):
             if nq != n:
                 raise ValueError("verify: q must have p's columns")
             qp = q.data_ptr()
-    n_accepted = torch.empty(S, dtype=torch.int32, device=dev)
-    tokens = torch.empty(rows, dtype=torch.int32, device=dev)
+    n_accepted, tokens = ids.new_empty(S + rows).split_with_sizes((S, rows))
     _call(lib().q8op_verify, dev, p.data_ptr(), ldp, qp, ldq, q_rows, ids.data_ptr(), seq_start.data_ptr(), rows, S,
           n, u.data_ptr(), n_accepted.data_ptr(), tokens.data_ptr())
     return n_accepted, tokens

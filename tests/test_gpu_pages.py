@@ -231,6 +231,14 @@ def test_copy_pages_past_the_bitmap_window(cuda):
     assert x[2 ** 18 + 9, 0] == 2 ** 18 + 9 and x[2 ** 18 + 10, 0] == 2  # two pairs wanted the former
 
 
+@pytest.mark.parametrize("pages", [65537, 100000, 131072, 2 ** 18])
+def test_copy_pages_bitmap_sizes(cuda, pages):
+    x = torch.arange(pages, device=cuda, dtype=torch.int32)[:, None].repeat(1, 4)
+    src, dst = [pages - 1, 3, 0], [4, pages - 2, pages // 2]
+    ops.kv_copy_pages([x], i32(src, cuda), i32(dst, cuda))
+    assert x[dst, 0].tolist() == src
+
+
 def test_many_pools_and_refusals(cuda):
     pools = [torch.randn((9, 8), device=cuda) for _ in range(130)]
     ops.kv_copy_pages(pools, i32([3], cuda), i32([4], cuda))
