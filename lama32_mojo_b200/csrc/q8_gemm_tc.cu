@@ -710,5 +710,6 @@ extern "C" int q8_device_status(void) {
   Q8_CUDA(cudaDeviceSynchronize());
   const int a = q8::gemm_tc_poll_error();
   const int b = q8::attn_dec_poll_error();
-  return a != 0 ? a : b;
+  const int c = q8::kv8_attn_tc_poll_error();
+  return a != 0 ? a : b != 0 ? b : c;
 }

@@ -112,6 +112,7 @@ size_t attention_decode_part_floats(int T, int nkv, int nsplit, int group, int h
 int attention_decode_nsplit(int items, int maxlen);
 int attn_dec_poll_error();
 int attn_dec_error_word(int** out);
+int kv8_attn_tc_poll_error();  // q8_kv8_attn_tc.cu
 // Fused RoPE / QK-norm / KV append for the decode attention: q and the new
 // k, v are read un-rotated from the q|k|v rows; kw / vw are the (same) pools.
 struct AttnRope {

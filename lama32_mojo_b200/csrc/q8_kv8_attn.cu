@@ -38,35 +38,14 @@
 // inside a unit leaves its partial result in the workspace, and
 // k_kv8_attn_join adds those up.  No atomics, a fixed order of every sum: the
 // same bits every time.
-#include "q8_kernels.h"
-#include "q8_kv8.cuh"
+#include "q8_kv8_attn.h"
 
 #include <algorithm>
 #include <cooperative_groups.h>
-#include <math.h>
 
 namespace cg = cooperative_groups;
 
 namespace q8 {
-
-constexpr float KA_LIFT = 32768.f;
-
-struct Kv8AttnArgs {
-  const void* q;
-  int64_t ldq;
-  int dtype, rows;
-  const int32_t* starts;
-  const int32_t* ctx;
-  int S, n_heads;
-  q8_kv8_pages kv;
-  const int32_t* table;
-  int max_pages;
-  void* out;
-  int64_t ldo;
-  int QT, GH, hgroups;  // tokens per group, heads per group, head groups per kv head
-  float* work;          // two partial results for every CTA
-  int4* work_meta;      // and what they are
-};
 
 template <int N>
 __device__ __forceinline__ void ka_load(uint32_t (&r)[N], const int8_t* p) {
@@ -83,25 +62,11 @@ __device__ __forceinline__ void ka_load(uint32_t (&r)[N], const int8_t* p) {
     asm volatile("ld.global.L1::no_allocate.v2.b32 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "l"(p));
 }
 
-__device__ __forceinline__ float ka_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 __device__ __forceinline__ void ka_imma(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
       : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// four biased codes (c + 128) -> f16 pairs (bytes 0, 1) and (bytes 2, 3): 0x64uu is 1024 + u
-__device__ __forceinline__ uint32_t ka_f16(uint32_t u, uint32_t sel) {
-  uint32_t x;
-  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(x) : "r"(u), "r"(0x64646464u), "r"(sel));
-  const __half2 h = __hsub2(*reinterpret_cast<__half2*>(&x), __half2half2(__ushort_as_half((unsigned short)0x6480)));
-  return *reinterpret_cast<const uint32_t*>(&h);
 }
 
 __device__ __forceinline__ void ka_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -115,11 +80,6 @@ __device__ __forceinline__ uint32_t ka_transpose(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
-}
-
-__device__ __forceinline__ uint32_t ka_pack(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
 }
 
 __device__ __forceinline__ float ka_remote(const float* p, int rank) {
@@ -139,78 +99,6 @@ __device__ __forceinline__ int kv8_find(const int32_t* starts, int S, int rows, 
     n += __syncthreads_count(b < S && min(max(starts[b], 0), rows) / QT + E * b <= slot);
   }
   return n - 1;
-}
-
-// N consecutive elements from element i0 on as floats
-template <bool WIDE, int N>
-__device__ __forceinline__ void ka_row(float (&v)[N], const void* base, int64_t i0, int dtype, bool aligned) {
-  if constexpr (WIDE) {
-    const float* p = (const float*)base + i0;
-    if (aligned) {
-#pragma unroll
-      for (int i = 0; i < N / 4; ++i) {
-        const float4 u = reinterpret_cast<const float4*>(p)[i];
-        v[4 * i] = u.x, v[4 * i + 1] = u.y, v[4 * i + 2] = u.z, v[4 * i + 3] = u.w;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = p[i];
-    }
-  } else {
-    const uint16_t* p = (const uint16_t*)base + i0;
-    uint32_t w[N / 2];
-    if (aligned) {
-#pragma unroll
-      for (int i = 0; i < N / 8; ++i) {
-        const uint4 u = reinterpret_cast<const uint4*>(p)[i];
-        w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < N / 2; ++i) w[i] = p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
-    }
-#pragma unroll
-    for (int i = 0; i < N / 2; ++i) {
-      const float2 f = __half22float2(*reinterpret_cast<__half2*>(&w[i]));
-      v[2 * i] = dtype == Q8_BF16 ? __uint_as_float(w[i] << 16) : f.x;
-      v[2 * i + 1] = dtype == Q8_BF16 ? __uint_as_float(w[i] & 0xffff0000u) : f.y;
-    }
-  }
-}
-
-template <bool WIDE>
-__device__ __forceinline__ void ka_store(const Kv8AttnArgs& a, int64_t i, float x) {
-  if (WIDE) ((float*)a.out)[i] = x;
-  else if (a.dtype == Q8_BF16) ((__nv_bfloat16*)a.out)[i] = __float2bfloat16_rn(x);
-  else ((__half*)a.out)[i] = __float2half_rn(x);
-}
-
-// A group of rows on one kv head.
-struct KaUnit {
-  int b, row0, toks;  // sequence, first row, tokens
-  int h, head0, heads;
-  int64_t pos0;       // position of the first token
-  int nblk;           // blocks that the last token sees
-};
-
-__device__ __forceinline__ int ka_blocks(const Kv8AttnArgs& a, int64_t end) {
-  const int64_t room = (int64_t)a.max_pages * a.kv.page;
-  return (int)((min(max(end, (int64_t)0), room) + KV8_BLOCK - 1) / KV8_BLOCK);
-}
-
-// j: kv head x head group; i0: first row of the group within the sequence
-__device__ __forceinline__ KaUnit ka_unit(const Kv8AttnArgs& a, const Kv8Seq& sq, int j, int i0) {
-  KaUnit u;
-  const int G = a.n_heads / a.kv.n_kv, hg = j % a.hgroups;
-  u.b = sq.b;
-  u.row0 = sq.row0 + i0;
-  u.toks = min(a.QT, sq.n - i0);
-  u.h = j / a.hgroups;
-  u.head0 = u.h * G + hg * a.GH;
-  u.heads = min(a.GH, G - hg * a.GH);
-  u.pos0 = sq.pos0 + i0;
-  u.nblk = ka_blocks(a, u.pos0 + u.toks);
-  return u;
 }
 
 template <bool WIDE, int HD, int NT>  // WIDE: f32 rows, digits of q, halves of P
@@ -568,16 +456,6 @@ __device__ __forceinline__ void ka_stretch(const Kv8AttnArgs& a, const KaUnit& u
   }
 }
 
-// Element k of a unit's rows, from its lifted sum x and the sum of the weights.
-template <bool WIDE, int HD>
-__device__ __forceinline__ void ka_write(const Kv8AttnArgs& a, int row0, int head0, int heads, int k, float x,
-                                         float sum) {
-  const int r = k / HD;
-  if (r % a.GH >= heads) return;
-  ka_store<WIDE>(a, (int64_t)(row0 + r / a.GH) * a.ldo + (head0 + r % a.GH) * HD + k % HD,
-                 sum > 0.f ? x * (1.f / KA_LIFT) / sum : 0.f * (x + sum));  // no position: 0; NaN stays
-}
-
 // Few units: a cluster of CTAs for each.
 template <bool WIDE, int HD, int NT>
 __global__ void __launch_bounds__(KaShape<WIDE, HD, NT>::WARPS * 32, 1) k_kv8_attn(Kv8AttnArgs a) {
@@ -623,26 +501,6 @@ __global__ void __launch_bounds__(KaShape<WIDE, HD, NT>::WARPS * 32, 1) k_kv8_at
     ka_write<WIDE, HD>(a, u.row0, u.head0, u.heads, k, x, sum);
   }
   cluster.sync();  // nobody leaves while its memory is read
-}
-
-// Inclusive sum over the CTA's threads; *total: all of them.  s: 33 words.
-__device__ __forceinline__ int64_t ka_scan(int64_t v, int64_t* s, int64_t* total) {
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t y = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += y;
-  }
-  __syncthreads();  // s may still be read
-  if (lane == 31) s[w] = v;
-  __syncthreads();
-  int64_t sum = 0;
-  for (int k = 0; k < nw; ++k) {
-    if (k == w) v += sum;
-    sum += s[k];
-  }
-  *total = sum;
-  return v;
 }
 
 // Many units: CTA c takes the c-th of gridDim.x equal stretches of all units'
@@ -759,7 +617,19 @@ __global__ void __launch_bounds__(256) k_kv8_attn_join(Kv8AttnArgs a, int RMAX) 
   }
 }
 
+template <bool WIDE, int HD>
+static int join_run(const Kv8AttnArgs& a, int ctas, int RMAX, cudaStream_t st) {
+  return launch_pdl("k_kv8_attn_join", k_kv8_attn_join<WIDE, HD>, dim3(ctas), dim3(256), 0, st, a, RMAX);
+}
+
+int kv8_attn_join(const Kv8AttnArgs& a, int ctas, int RMAX, cudaStream_t st) {
+  if (a.kv.head_dim == 128)
+    return a.dtype == Q8_F32 ? join_run<true, 128>(a, ctas, RMAX, st) : join_run<false, 128>(a, ctas, RMAX, st);
+  return a.dtype == Q8_F32 ? join_run<true, 64>(a, ctas, RMAX, st) : join_run<false, 64>(a, ctas, RMAX, st);
+}
+
 struct KaPlan {
+  bool tc;   // k_kv8_attn_tc
   int nt, GH, hgroups, QT, ctas;  // ctas: stretches of k_kv8_attn_many, 0: clusters
   int64_t slots, units;
   size_t meta, bytes;  // workspace
@@ -771,15 +641,16 @@ static KaPlan ka_plan(bool wide, int hd, int64_t rows, int64_t S, int n_heads, i
   const int64_t want = (rows + S - 1) / S * (int64_t)G;  // rows per kv head of an average sequence
   const int cols = wide ? 2 : 1;
   p.nt = want * cols <= 8 ? 1 : want * cols <= 16 ? 2 : 4;
-  const int rmax = 8 * p.nt / cols;
+  p.tc = want >= 64 && G <= KT_ROWS;
+  const int rmax = p.tc ? KT_ROWS : 8 * p.nt / cols;
   p.GH = std::min(G, rmax);
   p.hgroups = ceil_div(G, p.GH);
   p.QT = rows <= S ? 1 : rmax / p.GH;
   p.slots = p.QT > 1 ? rows / p.QT + S : rows;
   p.units = p.slots * n_kv * p.hgroups;
   // One n-tile: a unit is cheap to begin and its partial results are small.
-  if (p.nt == 1 && p.units > num_sms()) {
-    p.ctas = 3 * num_sms();
+  if (p.tc || (p.nt == 1 && p.units > num_sms())) {
+    p.ctas = p.tc ? kv8_attn_tc_ctas() : 3 * num_sms();
     p.meta = (size_t)p.ctas * 2 * rmax * (hd + 2) * 4;
     p.bytes = p.meta + (size_t)p.ctas * 2 * sizeof(int4);
   }
@@ -802,8 +673,7 @@ static int attn_run(Kv8AttnArgs& a, const KaPlan& p, cudaStream_t st) {
     if (p.ctas) {
       k_kv8_attn_many<WIDE, HD, NT><<<p.ctas, 128, Sh::smem(4), st>>>(a);
       Q8_TRY(launch_check("k_kv8_attn_many"));
-      return launch_pdl("k_kv8_attn_join", k_kv8_attn_join<WIDE, HD>, dim3(p.ctas), dim3(256), 0, st, a,
-                        (int)Sh::RMAX);
+      return kv8_attn_join(a, p.ctas, Sh::RMAX, st);
     }
   }
   // a cluster's CTAs: an SM each, but an iteration for every warp at the longest context
@@ -861,6 +731,10 @@ extern "C" int q8op_kv8_attention(const void* q, int64_t ldq, int dtype, int64_t
   Kv8AttnArgs a{q,   ldq,   dtype,       (int)rows, seq_start, ctx,  (int)S, n_heads,   *kv, block_table, max_pages,
                 out, ldo,   p.QT,        p.GH,      p.hgroups, (float*)work, (int4*)((char*)work + p.meta)};
   cudaStream_t st = (cudaStream_t)stream;
+  if (p.tc) {
+    Q8_TRY(kv8_attn_tc(a, p.ctas, st));
+    return kv8_attn_join(a, p.ctas, KT_ROWS, st);
+  }
   if (kv->head_dim == 128) return dtype == Q8_F32 ? attn_pick<true, 128>(a, p, st) : attn_pick<false, 128>(a, p, st);
   return dtype == Q8_F32 ? attn_pick<true, 64>(a, p, st) : attn_pick<false, 64>(a, p, st);
 }

@@ -1,0 +1,533 @@
+// Attention over the 8-bit cache for many query rows per kv head (chunks of
+// prompts), on the 5th-generation tensor cores (tcgen05 + TMEM).  The operator
+// and its softmax statistics (running M of s + log2(sv), weights e sv): see
+// q8_kv8_attn.cu.
+//
+// A CTA takes 128 rows (tokens x the heads that share a kv head) against key
+// tiles of 64 positions, four scale blocks:
+//   warps 4-7  load the tile's codes and write them as f16 (exact) into shared
+//              memory, rows of 64 dims in the 128-byte swizzle; K is read
+//              K-major, V (same layout) MN-major.  One lane of warp 7 issues
+//              S = Q K^T (128 x 64 x hd) into TMEM behind K, and O += P V
+//              (128 x hd x 64, P read from TMEM) behind V of the tile before.
+//   warps 0-3  a thread per row: reads its 64 scores from TMEM, keeps M and l,
+//              writes P over them.  S / P have two buffers, so the next tile's
+//              scores are computed meanwhile.
+// f32 rows: q = qh + ql and p = ph + pl, two products each (22 bits; the codes
+// need one f16): 4 x 128 x 64 x hd multiply-adds a tile.  bf16 / f16 rows: one.
+// M moves only when it has grown by more than 1, so that O in TMEM is scaled
+// seldom; weights stay below 2, lifted by 2^14.
+//
+// Two CTAs an SM (256 TMEM columns each) cover one another's waits.  Their
+// number is fixed; each takes an equal stretch of all units' work and leaves
+// partial results where it begins or ends inside a unit (q8_kv8_attn.cu).
+// Every wait is bounded (mbar_wait).
+#include "q8_kv8_attn.h"
+
+namespace q8 {
+
+constexpr int KT_KEYS = 64, KT_BLOCKS = KT_KEYS / KV8_BLOCK;
+constexpr int KT_THREADS = 256;  // 16 warps an SM: 128 registers a thread
+constexpr float KT_LIFT = 16384.f;
+constexpr int KT_FIXED = 512;  // work of beginning and ending a unit, in positions
+
+__device__ __forceinline__ void kt_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void kt_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void kt_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void kt_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// Shared-memory matrix descriptors, 128-byte swizzle (layout type 2, version 1),
+// atoms of 8 rows x 128 bytes 1024 apart (SBO).  lbo: bytes between the 64-dim
+// halves of an MN-major operand.
+__device__ __forceinline__ uint64_t kt_desc(uint32_t addr, uint32_t lbo) {
+  return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(lbo >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// d += A B with A from shared memory, and with A from TMEM
+__device__ __forceinline__ void kt_mma_ss(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}\n" ::"r"(d),
+      "l"(da), "l"(db), "r"(idesc), "r"(acc), "r"(0));
+}
+__device__ __forceinline__ void kt_mma_ts(uint32_t d, uint32_t ta, uint64_t db, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}\n" ::"r"(d),
+      "r"(ta), "l"(db), "r"(idesc), "r"(acc), "r"(0));
+}
+
+__device__ __forceinline__ void kt_ld32(uint32_t addr, float (&v)[32]) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+__device__ __forceinline__ void kt_st16(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n" ::"r"(
+          addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void kt_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+template <bool WIDE, int HD>
+struct KtShape {
+  static constexpr int HALVES = HD / 64;            // 64-dim planes of an operand
+  static constexpr int QP = KT_ROWS * 128;          // bytes of a plane of q
+  static constexpr int Q = QP * HALVES * (WIDE ? 2 : 1);
+  static constexpr int KP = KT_KEYS * 128, K = KP * HALVES;
+  static constexpr int SMEM = Q + 2 * K + 1024;     // + alignment
+  static constexpr int REC = KT_ROWS * (HD + 2);
+};
+
+template <bool WIDE, int HD>
+__global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
+  using Sh = KtShape<WIDE, HD>;
+  constexpr int HALVES = Sh::HALVES;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sq_ = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);  // q | k | v
+  uint8_t *sk_ = sq_ + Sh::Q, *sv_ = sk_ + Sh::K;
+  __shared__ __align__(8) uint64_t kfull, kfree, vfull, pvdone, sfull[2], pfull[2], scfull[4];
+  __shared__ uint32_t s_tmem;
+  __shared__ float s_fac[KT_ROWS];
+  __shared__ float4 s_sc[4][KT_BLOCKS];  // sk, lifted sv, log2 sv (-inf: no page)
+  __shared__ int64_t s_scan[KT_THREADS / 32], s_at;
+  __shared__ int s_b;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  pdl_trigger();
+
+  if (threadIdx.x == 0) {
+    mbar_init(&kfull, 4);
+    mbar_init(&kfree, 1);
+    mbar_init(&vfull, 4);
+    mbar_init(&pvdone, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sfull[i], 1);
+      mbar_init(&pfull[i], 4);
+    }
+    for (int i = 0; i < 4; ++i) mbar_init(&scfull[i], 1);
+    fence_barrier_init();
+  }
+  if (warp == 7) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 256;" ::"r"(smem_u32(&s_tmem))
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  kt_fence_before();
+  __syncthreads();
+  kt_fence_after();
+  const uint32_t tmem = s_tmem, tmem_o = tmem + 2 * KT_KEYS;
+
+  // the CTA's stretch of all units' work: a unit (group i of QT tokens, kv head)
+  // weighs KT_FIXED + the positions that its last token sees
+  const int H = a.kv.n_kv * a.hgroups, c = blockIdx.x, nc = gridDim.x;
+  auto sum_to = [&](int64_t base, int64_t i) { return H * (i * (KT_FIXED + base) + a.QT * (i * (i + 1) / 2)); };
+  auto weight = [&](int b) -> int64_t {
+    const Kv8Seq sq = kv8_seq(a.starts, a.ctx, b, a.rows);
+    return sum_to(max(sq.pos0, (int64_t)0), (sq.n + a.QT - 1) / a.QT);
+  };
+  int64_t all = 0, mine = 0;
+  for (int b = threadIdx.x; b < a.S; b += KT_THREADS) all += mine = weight(b);
+  int64_t total;
+  ka_scan(all, s_scan, &total);
+  const int64_t at = total / nc * c + total % nc * c / nc, end = total / nc * (c + 1) + total % nc * (c + 1) / nc;
+  if (threadIdx.x == 0) a.work_meta[2 * c] = a.work_meta[2 * c + 1] = make_int4(-1, 0, 0, 0);
+  int64_t before = 0;
+  for (int b0 = 0; b0 < a.S && at < end; b0 += KT_THREADS) {
+    const int b = b0 + threadIdx.x;
+    if (a.S > KT_THREADS) mine = b < a.S ? weight(b) : 0;
+    int64_t sum;
+    const int64_t to = before + ka_scan(mine, s_scan, &sum);
+    if (to > at && to - mine <= at) {
+      s_b = b;
+      s_at = at - (to - mine);
+    }
+    before += sum;
+    if (before > at) break;
+  }
+  __syncthreads();
+
+  const int ppb = a.kv.page / KV8_BLOCK;
+  const int64_t room = (int64_t)a.max_pages * a.kv.page;
+  const bool aligned = (((uintptr_t)a.q | (uintptr_t)(a.ldq * (WIDE ? 4 : 2))) & 15) == 0;
+  uint32_t T = 0;  // tiles so far: the phases of all barriers
+  int b = at < end ? s_b : 0;
+  int64_t off = at < end ? s_at : 0, left = end - at;
+  while (left > 0 && b < a.S) {
+    const Kv8Seq sq = kv8_seq(a.starts, a.ctx, b, a.rows);
+    const int64_t base = max(sq.pos0, (int64_t)0);
+    const int groups = (sq.n + a.QT - 1) / a.QT;
+    const int64_t w = sum_to(base, groups);
+    while (off < w && left > 0) {
+      int gi = 0;  // the last group whose sum_to is not beyond off
+      for (int hi = groups; hi - gi > 1;) {
+        const int mid = (gi + hi) / 2;
+        if (sum_to(base, mid) <= off) gi = mid;
+        else hi = mid;
+      }
+      const int64_t each = KT_FIXED + base + (int64_t)(gi + 1) * a.QT, rest = off - sum_to(base, gi);
+      const int head = (int)(rest / each);
+      const int64_t w0 = rest - head * each, take = min(left, each - w0);
+      const bool ends = w0 + take == each;
+      const KaUnit u = ka_unit(a, sq, head, gi * a.QT);
+      const int tiles = (u.nblk + KT_BLOCKS - 1) / KT_BLOCKS;
+      const int t0 = (int)min((int64_t)tiles, max(w0 - KT_FIXED, (int64_t)0) / KT_KEYS);
+      const int t1 = ends ? tiles : (int)min((int64_t)tiles, max(w0 + take - KT_FIXED, (int64_t)0) / KT_KEYS);
+      const bool begins = w0 <= KT_FIXED || t0 == 0;
+      off += take;
+      left -= take;
+      if (t1 == 0 && !ends) continue;  // the next CTA begins it
+      const int n = t1 - t0, nrow = u.toks * a.GH;
+      const int32_t* trow = a.table + (int64_t)u.b * a.max_pages;
+
+      // ---- q into shared memory, two threads a row
+      if (threadIdx.x < 2 * KT_ROWS) {
+        constexpr int PART = HD / 2;
+        const int r = threadIdx.x >> 1, d0 = (threadIdx.x & 1) * PART;
+        const bool live = r < nrow && r % a.GH < u.heads;
+        const int64_t i0 = live ? (int64_t)(u.row0 + r / a.GH) * a.ldq + (u.head0 + r % a.GH) * HD + d0 : 0;
+        float top = 0.f;
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = 0.f;
+#pragma unroll 4
+        for (int d = 0; d < PART; d += 8) {
+          if (live) ka_row<WIDE>(x, a.q, i0 + d, a.dtype, aligned);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]));
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        const int k = top > 0.f && top < INFINITY ? min(14 - ilogbf(top), 126) : 0;
+        const float up = scalbnf(1.f, k);
+        if (d0 == 0) s_fac[r] = scalbnf(1.4426950408889634f / sqrtf((float)HD), -k);
+#pragma unroll 2
+        for (int d = 0; d < PART; d += 8) {
+          if (live) ka_row<WIDE>(x, a.q, i0 + d, a.dtype, aligned);
+          uint32_t hi[4], lo[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float y0 = x[2 * e] * up, y1 = x[2 * e + 1] * up;
+            hi[e] = ka_pack(y0, y1);
+            const float2 f = __half22float2(*reinterpret_cast<__half2*>(&hi[e]));
+            lo[e] = ka_pack(y0 - f.x, y1 - f.y);
+          }
+          const int dim = d0 + d;
+          uint8_t* to = sq_ + (dim >> 6) * Sh::QP + r * 128 + ((((dim >> 3) & 7) ^ (r & 7)) << 4);
+          *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          if (WIDE) *reinterpret_cast<uint4*>(to + HALVES * Sh::QP) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncthreads();
+
+      float m = -INFINITY, l = 0.f;
+      if (warp < 4) {
+        // ---- softmax, a thread per row
+        const int r = threadIdx.x;
+        const float fac = s_fac[r];
+        const int lim = r < nrow ? (int)min(max(u.pos0 + r / a.GH + 1, (int64_t)0), room) : 0;
+        const int64_t seen = u.pos0 + 1;  // by the first token: no tile before needs a mask
+        const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+        for (int j = 0; j < n; ++j) {
+          const uint32_t t = T + j, s_at_ = tmem + lanes + (t & 1) * KT_KEYS;
+          const int p0 = (t0 + j) * KT_KEYS;
+          const bool masked = p0 + KT_KEYS > seen;
+          mbar_wait(&scfull[t & 3], (t >> 2) & 1);
+          mbar_wait(&sfull[t & 1], (t >> 1) & 1);
+          kt_fence_after();
+          float top = -INFINITY;
+          float v[32];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            kt_ld32(s_at_ + h * 32, v);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const float4 sc = s_sc[t & 3][h * 2 + k];
+              float bm = -INFINITY;
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                if (!masked || p0 + h * 32 + k * 16 + i < lim) bm = fmaxf(bm, v[k * 16 + i]);
+              // a scale of 0 or a missing page: no 0 x infinity
+              if (bm > -INFINITY) top = fmaxf(top, fmaf(bm, fac * sc.x, sc.z));
+            }
+          }
+          float alpha = 1.f;
+          const bool grew = top > m + 1.f || (m == -INFINITY && top > -INFINITY);
+          if (grew) {
+            alpha = ka_exp2(m - top);
+            m = top;
+            l *= alpha;
+          }
+          mbar_wait(&pvdone, (t & 1) ^ 1);  // O is up to date, and P's other buffer free
+          kt_fence_after();
+          if (j > 0 && __any_sync(0xffffffffu, grew)) {
+#pragma unroll 1
+            for (int h = 0; h < HD / 32; ++h) {
+              kt_ld32(tmem_o + lanes + h * 32, v);
+              uint32_t x[2][16];
+#pragma unroll
+              for (int i = 0; i < 32; ++i) x[i >> 4][i & 15] = __float_as_uint(v[i] * alpha);
+              kt_st16(tmem_o + lanes + h * 32, x[0]);
+              kt_st16(tmem_o + lanes + h * 32 + 16, x[1]);
+            }
+          }
+          const float ref = m == -INFINITY ? 0.f : m;
+          float sum = 0.f;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            kt_ld32(s_at_ + h * 32, v);
+            uint32_t hi[16], lo[16];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const float4 sc = s_sc[t & 3][h * 2 + k];
+              const float f = fac * sc.x;
+              const bool dead = sc.z == -INFINITY;
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                float e[2], p[2];
+#pragma unroll
+                for (int z = 0; z < 2; ++z) {
+                  const int q = k * 16 + 2 * i + z;
+                  e[z] = ka_exp2(fmaf(v[q], f, -ref));
+                  if (dead || (masked && p0 + h * 32 + q >= lim)) e[z] = 0.f;
+                  p[z] = e[z] * sc.y;
+                }
+                sum += e[0] + e[1];
+                const uint32_t x = ka_pack(p[0], p[1]);
+                hi[k * 8 + i] = x;
+                if (WIDE) {
+                  const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&x));
+                  lo[k * 8 + i] = ka_pack(p[0] - y.x, p[1] - y.y);
+                }
+              }
+            }
+            kt_st16(s_at_ + h * 32, hi);
+            if (WIDE) kt_st16(s_at_ + h * 32 + 16, lo);
+          }
+          l += sum;
+          kt_wait_st();
+          kt_fence_before();
+          __syncwarp();
+          if (lane == 0) kt_arrive(&pfull[t & 1]);
+        }
+      } else {
+        // ---- codes to f16, and the products
+        constexpr int CPR = HD / 16, STEP = 128 / CPR, NI = KT_KEYS / STEP;
+        const int ct = threadIdx.x - 128, qd = ct % CPR, r0 = ct / CPR;
+        uint4 kc[NI], vc[NI];
+        float sk = 0.f, sv = 0.f;  // lanes 0-3 of warp 4: of the tile's blocks
+        bool there = false;
+        auto id_of = [&](int blk) {
+          if (blk >= u.nblk) return -1;
+          const int e = trow[blk / ppb];
+          return e >= 0 && e < a.kv.num_pages ? (e * a.kv.n_kv + u.h) * ppb + blk % ppb : -1;
+        };
+        auto load = [&](uint4 (&cs)[NI], const int8_t* codes, int j) {
+          const int b0 = (t0 + j) * KT_BLOCKS;
+#pragma unroll
+          for (int i = 0; i < NI; ++i) {
+            const int row = r0 + i * STEP, id = id_of(b0 + (row >> 4));
+            cs[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (id >= 0)
+              cs[i] = __ldg(reinterpret_cast<const uint4*>(codes + (int64_t)id * (KV8_BLOCK * HD) + (row & 15) * HD +
+                                                           qd * 16));
+          }
+          if (codes == a.kv.k && warp == 4 && lane < KT_BLOCKS) {
+            const int id = id_of(b0 + lane);
+            there = id >= 0;
+            sk = there ? a.kv.k_scale[id] : 0.f;
+            sv = there ? a.kv.v_scale[id] : 0.f;
+          }
+        };
+        auto put = [&](uint8_t* plane0, const uint4 (&cs)[NI]) {
+#pragma unroll
+          for (int i = 0; i < NI; ++i) {
+            const int row = r0 + i * STEP;
+            const uint32_t wd[4] = {cs[i].x ^ 0x80808080u, cs[i].y ^ 0x80808080u, cs[i].z ^ 0x80808080u,
+                                    cs[i].w ^ 0x80808080u};
+            uint4 x[2];
+            x[0] = make_uint4(ka_f16(wd[0], 0x5140), ka_f16(wd[0], 0x5342), ka_f16(wd[1], 0x5140),
+                              ka_f16(wd[1], 0x5342));
+            x[1] = make_uint4(ka_f16(wd[2], 0x5140), ka_f16(wd[2], 0x5342), ka_f16(wd[3], 0x5140),
+                              ka_f16(wd[3], 0x5342));
+            uint8_t* to = plane0 + (qd >> 2) * Sh::KP + row * 128;
+            const int c0 = (2 * qd) & 7, first = (qd >> 2) & 1;  // the planes' lanes take turns: no bank twice
+            *reinterpret_cast<uint4*>(to + (((c0 + first) ^ (row & 7)) << 4)) = first ? x[1] : x[0];
+            *reinterpret_cast<uint4*>(to + (((c0 + 1 - first) ^ (row & 7)) << 4)) = first ? x[0] : x[1];
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+        };
+        // products: f32 sums (bit 4), f16 operands, M = 128; V is MN-major (bit 16)
+        const uint32_t is = (1u << 4) | ((uint32_t)(KT_KEYS >> 3) << 17) | ((uint32_t)(KT_ROWS >> 4) << 24);
+        const uint32_t io = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(KT_ROWS >> 4) << 24);
+        const uint64_t dq = kt_desc(smem_u32(sq_), 16), dk = kt_desc(smem_u32(sk_), 16),
+                       dv = kt_desc(smem_u32(sv_), Sh::KP);
+        if (n > 0) load(kc, a.kv.k, 0);
+        for (int j = 0; j <= n; ++j) {
+          const uint32_t t = T + j;
+          if (j < n) {
+            mbar_wait(&kfree, (t & 1) ^ 1);
+            if (warp == 4) {
+              if (lane < KT_BLOCKS)
+                s_sc[t & 3][lane] = make_float4(sk, sv * KT_LIFT, there ? fmaxf(__log2f(sv), -100.f) : -INFINITY, 0.f);
+              __syncwarp();
+              if (lane == 0) kt_arrive(&scfull[t & 3]);
+            }
+            put(sk_, kc);
+            if (lane == 0) kt_arrive(&kfull);
+            if (j + 1 < n) load(kc, a.kv.k, j + 1);
+            if (warp == 7 && lane == 0) {
+              mbar_wait(&kfull, t & 1);
+              kt_fence_after();
+              const uint32_t d = tmem + (t & 1) * KT_KEYS;
+#pragma unroll
+              for (int x = 0; x < (WIDE ? 2 : 1); ++x)
+#pragma unroll
+                for (int k = 0; k < HD / 16; ++k)  // 16 dims: 32 bytes further inside the swizzle atom
+                  kt_mma_ss(d, dq + (x * HALVES + (k >> 2)) * (Sh::QP >> 4) + (k & 3) * 2,
+                            dk + (k >> 2) * (Sh::KP >> 4) + (k & 3) * 2, is, (x | k) != 0);
+              kt_commit(&kfree);
+              kt_commit(&sfull[t & 1]);
+            }
+            __syncwarp();
+          }
+          if (j > 0) {
+            const uint32_t p = t - 1;  // the tile before
+            mbar_wait(&pvdone, (p & 1) ^ 1);
+            put(sv_, vc);
+            if (lane == 0) kt_arrive(&vfull);
+            if (j < n) load(vc, a.kv.v, j);
+            if (warp == 7 && lane == 0) {
+              mbar_wait(&vfull, p & 1);
+              mbar_wait(&pfull[p & 1], (p >> 1) & 1);
+              kt_fence_after();
+#pragma unroll
+              for (int x = 0; x < (WIDE ? 2 : 1); ++x)
+#pragma unroll
+                for (int k = 0; k < KT_KEYS / 16; ++k)  // 16 positions: two atoms further
+                  kt_mma_ts(tmem_o, tmem + (p & 1) * KT_KEYS + (k >> 1) * 32 + x * 16 + (k & 1) * 8,
+                            dv + k * (2048 >> 4), io, (j != 1) | ((x | k) != 0));
+              kt_commit(&pvdone);
+            }
+            __syncwarp();
+          } else if (n > 0) {
+            load(vc, a.kv.v, 0);
+          }
+        }
+      }
+      __syncwarp();
+      T += n;
+
+      // ---- results
+      if (warp < 4) {
+        const int r = threadIdx.x;
+        const bool whole = begins && ends, live = r < nrow && r % a.GH < u.heads;
+        float* rec = a.work + (int64_t)(2 * c + (begins ? 1 : 0)) * Sh::REC;
+        if (n > 0) {
+          mbar_wait(&pvdone, (T - 1) & 1);
+          kt_fence_after();
+        }
+        const float scale = whole ? (l > 0.f ? 1.f / (KT_LIFT * l) : 0.f * l) : KA_LIFT / KT_LIFT;
+        const int64_t o0 = (int64_t)(u.row0 + r / a.GH) * a.ldo + (int64_t)(u.head0 + r % a.GH) * HD;
+        const bool wide_out = (((uintptr_t)a.out | (uintptr_t)(a.ldo * (WIDE ? 4 : 2))) & 15) == 0;
+#pragma unroll 1
+        for (int h = 0; h < HD / 32; ++h) {
+          float v[32];
+          if (n > 0) {
+            kt_ld32(tmem_o + ((uint32_t)(warp * 32) << 16) + h * 32, v);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = 0.f;
+          }
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] *= scale;
+          if (!whole) {
+            if (r < nrow) {
+#pragma unroll
+              for (int i = 0; i < 32; i += 4)
+                *reinterpret_cast<float4*>(rec + r * HD + h * 32 + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+            }
+          } else if (live) {
+            if (WIDE && wide_out) {
+#pragma unroll
+              for (int i = 0; i < 32; i += 4)
+                *reinterpret_cast<float4*>((float*)a.out + o0 + h * 32 + i) =
+                    make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) ka_store<WIDE>(a, o0 + h * 32 + i, v[i]);
+            }
+          }
+        }
+        if (!whole) {
+          rec[KT_ROWS * HD + r] = m;
+          rec[KT_ROWS * HD + KT_ROWS + r] = l;
+          if (threadIdx.x == 0)
+            a.work_meta[2 * c + (begins ? 1 : 0)] = make_int4(u.row0, u.head0, u.toks | u.heads << 16, ends);
+        }
+        kt_fence_before();
+      }
+      __syncthreads();  // q and O are used again
+      kt_fence_after();
+    }
+    off = 0;
+    ++b;
+  }
+  kt_fence_before();
+  __syncthreads();
+  if (warp == 7) {
+    kt_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 256;" ::"r"(tmem));
+  }
+}
+
+int kv8_attn_tc_ctas() { return 2 * num_sms(); }
+
+template <bool WIDE, int HD>
+static int tc_run(const Kv8AttnArgs& a, int ctas, cudaStream_t st) {
+  using Sh = KtShape<WIDE, HD>;
+  static bool ready[64] = {false};
+  int dev = 0;
+  Q8_CUDA(cudaGetDevice(&dev));
+  if (!ready[dev & 63]) {
+    Q8_CUDA(cudaFuncSetAttribute(k_kv8_attn_tc<WIDE, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM));
+    ready[dev & 63] = true;
+  }
+  k_kv8_attn_tc<WIDE, HD><<<ctas, KT_THREADS, Sh::SMEM, st>>>(a);
+  return launch_check("k_kv8_attn_tc");
+}
+
+int kv8_attn_tc(const Kv8AttnArgs& a, int ctas, cudaStream_t st) {
+  if (a.kv.head_dim == 128) return a.dtype == Q8_F32 ? tc_run<true, 128>(a, ctas, st) : tc_run<false, 128>(a, ctas, st);
+  return a.dtype == Q8_F32 ? tc_run<true, 64>(a, ctas, st) : tc_run<false, 64>(a, ctas, st);
+}
+
+int kv8_attn_tc_poll_error() {
+  int v = 0;
+  Q8_CUDA(cudaMemcpyFromSymbol(&v, g_q8_device_error, sizeof(int)));
+  if (v == 0) return Q8_OK;
+  const int z = 0;
+  Q8_CUDA(cudaMemcpyToSymbol(g_q8_device_error, &z, sizeof(int)));
+  set_error("k_kv8_attn_tc: a barrier wait timed out (device status %d)", v);
+  return v;
+}
+
+}  // namespace q8
