@@ -589,37 +589,44 @@ __global__ void __launch_bounds__(128, KaShape<WIDE, HD, NT>::WARPS / 4) k_kv8_a
 }
 
 // A unit that begins in CTA c and goes on behind it: record 1 of c, then
-// records 0 of the next ones up to the one that ends it.
+// records 0 of the next ones up to the one that ends it.  A warp per row.
 template <bool WIDE, int HD>
 __global__ void __launch_bounds__(256) k_kv8_attn_join(Kv8AttnArgs a, int RMAX) {
+  constexpr int E = HD / 32;
   pdl_wait();
-  const int c = blockIdx.x, nc = gridDim.x, REC = RMAX * (HD + 2);
+  const int c = blockIdx.x, nc = gridDim.x, REC = RMAX * (HD + 2), lane = threadIdx.x & 31;
+  const int r = blockIdx.y * (blockDim.x >> 5) + (threadIdx.x >> 5);
   const int4 me = a.work_meta[2 * c + 1];
-  if (me.x < 0) return;
+  const int toks = me.z & 0xffff, heads = me.z >> 16;
+  if (me.x < 0 || r >= toks * a.GH || r % a.GH >= heads) return;
   int last = c + 1;  // CTAs without work (x < 0) may lie between
   while (last < nc - 1 && !a.work_meta[2 * last].w) ++last;
-  auto there = [&](int i) { return i == c || a.work_meta[2 * i].x >= 0; };
-  const int toks = me.z & 0xffff, heads = me.z >> 16;
-  for (int k = threadIdx.x; k < toks * a.GH * HD; k += blockDim.x) {
-    const int r = k / HD;
-    float mx = -INFINITY;
-    for (int i = c; i <= last; ++i)
-      if (there(i)) mx = fmaxf(mx, a.work[(int64_t)(2 * i + (i == c)) * REC + RMAX * HD + r]);
-    float x = 0.f, sum = 0.f;
-    for (int i = c; i <= last; ++i) {
-      if (!there(i)) continue;
-      const float* rec = a.work + (int64_t)(2 * i + (i == c)) * REC;
-      const float w = rec[RMAX * HD + r] == -INFINITY ? 0.f : exp2f(rec[RMAX * HD + r] - mx);
-      x += w * rec[k];
-      sum += w * rec[RMAX * HD + RMAX + r];
-    }
-    ka_write<WIDE, HD>(a, me.x, me.y, heads, k, x, sum);
+  float mx = -INFINITY, sum = 0.f, x[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) x[e] = 0.f;
+  for (int i = c; i <= last; ++i) {
+    if (i != c && a.work_meta[2 * i].x < 0) continue;
+    const float* rec = a.work + (int64_t)(2 * i + (i == c)) * REC;
+    float v[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = rec[r * HD + lane * E + e];
+    const float m = rec[RMAX * HD + r], l = rec[RMAX * HD + RMAX + r];
+    const float top = fmaxf(mx, m), ref = top == -INFINITY ? 0.f : top;
+    const float f0 = exp2f(mx - ref), f1 = exp2f(m - ref);
+    sum = sum * f0 + l * f1;
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = x[e] * f0 + v[e] * f1;
+    mx = top;
   }
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    ka_write<WIDE, HD>(a, me.x, me.y, heads, r * HD + lane * E + e, x[e], sum);
 }
 
 template <bool WIDE, int HD>
 static int join_run(const Kv8AttnArgs& a, int ctas, int RMAX, cudaStream_t st) {
-  return launch_pdl("k_kv8_attn_join", k_kv8_attn_join<WIDE, HD>, dim3(ctas), dim3(256), 0, st, a, RMAX);
+  return launch_pdl("k_kv8_attn_join", k_kv8_attn_join<WIDE, HD>, dim3(ctas, ceil_div(RMAX, 8)), dim3(256), 0, st, a,
+                    RMAX);
 }
 
 int kv8_attn_join(const Kv8AttnArgs& a, int ctas, int RMAX, cudaStream_t st) {

@@ -87,6 +87,89 @@ __device__ __forceinline__ void kt_st16(uint32_t addr, const uint32_t (&r)[16]) 
 }
 __device__ __forceinline__ void kt_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// two floats in a register pair, and packed operations on them
+__device__ __forceinline__ uint64_t kt_two(float a, float b) {
+  return (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a);
+}
+__device__ __forceinline__ float kt_lo(uint64_t x) { return __uint_as_float((uint32_t)x); }
+__device__ __forceinline__ float kt_hi(uint64_t x) { return __uint_as_float((uint32_t)(x >> 32)); }
+__device__ __forceinline__ uint64_t kt_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t kt_mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t kt_add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+// The largest score + log2(sv) of a row's tile; left: positions of the tile that the row sees.
+template <bool MASKED>
+__device__ __forceinline__ float kt_top(uint32_t addr, const float4* sc, float fac, int left) {
+  float top = -INFINITY;
+#pragma unroll 1
+  for (int h = 0; h < 2; ++h) {
+    float v[32];
+    kt_ld32(addr + h * 32, v);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const float4 s = sc[h * 2 + k];
+      float bm = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (!MASKED || k * 16 + i < left - h * 32) bm = fmaxf(bm, v[k * 16 + i]);
+      if (!MASKED || bm > -INFINITY) top = fmaxf(top, fmaf(bm, fac * s.x, s.z));  // masked: no 0 x infinity
+    }
+  }
+  return top;
+}
+
+// Scores -> weights, in place; returns their sum before sv.
+template <bool WIDE, bool MASKED>
+__device__ __forceinline__ float kt_weights(uint32_t addr, const float4* sc, float fac, float ref, int left) {
+  uint64_t sum = 0ull;
+  const uint64_t minus = kt_two(-1.f, -1.f);
+#pragma unroll 1
+  for (int h = 0; h < 2; ++h) {
+    float v[32];
+    kt_ld32(addr + h * 32, v);
+    uint32_t hi[16], lo[16];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const float4 s = sc[h * 2 + k];
+      const float f = fac * s.x, b = s.z == -INFINITY ? -INFINITY : -ref;  // a missing page: 0 s - infinity
+      const uint64_t f2 = kt_two(f, f), b2 = kt_two(b, b), w2 = kt_two(s.y, s.y);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int q = k * 16 + 2 * i;
+        const uint64_t x = kt_fma2(kt_two(v[q], v[q + 1]), f2, b2);
+        float e0 = ka_exp2(kt_lo(x)), e1 = ka_exp2(kt_hi(x));
+        if (MASKED) {
+          if (q >= left - h * 32) e0 = 0.f;
+          if (q + 1 >= left - h * 32) e1 = 0.f;
+        }
+        const uint64_t e = kt_two(e0, e1), p = kt_mul2(e, w2);
+        sum = kt_add2(sum, e);
+        hi[k * 8 + i] = ka_pack(kt_lo(p), kt_hi(p));
+        if (WIDE) {
+          const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&hi[k * 8 + i]));
+          const uint64_t r = kt_fma2(kt_two(y.x, y.y), minus, p);
+          lo[k * 8 + i] = ka_pack(kt_lo(r), kt_hi(r));
+        }
+      }
+    }
+    kt_st16(addr + h * 32, hi);
+    if (WIDE) kt_st16(addr + h * 32 + 16, lo);
+  }
+  return kt_lo(sum) + kt_hi(sum);
+}
+
 template <bool WIDE, int HD>
 struct KtShape {
   static constexpr int HALVES = HD / 64;            // 64-dim planes of an operand
@@ -252,22 +335,9 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
           mbar_wait(&scfull[t & 3], (t >> 2) & 1);
           mbar_wait(&sfull[t & 1], (t >> 1) & 1);
           kt_fence_after();
-          float top = -INFINITY;
-          float v[32];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            kt_ld32(s_at_ + h * 32, v);
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const float4 sc = s_sc[t & 3][h * 2 + k];
-              float bm = -INFINITY;
-#pragma unroll
-              for (int i = 0; i < 16; ++i)
-                if (!masked || p0 + h * 32 + k * 16 + i < lim) bm = fmaxf(bm, v[k * 16 + i]);
-              // a scale of 0 or a missing page: no 0 x infinity
-              if (bm > -INFINITY) top = fmaxf(top, fmaf(bm, fac * sc.x, sc.z));
-            }
-          }
+          const int left = lim - p0;
+          const float top = masked ? kt_top<true>(s_at_, s_sc[t & 3], fac, left)
+                                   : kt_top<false>(s_at_, s_sc[t & 3], fac, left);
           float alpha = 1.f;
           const bool grew = top > m + 1.f || (m == -INFINITY && top > -INFINITY);
           if (grew) {
@@ -275,11 +345,12 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
             m = top;
             l *= alpha;
           }
-          mbar_wait(&pvdone, (t & 1) ^ 1);  // O is up to date, and P's other buffer free
-          kt_fence_after();
           if (j > 0 && __any_sync(0xffffffffu, grew)) {
+            mbar_wait(&pvdone, (t & 1) ^ 1);  // O is up to date
+            kt_fence_after();
 #pragma unroll 1
             for (int h = 0; h < HD / 32; ++h) {
+              float v[32];
               kt_ld32(tmem_o + lanes + h * 32, v);
               uint32_t x[2][16];
 #pragma unroll
@@ -289,39 +360,8 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
             }
           }
           const float ref = m == -INFINITY ? 0.f : m;
-          float sum = 0.f;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            kt_ld32(s_at_ + h * 32, v);
-            uint32_t hi[16], lo[16];
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const float4 sc = s_sc[t & 3][h * 2 + k];
-              const float f = fac * sc.x;
-              const bool dead = sc.z == -INFINITY;
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                float e[2], p[2];
-#pragma unroll
-                for (int z = 0; z < 2; ++z) {
-                  const int q = k * 16 + 2 * i + z;
-                  e[z] = ka_exp2(fmaf(v[q], f, -ref));
-                  if (dead || (masked && p0 + h * 32 + q >= lim)) e[z] = 0.f;
-                  p[z] = e[z] * sc.y;
-                }
-                sum += e[0] + e[1];
-                const uint32_t x = ka_pack(p[0], p[1]);
-                hi[k * 8 + i] = x;
-                if (WIDE) {
-                  const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&x));
-                  lo[k * 8 + i] = ka_pack(p[0] - y.x, p[1] - y.y);
-                }
-              }
-            }
-            kt_st16(s_at_ + h * 32, hi);
-            if (WIDE) kt_st16(s_at_ + h * 32 + 16, lo);
-          }
-          l += sum;
+          l += masked ? kt_weights<WIDE, true>(s_at_, s_sc[t & 3], fac, ref, left)
+                      : kt_weights<WIDE, false>(s_at_, s_sc[t & 3], fac, ref, left);
           kt_wait_st();
           kt_fence_before();
           __syncwarp();
@@ -334,26 +374,29 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
         uint4 kc[NI], vc[NI];
         float sk = 0.f, sv = 0.f;  // lanes 0-3 of warp 4: of the tile's blocks
         bool there = false;
-        auto id_of = [&](int blk) {
-          if (blk >= u.nblk) return -1;
-          const int e = trow[blk / ppb];
-          return e >= 0 && e < a.kv.num_pages ? (e * a.kv.n_kv + u.h) * ppb + blk % ppb : -1;
+        int idk = -1, idv = -1;  // lanes 0-3: the blocks of the next tile of K, of V
+        auto look_up = [&](int j) {  // of K; V's are the ones before
+          idv = idk;
+          idk = -1;
+          const int blk = (t0 + j) * KT_BLOCKS + lane;
+          if (lane < KT_BLOCKS && blk < u.nblk) {
+            const int e = trow[(uint32_t)blk / (uint32_t)ppb];
+            if (e >= 0 && e < a.kv.num_pages) idk = (e * a.kv.n_kv + u.h) * ppb + (uint32_t)blk % (uint32_t)ppb;
+          }
+          if (warp == 4) {
+            there = idk >= 0;
+            sk = there ? a.kv.k_scale[idk] : 0.f;
+            sv = there ? a.kv.v_scale[idk] : 0.f;
+          }
         };
-        auto load = [&](uint4 (&cs)[NI], const int8_t* codes, int j) {
-          const int b0 = (t0 + j) * KT_BLOCKS;
+        auto load = [&](uint4 (&cs)[NI], const int8_t* codes, int ids) {
 #pragma unroll
           for (int i = 0; i < NI; ++i) {
-            const int row = r0 + i * STEP, id = id_of(b0 + (row >> 4));
+            const int row = r0 + i * STEP, id = __shfl_sync(0xffffffffu, ids, row >> 4);
             cs[i] = make_uint4(0u, 0u, 0u, 0u);
             if (id >= 0)
               cs[i] = __ldg(reinterpret_cast<const uint4*>(codes + (int64_t)id * (KV8_BLOCK * HD) + (row & 15) * HD +
                                                            qd * 16));
-          }
-          if (codes == a.kv.k && warp == 4 && lane < KT_BLOCKS) {
-            const int id = id_of(b0 + lane);
-            there = id >= 0;
-            sk = there ? a.kv.k_scale[id] : 0.f;
-            sv = there ? a.kv.v_scale[id] : 0.f;
           }
         };
         auto put = [&](uint8_t* plane0, const uint4 (&cs)[NI]) {
@@ -380,7 +423,11 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
         const uint32_t io = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(KT_ROWS >> 4) << 24);
         const uint64_t dq = kt_desc(smem_u32(sq_), 16), dk = kt_desc(smem_u32(sk_), 16),
                        dv = kt_desc(smem_u32(sv_), Sh::KP);
-        if (n > 0) load(kc, a.kv.k, 0);
+        if (n > 0) {
+          look_up(0);
+          load(kc, a.kv.k, idk);
+          load(vc, a.kv.v, idk);
+        }
         for (int j = 0; j <= n; ++j) {
           const uint32_t t = T + j;
           if (j < n) {
@@ -393,7 +440,6 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
             }
             put(sk_, kc);
             if (lane == 0) kt_arrive(&kfull);
-            if (j + 1 < n) load(kc, a.kv.k, j + 1);
             if (warp == 7 && lane == 0) {
               mbar_wait(&kfull, t & 1);
               kt_fence_after();
@@ -408,13 +454,16 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
               kt_commit(&sfull[t & 1]);
             }
             __syncwarp();
+            if (j + 1 < n) {
+              look_up(j + 1);
+              load(kc, a.kv.k, idk);
+            }
           }
           if (j > 0) {
             const uint32_t p = t - 1;  // the tile before
             mbar_wait(&pvdone, (p & 1) ^ 1);
             put(sv_, vc);
             if (lane == 0) kt_arrive(&vfull);
-            if (j < n) load(vc, a.kv.v, j);
             if (warp == 7 && lane == 0) {
               mbar_wait(&vfull, p & 1);
               mbar_wait(&pfull[p & 1], (p >> 1) & 1);
@@ -428,8 +477,7 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
               kt_commit(&pvdone);
             }
             __syncwarp();
-          } else if (n > 0) {
-            load(vc, a.kv.v, 0);
+            if (j < n) load(vc, a.kv.v, j + 1 < n ? idv : idk);
           }
         }
       }
