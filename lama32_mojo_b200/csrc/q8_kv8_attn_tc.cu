@@ -7,9 +7,9 @@
 // tiles of 64 positions, four scale blocks:
 //   warps 4-7  load the tile's codes and write them as f16 (exact) into shared
 //              memory, rows of 64 dims in the 128-byte swizzle; K is read
-//              K-major, V (same layout) MN-major.  One lane of warp 7 issues
-//              S = Q K^T (128 x 64 x hd) into TMEM behind K, and O += P V
-//              (128 x hd x 64, P read from TMEM) behind V of the tile before.
+//              K-major, V (same layout) MN-major.
+//   warp 8     one lane issues S = Q K^T (128 x 64 x hd) into TMEM and, once the
+//              weights are there, O += P V (128 x hd x 64), P read from TMEM.
 //   warps 0-3  a thread per row: reads its 64 scores from TMEM, keeps M and l,
 //              writes P over them.  S / P have two buffers, so the next tile's
 //              scores are computed meanwhile.
@@ -27,7 +27,7 @@
 namespace q8 {
 
 constexpr int KT_KEYS = 64, KT_BLOCKS = KT_KEYS / KV8_BLOCK;
-constexpr int KT_THREADS = 256;  // 16 warps an SM: 128 registers a thread
+constexpr int KT_THREADS = 288;
 constexpr float KT_LIFT = 16384.f;
 constexpr int KT_FIXED = 512;  // work of beginning and ending a unit, in positions
 
@@ -40,6 +40,15 @@ __device__ __forceinline__ void kt_commit(uint64_t* bar) {
 }
 __device__ __forceinline__ void kt_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void kt_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// One lane of a converged warp.  Products are issued under this predicate rather
+// than a lane's number: their descriptors then stay in uniform registers (110
+// clocks each otherwise, whatever their size; measured).
+__device__ __forceinline__ bool kt_elect() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+  return p != 0;
+}
 
 // Shared-memory matrix descriptors, 128-byte swizzle (layout type 2, version 1),
 // atoms of 8 rows x 128 bytes 1024 apart (SBO).  lbo: bytes between the 64-dim
@@ -208,7 +217,7 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
     for (int i = 0; i < 4; ++i) mbar_init(&scfull[i], 1);
     fence_barrier_init();
   }
-  if (warp == 7) {
+  if (warp == 8) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 256;" ::"r"(smem_u32(&s_tmem))
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -367,27 +376,26 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
           __syncwarp();
           if (lane == 0) kt_arrive(&pfull[t & 1]);
         }
-      } else {
-        // ---- codes to f16, and the products
+      } else if (warp < 8) {
+        // ---- codes to f16
         constexpr int CPR = HD / 16, STEP = 128 / CPR, NI = KT_KEYS / STEP;
         const int ct = threadIdx.x - 128, qd = ct % CPR, r0 = ct / CPR;
         uint4 kc[NI], vc[NI];
-        float sk = 0.f, sv = 0.f;  // lanes 0-3 of warp 4: of the tile's blocks
-        bool there = false;
-        int idk = -1, idv = -1;  // lanes 0-3: the blocks of the next tile of K, of V
-        auto look_up = [&](int j) {  // of K; V's are the ones before
-          idv = idk;
-          idk = -1;
+        // lanes 0-3: table entries of a tile's blocks, asked for long before their use, and pool numbers (-1: no page)
+        auto look_up = [&](int j) {
           const int blk = (t0 + j) * KT_BLOCKS + lane;
-          if (lane < KT_BLOCKS && blk < u.nblk) {
-            const int e = trow[(uint32_t)blk / (uint32_t)ppb];
-            if (e >= 0 && e < a.kv.num_pages) idk = (e * a.kv.n_kv + u.h) * ppb + (uint32_t)blk % (uint32_t)ppb;
-          }
-          if (warp == 4) {
-            there = idk >= 0;
-            sk = there ? a.kv.k_scale[idk] : 0.f;
-            sv = there ? a.kv.v_scale[idk] : 0.f;
-          }
+          return lane < KT_BLOCKS && j < n && blk < u.nblk ? trow[(uint32_t)blk / (uint32_t)ppb] : -1;
+        };
+        auto id_of = [&](int e, int j) {
+          const uint32_t blk = (t0 + j) * KT_BLOCKS + lane;
+          return e >= 0 && e < a.kv.num_pages ? (e * a.kv.n_kv + u.h) * ppb + (int)(blk % (uint32_t)ppb) : -1;
+        };
+        // of tiles j (V), j + 1 (K) and, by their entries, j + 2
+        int id0 = id_of(look_up(0), 0), id1 = id_of(look_up(1), 1), e2 = look_up(2);
+        float sk = 0.f, sv = 0.f;
+        auto scales = [&](int id) {
+          sk = id >= 0 ? a.kv.k_scale[id] : 0.f;
+          sv = id >= 0 ? a.kv.v_scale[id] : 0.f;
         };
         auto load = [&](uint4 (&cs)[NI], const int8_t* codes, int ids) {
 #pragma unroll
@@ -418,32 +426,55 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
         };
-        // products: f32 sums (bit 4), f16 operands, M = 128; V is MN-major (bit 16)
+        auto scales_out = [&](uint32_t t, int id) {
+          if (warp != 4) return;
+          if (lane < KT_BLOCKS)
+            s_sc[t & 3][lane] = make_float4(sk, sv * KT_LIFT, id >= 0 ? fmaxf(__log2f(sv), -100.f) : -INFINITY, 0.f);
+          __syncwarp();
+          if (lane == 0) kt_arrive(&scfull[t & 3]);
+        };
+        load(kc, a.kv.k, id0);
+        load(vc, a.kv.v, id0);
+        if (warp == 4) scales(id0);
+        if (n > 0) {  // K of the first tile
+          mbar_wait(&kfree, (T & 1) ^ 1);
+          scales_out(T, id0);
+          put(sk_, kc);
+          if (lane == 0) kt_arrive(&kfull);
+          load(kc, a.kv.k, id1);
+          if (warp == 4) scales(id1);
+        }
+        for (int j = 0; j < n; ++j) {  // K of tile j + 1, then V of tile j; their registers are loaded again at once
+          const uint32_t t = T + j;
+          const int id2 = id_of(e2, j + 2);
+          e2 = look_up(j + 3);
+          if (j + 1 < n) {
+            mbar_wait(&kfree, t & 1);
+            scales_out(t + 1, id1);
+            put(sk_, kc);
+            if (lane == 0) kt_arrive(&kfull);
+            load(kc, a.kv.k, id2);
+            if (warp == 4) scales(id2);
+          }
+          mbar_wait(&pvdone, (t & 1) ^ 1);
+          put(sv_, vc);
+          if (lane == 0) kt_arrive(&vfull);
+          load(vc, a.kv.v, id1);
+          id1 = id2;
+        }
+      } else {
+        // ---- products: f32 sums (bit 4), f16 operands, M = 128; V is MN-major (bit 16)
         const uint32_t is = (1u << 4) | ((uint32_t)(KT_KEYS >> 3) << 17) | ((uint32_t)(KT_ROWS >> 4) << 24);
         const uint32_t io = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(KT_ROWS >> 4) << 24);
         const uint64_t dq = kt_desc(smem_u32(sq_), 16), dk = kt_desc(smem_u32(sk_), 16),
                        dv = kt_desc(smem_u32(sv_), Sh::KP);
-        if (n > 0) {
-          look_up(0);
-          load(kc, a.kv.k, idk);
-          load(vc, a.kv.v, idk);
-        }
         for (int j = 0; j <= n; ++j) {
           const uint32_t t = T + j;
-          if (j < n) {
-            mbar_wait(&kfree, (t & 1) ^ 1);
-            if (warp == 4) {
-              if (lane < KT_BLOCKS)
-                s_sc[t & 3][lane] = make_float4(sk, sv * KT_LIFT, there ? fmaxf(__log2f(sv), -100.f) : -INFINITY, 0.f);
-              __syncwarp();
-              if (lane == 0) kt_arrive(&scfull[t & 3]);
-            }
-            put(sk_, kc);
-            if (lane == 0) kt_arrive(&kfull);
-            if (warp == 7 && lane == 0) {
-              mbar_wait(&kfull, t & 1);
-              kt_fence_after();
-              const uint32_t d = tmem + (t & 1) * KT_KEYS;
+          if (j < n) {  // scores of tile j
+            mbar_wait(&kfull, t & 1);
+            kt_fence_after();
+            const uint32_t d = tmem + (t & 1) * KT_KEYS;
+            if (kt_elect()) {
 #pragma unroll
               for (int x = 0; x < (WIDE ? 2 : 1); ++x)
 #pragma unroll
@@ -454,20 +485,13 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
               kt_commit(&sfull[t & 1]);
             }
             __syncwarp();
-            if (j + 1 < n) {
-              look_up(j + 1);
-              load(kc, a.kv.k, idk);
-            }
           }
-          if (j > 0) {
-            const uint32_t p = t - 1;  // the tile before
-            mbar_wait(&pvdone, (p & 1) ^ 1);
-            put(sv_, vc);
-            if (lane == 0) kt_arrive(&vfull);
-            if (warp == 7 && lane == 0) {
-              mbar_wait(&vfull, p & 1);
-              mbar_wait(&pfull[p & 1], (p >> 1) & 1);
-              kt_fence_after();
+          if (j > 0) {  // outputs of the tile before
+            const uint32_t p = t - 1;
+            mbar_wait(&vfull, p & 1);
+            mbar_wait(&pfull[p & 1], (p >> 1) & 1);
+            kt_fence_after();
+            if (kt_elect()) {
 #pragma unroll
               for (int x = 0; x < (WIDE ? 2 : 1); ++x)
 #pragma unroll
@@ -477,7 +501,6 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
               kt_commit(&pvdone);
             }
             __syncwarp();
-            if (j < n) load(vc, a.kv.v, j + 1 < n ? idv : idk);
           }
         }
       }
@@ -541,7 +564,7 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
   }
   kt_fence_before();
   __syncthreads();
-  if (warp == 7) {
+  if (warp == 8) {
     kt_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 256;" ::"r"(tmem));
   }
