@@ -189,6 +189,59 @@ struct KtShape {
   static constexpr int REC = KT_ROWS * (HD + 2);
 };
 
+// The units of a CTA's stretch, one after the other.  A unit (group of QT tokens,
+// kv head) weighs KT_FIXED + the positions that its last token sees; units are
+// ordered by (sequence, group, kv head).  Every warp walks for itself.
+struct KtWalk {
+  int b;
+  int64_t off, left;
+  // the unit
+  KaUnit u;
+  int t0, n;  // its tiles here
+  bool begins, ends;
+
+  static __device__ __forceinline__ int64_t sum_to(const Kv8AttnArgs& a, int64_t base, int64_t i) {
+    return (int64_t)a.kv.n_kv * a.hgroups * (i * (KT_FIXED + base) + a.QT * (i * (i + 1) / 2));
+  }
+  static __device__ __forceinline__ int64_t weight(const Kv8AttnArgs& a, int b) {
+    const Kv8Seq sq = kv8_seq(a.starts, a.ctx, b, a.rows);
+    return sum_to(a, max(sq.pos0, (int64_t)0), (sq.n + a.QT - 1) / a.QT);
+  }
+
+  __device__ __forceinline__ bool next(const Kv8AttnArgs& a) {
+    while (left > 0 && b < a.S) {
+      const Kv8Seq sq = kv8_seq(a.starts, a.ctx, b, a.rows);
+      const int64_t base = max(sq.pos0, (int64_t)0);
+      const int groups = (sq.n + a.QT - 1) / a.QT;
+      const int64_t w = sum_to(a, base, groups);
+      while (off < w && left > 0) {
+        int gi = 0;  // the last group whose sum_to is not beyond off
+        for (int hi = groups; hi - gi > 1;) {
+          const int mid = (gi + hi) / 2;
+          if (sum_to(a, base, mid) <= off) gi = mid;
+          else hi = mid;
+        }
+        const int64_t each = KT_FIXED + base + (int64_t)(gi + 1) * a.QT, rest = off - sum_to(a, base, gi);
+        const int head = (int)(rest / each);
+        const int64_t w0 = rest - head * each, take = min(left, each - w0);
+        ends = w0 + take == each;
+        u = ka_unit(a, sq, head, gi * a.QT);
+        const int tiles = (u.nblk + KT_BLOCKS - 1) / KT_BLOCKS;
+        t0 = (int)min((int64_t)tiles, max(w0 - KT_FIXED, (int64_t)0) / KT_KEYS);
+        const int t1 = ends ? tiles : (int)min((int64_t)tiles, max(w0 + take - KT_FIXED, (int64_t)0) / KT_KEYS);
+        begins = w0 <= KT_FIXED || t0 == 0;
+        n = t1 - t0;
+        off += take;
+        left -= take;
+        if (t1 > 0 || ends) return true;  // else the next CTA begins it
+      }
+      off = 0;
+      ++b;
+    }
+    return false;
+  }
+};
+
 template <bool WIDE, int HD>
 __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
   using Sh = KtShape<WIDE, HD>;
@@ -196,7 +249,7 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sq_ = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);  // q | k | v
   uint8_t *sk_ = sq_ + Sh::Q, *sv_ = sk_ + Sh::K;
-  __shared__ __align__(8) uint64_t kfull, kfree, vfull, pvdone, sfull[2], pfull[2], scfull[4];
+  __shared__ __align__(8) uint64_t qfull, kfull, kfree, vfull, pvdone, sfull[2], pfull[2], scfull[4];
   __shared__ uint32_t s_tmem;
   __shared__ float s_fac[KT_ROWS];
   __shared__ float4 s_sc[4][KT_BLOCKS];  // sk, lifted sv, log2 sv (-inf: no page)
@@ -206,6 +259,7 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
   pdl_trigger();
 
   if (threadIdx.x == 0) {
+    mbar_init(&qfull, 4);
     mbar_init(&kfull, 4);
     mbar_init(&kfree, 1);
     mbar_init(&vfull, 4);
@@ -227,16 +281,10 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
   kt_fence_after();
   const uint32_t tmem = s_tmem, tmem_o = tmem + 2 * KT_KEYS;
 
-  // the CTA's stretch of all units' work: a unit (group i of QT tokens, kv head)
-  // weighs KT_FIXED + the positions that its last token sees
-  const int H = a.kv.n_kv * a.hgroups, c = blockIdx.x, nc = gridDim.x;
-  auto sum_to = [&](int64_t base, int64_t i) { return H * (i * (KT_FIXED + base) + a.QT * (i * (i + 1) / 2)); };
-  auto weight = [&](int b) -> int64_t {
-    const Kv8Seq sq = kv8_seq(a.starts, a.ctx, b, a.rows);
-    return sum_to(max(sq.pos0, (int64_t)0), (sq.n + a.QT - 1) / a.QT);
-  };
+  // where the CTA's stretch begins
+  const int c = blockIdx.x, nc = gridDim.x;
   int64_t all = 0, mine = 0;
-  for (int b = threadIdx.x; b < a.S; b += KT_THREADS) all += mine = weight(b);
+  for (int b = threadIdx.x; b < a.S; b += KT_THREADS) all += mine = KtWalk::weight(a, b);
   int64_t total;
   ka_scan(all, s_scan, &total);
   const int64_t at = total / nc * c + total % nc * c / nc, end = total / nc * (c + 1) + total % nc * (c + 1) / nc;
@@ -244,7 +292,7 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
   int64_t before = 0;
   for (int b0 = 0; b0 < a.S && at < end; b0 += KT_THREADS) {
     const int b = b0 + threadIdx.x;
-    if (a.S > KT_THREADS) mine = b < a.S ? weight(b) : 0;
+    if (a.S > KT_THREADS) mine = b < a.S ? KtWalk::weight(a, b) : 0;
     int64_t sum;
     const int64_t to = before + ka_scan(mine, s_scan, &sum);
     if (to > at && to - mine <= at) {
@@ -255,312 +303,332 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
     if (before > at) break;
   }
   __syncthreads();
+  KtWalk w;
+  w.b = at < end ? s_b : 0;
+  w.off = at < end ? s_at : 0;
+  w.left = end - at;
 
-  const int ppb = a.kv.page / KV8_BLOCK;
-  const int64_t room = (int64_t)a.max_pages * a.kv.page;
-  const bool aligned = (((uintptr_t)a.q | (uintptr_t)(a.ldq * (WIDE ? 4 : 2))) & 15) == 0;
-  uint32_t T = 0;  // tiles so far: the phases of all barriers
-  int b = at < end ? s_b : 0;
-  int64_t off = at < end ? s_at : 0, left = end - at;
-  while (left > 0 && b < a.S) {
-    const Kv8Seq sq = kv8_seq(a.starts, a.ctx, b, a.rows);
-    const int64_t base = max(sq.pos0, (int64_t)0);
-    const int groups = (sq.n + a.QT - 1) / a.QT;
-    const int64_t w = sum_to(base, groups);
-    while (off < w && left > 0) {
-      int gi = 0;  // the last group whose sum_to is not beyond off
-      for (int hi = groups; hi - gi > 1;) {
-        const int mid = (gi + hi) / 2;
-        if (sum_to(base, mid) <= off) gi = mid;
-        else hi = mid;
-      }
-      const int64_t each = KT_FIXED + base + (int64_t)(gi + 1) * a.QT, rest = off - sum_to(base, gi);
-      const int head = (int)(rest / each);
-      const int64_t w0 = rest - head * each, take = min(left, each - w0);
-      const bool ends = w0 + take == each;
-      const KaUnit u = ka_unit(a, sq, head, gi * a.QT);
-      const int tiles = (u.nblk + KT_BLOCKS - 1) / KT_BLOCKS;
-      const int t0 = (int)min((int64_t)tiles, max(w0 - KT_FIXED, (int64_t)0) / KT_KEYS);
-      const int t1 = ends ? tiles : (int)min((int64_t)tiles, max(w0 + take - KT_FIXED, (int64_t)0) / KT_KEYS);
-      const bool begins = w0 <= KT_FIXED || t0 == 0;
-      off += take;
-      left -= take;
-      if (t1 == 0 && !ends) continue;  // the next CTA begins it
-      const int n = t1 - t0, nrow = u.toks * a.GH;
-      const int32_t* trow = a.table + (int64_t)u.b * a.max_pages;
-
-      // ---- q into shared memory, two threads a row
-      if (threadIdx.x < 2 * KT_ROWS) {
-        constexpr int PART = HD / 2;
-        const int r = threadIdx.x >> 1, d0 = (threadIdx.x & 1) * PART;
-        const bool live = r < nrow && r % a.GH < u.heads;
-        const int64_t i0 = live ? (int64_t)(u.row0 + r / a.GH) * a.ldq + (u.head0 + r % a.GH) * HD + d0 : 0;
-        float top = 0.f;
-        float x[8];
+  // T counts tiles, U units with tiles: the phases of all barriers.  No role waits for
+  // another but through them; q's buffer is free once the scores of a unit's
+  // last tile have been read, O once the softmax warps have taken it, before
+  // they announce the next unit's first weights.
+  uint32_t T = 0;
+  if (warp < 4) {
+    // ---- softmax, a thread per row
+    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+    const int r = threadIdx.x;
+    const int64_t room = (int64_t)a.max_pages * a.kv.page;
+    const bool aligned = (((uintptr_t)a.q | (uintptr_t)(a.ldq * (WIDE ? 4 : 2))) & 15) == 0;
+    const bool wide_out = (((uintptr_t)a.out | (uintptr_t)(a.ldo * (WIDE ? 4 : 2))) & 15) == 0;
+    while (w.next(a)) {
+      const int nrow = w.u.toks * a.GH;
+      // q into shared memory: a warp its 32 rows, eight at a time, a lane HD / 32 dims of each
+      constexpr int E = HD / 32;
+#pragma unroll 1
+      for (int i0 = 0; i0 < 32 && w.n > 0; i0 += 8) {
+        float x[8][E];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = 0.f;
-#pragma unroll 4
-        for (int d = 0; d < PART; d += 8) {
-          if (live) ka_row<WIDE>(x, a.q, i0 + d, a.dtype, aligned);
+        for (int i = 0; i < 8; ++i) {
+          const int row = warp * 32 + i0 + i;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]));
+          for (int e = 0; e < E; ++e) x[i][e] = 0.f;
+          if (row >= nrow || row % a.GH >= w.u.heads) continue;
+          const int64_t at_q = (int64_t)(w.u.row0 + row / a.GH) * a.ldq + (w.u.head0 + row % a.GH) * HD + lane * E;
+          if constexpr (WIDE) {
+            const float* p = (const float*)a.q + at_q;
+            if (E == 4 && aligned) {
+              const float4 f = *reinterpret_cast<const float4*>(p);
+              x[i][0] = f.x, x[i][1] = f.y, x[i][E - 2] = f.z, x[i][E - 1] = f.w;
+            } else {
+#pragma unroll
+              for (int e = 0; e < E; ++e) x[i][e] = p[e];
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+              const uint16_t h = ((const uint16_t*)a.q)[at_q + e];
+              x[i][e] = a.dtype == Q8_BF16 ? bf16_bits_to_f32(h) : __half2float(__ushort_as_half(h));
+            }
+          }
         }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        const int k = top > 0.f && top < INFINITY ? min(14 - ilogbf(top), 126) : 0;
-        const float up = scalbnf(1.f, k);
-        if (d0 == 0) s_fac[r] = scalbnf(1.4426950408889634f / sqrtf((float)HD), -k);
-#pragma unroll 2
-        for (int d = 0; d < PART; d += 8) {
-          if (live) ka_row<WIDE>(x, a.q, i0 + d, a.dtype, aligned);
-          uint32_t hi[4], lo[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float y0 = x[2 * e] * up, y1 = x[2 * e + 1] * up;
+        for (int i = 0; i < 8; ++i) {
+          const int row = warp * 32 + i0 + i;
+          // the largest |q| into [2^14, 2^15): times 2^k, k from its exponent, at most 126
+          unsigned top = 0u;
+#pragma unroll
+          for (int e = 0; e < E; ++e) top = max(top, __float_as_uint(x[i][e]) & 0x7fffffffu);
+          top = __reduce_max_sync(0xffffffffu, top);
+          const int ex = top >> 23, k = top == 0u || ex == 255 ? 0 : min(141 - ex, 126);
+          const float up = __uint_as_float((unsigned)(127 + k) << 23);
+          if (lane == 0)
+            s_fac[row] = 1.4426950408889634f / (HD == 64 ? 8.f : 11.313708498984761f) *
+                         __uint_as_float((unsigned)(127 - k) << 23);
+          uint32_t hi[E / 2], lo[E / 2];
+#pragma unroll
+          for (int e = 0; e < E / 2; ++e) {
+            const float y0 = x[i][2 * e] * up, y1 = x[i][2 * e + 1] * up;
             hi[e] = ka_pack(y0, y1);
             const float2 f = __half22float2(*reinterpret_cast<__half2*>(&hi[e]));
             lo[e] = ka_pack(y0 - f.x, y1 - f.y);
           }
-          const int dim = d0 + d;
-          uint8_t* to = sq_ + (dim >> 6) * Sh::QP + r * 128 + ((((dim >> 3) & 7) ^ (r & 7)) << 4);
-          *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-          if (WIDE) *reinterpret_cast<uint4*>(to + HALVES * Sh::QP) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          const int dim = lane * E;
+          uint8_t* to = sq_ + (dim >> 6) * Sh::QP + row * 128 + ((((dim >> 3) & 7) ^ (row & 7)) << 4) + (dim & 7) * 2;
+          if constexpr (E == 4) {
+            *reinterpret_cast<uint2*>(to) = make_uint2(hi[0], hi[E / 2 - 1]);
+            if (WIDE) *reinterpret_cast<uint2*>(to + HALVES * Sh::QP) = make_uint2(lo[0], lo[E / 2 - 1]);
+          } else {
+            *reinterpret_cast<uint32_t*>(to) = hi[0];
+            if (WIDE) *reinterpret_cast<uint32_t*>(to + HALVES * Sh::QP) = lo[0];
+          }
         }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncthreads();
+      __syncwarp();
+      if (lane == 0 && w.n > 0) kt_arrive(&qfull);
 
       float m = -INFINITY, l = 0.f;
-      if (warp < 4) {
-        // ---- softmax, a thread per row
-        const int r = threadIdx.x;
-        const float fac = s_fac[r];
-        const int lim = r < nrow ? (int)min(max(u.pos0 + r / a.GH + 1, (int64_t)0), room) : 0;
-        const int64_t seen = u.pos0 + 1;  // by the first token: no tile before needs a mask
-        const uint32_t lanes = (uint32_t)(warp * 32) << 16;
-        for (int j = 0; j < n; ++j) {
-          const uint32_t t = T + j, s_at_ = tmem + lanes + (t & 1) * KT_KEYS;
-          const int p0 = (t0 + j) * KT_KEYS;
-          const bool masked = p0 + KT_KEYS > seen;
-          mbar_wait(&scfull[t & 3], (t >> 2) & 1);
-          mbar_wait(&sfull[t & 1], (t >> 1) & 1);
+      const float fac = s_fac[r];
+      const int lim = r < nrow ? (int)min(max(w.u.pos0 + r / a.GH + 1, (int64_t)0), room) : 0;
+      const int seen = (int)min(max(w.u.pos0 + 1, (int64_t)0), room);  // by the first token: no tile before needs a mask
+      for (int j = 0; j < w.n; ++j) {
+        const uint32_t t = T + j, at_s = tmem + lanes + (t & 1) * KT_KEYS;
+        const int p0 = (w.t0 + j) * KT_KEYS, left = lim - p0;
+        const bool masked = p0 + KT_KEYS > seen;
+        mbar_wait(&scfull[t & 3], (t >> 2) & 1);
+        mbar_wait(&sfull[t & 1], (t >> 1) & 1);
+        kt_fence_after();
+        const float top = masked ? kt_top<true>(at_s, s_sc[t & 3], fac, left)
+                                 : kt_top<false>(at_s, s_sc[t & 3], fac, left);
+        float alpha = 1.f;
+        const bool grew = top > m + 1.f || (m == -INFINITY && top > -INFINITY);
+        if (grew) {
+          alpha = ka_exp2(m - top);
+          m = top;
+          l *= alpha;
+        }
+        if (j > 0 && __any_sync(0xffffffffu, grew)) {
+          mbar_wait(&pvdone, (t & 1) ^ 1);  // O is up to date
           kt_fence_after();
-          const int left = lim - p0;
-          const float top = masked ? kt_top<true>(s_at_, s_sc[t & 3], fac, left)
-                                   : kt_top<false>(s_at_, s_sc[t & 3], fac, left);
-          float alpha = 1.f;
-          const bool grew = top > m + 1.f || (m == -INFINITY && top > -INFINITY);
-          if (grew) {
-            alpha = ka_exp2(m - top);
-            m = top;
-            l *= alpha;
-          }
-          if (j > 0 && __any_sync(0xffffffffu, grew)) {
-            mbar_wait(&pvdone, (t & 1) ^ 1);  // O is up to date
-            kt_fence_after();
 #pragma unroll 1
-            for (int h = 0; h < HD / 32; ++h) {
-              float v[32];
-              kt_ld32(tmem_o + lanes + h * 32, v);
-              uint32_t x[2][16];
+          for (int h = 0; h < HD / 32; ++h) {
+            float v[32];
+            kt_ld32(tmem_o + lanes + h * 32, v);
+            uint32_t x[2][16];
 #pragma unroll
-              for (int i = 0; i < 32; ++i) x[i >> 4][i & 15] = __float_as_uint(v[i] * alpha);
-              kt_st16(tmem_o + lanes + h * 32, x[0]);
-              kt_st16(tmem_o + lanes + h * 32 + 16, x[1]);
-            }
-          }
-          const float ref = m == -INFINITY ? 0.f : m;
-          l += masked ? kt_weights<WIDE, true>(s_at_, s_sc[t & 3], fac, ref, left)
-                      : kt_weights<WIDE, false>(s_at_, s_sc[t & 3], fac, ref, left);
-          kt_wait_st();
-          kt_fence_before();
-          __syncwarp();
-          if (lane == 0) kt_arrive(&pfull[t & 1]);
-        }
-      } else if (warp < 8) {
-        // ---- codes to f16
-        constexpr int CPR = HD / 16, STEP = 128 / CPR, NI = KT_KEYS / STEP;
-        const int ct = threadIdx.x - 128, qd = ct % CPR, r0 = ct / CPR;
-        uint4 kc[NI], vc[NI];
-        // lanes 0-3: table entries of a tile's blocks, asked for long before their use, and pool numbers (-1: no page)
-        auto look_up = [&](int j) {
-          const int blk = (t0 + j) * KT_BLOCKS + lane;
-          return lane < KT_BLOCKS && j < n && blk < u.nblk ? trow[(uint32_t)blk / (uint32_t)ppb] : -1;
-        };
-        auto id_of = [&](int e, int j) {
-          const uint32_t blk = (t0 + j) * KT_BLOCKS + lane;
-          return e >= 0 && e < a.kv.num_pages ? (e * a.kv.n_kv + u.h) * ppb + (int)(blk % (uint32_t)ppb) : -1;
-        };
-        // of tiles j (V), j + 1 (K) and, by their entries, j + 2
-        int id0 = id_of(look_up(0), 0), id1 = id_of(look_up(1), 1), e2 = look_up(2);
-        float sk = 0.f, sv = 0.f;
-        auto scales = [&](int id) {
-          sk = id >= 0 ? a.kv.k_scale[id] : 0.f;
-          sv = id >= 0 ? a.kv.v_scale[id] : 0.f;
-        };
-        auto load = [&](uint4 (&cs)[NI], const int8_t* codes, int ids) {
-#pragma unroll
-          for (int i = 0; i < NI; ++i) {
-            const int row = r0 + i * STEP, id = __shfl_sync(0xffffffffu, ids, row >> 4);
-            cs[i] = make_uint4(0u, 0u, 0u, 0u);
-            if (id >= 0)
-              cs[i] = __ldg(reinterpret_cast<const uint4*>(codes + (int64_t)id * (KV8_BLOCK * HD) + (row & 15) * HD +
-                                                           qd * 16));
-          }
-        };
-        auto put = [&](uint8_t* plane0, const uint4 (&cs)[NI]) {
-#pragma unroll
-          for (int i = 0; i < NI; ++i) {
-            const int row = r0 + i * STEP;
-            const uint32_t wd[4] = {cs[i].x ^ 0x80808080u, cs[i].y ^ 0x80808080u, cs[i].z ^ 0x80808080u,
-                                    cs[i].w ^ 0x80808080u};
-            uint4 x[2];
-            x[0] = make_uint4(ka_f16(wd[0], 0x5140), ka_f16(wd[0], 0x5342), ka_f16(wd[1], 0x5140),
-                              ka_f16(wd[1], 0x5342));
-            x[1] = make_uint4(ka_f16(wd[2], 0x5140), ka_f16(wd[2], 0x5342), ka_f16(wd[3], 0x5140),
-                              ka_f16(wd[3], 0x5342));
-            uint8_t* to = plane0 + (qd >> 2) * Sh::KP + row * 128;
-            const int c0 = (2 * qd) & 7, first = (qd >> 2) & 1;  // the planes' lanes take turns: no bank twice
-            *reinterpret_cast<uint4*>(to + (((c0 + first) ^ (row & 7)) << 4)) = first ? x[1] : x[0];
-            *reinterpret_cast<uint4*>(to + (((c0 + 1 - first) ^ (row & 7)) << 4)) = first ? x[0] : x[1];
-          }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-        };
-        auto scales_out = [&](uint32_t t, int id) {
-          if (warp != 4) return;
-          if (lane < KT_BLOCKS)
-            s_sc[t & 3][lane] = make_float4(sk, sv * KT_LIFT, id >= 0 ? fmaxf(__log2f(sv), -100.f) : -INFINITY, 0.f);
-          __syncwarp();
-          if (lane == 0) kt_arrive(&scfull[t & 3]);
-        };
-        load(kc, a.kv.k, id0);
-        load(vc, a.kv.v, id0);
-        if (warp == 4) scales(id0);
-        if (n > 0) {  // K of the first tile
-          mbar_wait(&kfree, (T & 1) ^ 1);
-          scales_out(T, id0);
-          put(sk_, kc);
-          if (lane == 0) kt_arrive(&kfull);
-          load(kc, a.kv.k, id1);
-          if (warp == 4) scales(id1);
-        }
-        for (int j = 0; j < n; ++j) {  // K of tile j + 1, then V of tile j; their registers are loaded again at once
-          const uint32_t t = T + j;
-          const int id2 = id_of(e2, j + 2);
-          e2 = look_up(j + 3);
-          if (j + 1 < n) {
-            mbar_wait(&kfree, t & 1);
-            scales_out(t + 1, id1);
-            put(sk_, kc);
-            if (lane == 0) kt_arrive(&kfull);
-            load(kc, a.kv.k, id2);
-            if (warp == 4) scales(id2);
-          }
-          mbar_wait(&pvdone, (t & 1) ^ 1);
-          put(sv_, vc);
-          if (lane == 0) kt_arrive(&vfull);
-          load(vc, a.kv.v, id1);
-          id1 = id2;
-        }
-      } else {
-        // ---- products: f32 sums (bit 4), f16 operands, M = 128; V is MN-major (bit 16)
-        const uint32_t is = (1u << 4) | ((uint32_t)(KT_KEYS >> 3) << 17) | ((uint32_t)(KT_ROWS >> 4) << 24);
-        const uint32_t io = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(KT_ROWS >> 4) << 24);
-        const uint64_t dq = kt_desc(smem_u32(sq_), 16), dk = kt_desc(smem_u32(sk_), 16),
-                       dv = kt_desc(smem_u32(sv_), Sh::KP);
-        for (int j = 0; j <= n; ++j) {
-          const uint32_t t = T + j;
-          if (j < n) {  // scores of tile j
-            mbar_wait(&kfull, t & 1);
-            kt_fence_after();
-            const uint32_t d = tmem + (t & 1) * KT_KEYS;
-            if (kt_elect()) {
-#pragma unroll
-              for (int x = 0; x < (WIDE ? 2 : 1); ++x)
-#pragma unroll
-                for (int k = 0; k < HD / 16; ++k)  // 16 dims: 32 bytes further inside the swizzle atom
-                  kt_mma_ss(d, dq + (x * HALVES + (k >> 2)) * (Sh::QP >> 4) + (k & 3) * 2,
-                            dk + (k >> 2) * (Sh::KP >> 4) + (k & 3) * 2, is, (x | k) != 0);
-              kt_commit(&kfree);
-              kt_commit(&sfull[t & 1]);
-            }
-            __syncwarp();
-          }
-          if (j > 0) {  // outputs of the tile before
-            const uint32_t p = t - 1;
-            mbar_wait(&vfull, p & 1);
-            mbar_wait(&pfull[p & 1], (p >> 1) & 1);
-            kt_fence_after();
-            if (kt_elect()) {
-#pragma unroll
-              for (int x = 0; x < (WIDE ? 2 : 1); ++x)
-#pragma unroll
-                for (int k = 0; k < KT_KEYS / 16; ++k)  // 16 positions: two atoms further
-                  kt_mma_ts(tmem_o, tmem + (p & 1) * KT_KEYS + (k >> 1) * 32 + x * 16 + (k & 1) * 8,
-                            dv + k * (2048 >> 4), io, (j != 1) | ((x | k) != 0));
-              kt_commit(&pvdone);
-            }
-            __syncwarp();
+            for (int i = 0; i < 32; ++i) x[i >> 4][i & 15] = __float_as_uint(v[i] * alpha);
+            kt_st16(tmem_o + lanes + h * 32, x[0]);
+            kt_st16(tmem_o + lanes + h * 32 + 16, x[1]);
           }
         }
+        const float ref = m == -INFINITY ? 0.f : m;
+        l += masked ? kt_weights<WIDE, true>(at_s, s_sc[t & 3], fac, ref, left)
+                    : kt_weights<WIDE, false>(at_s, s_sc[t & 3], fac, ref, left);
+        kt_wait_st();
+        kt_fence_before();
+        __syncwarp();
+        if (lane == 0) kt_arrive(&pfull[t & 1]);
       }
-      __syncwarp();
-      T += n;
+      T += w.n;
 
-      // ---- results
-      if (warp < 4) {
-        const int r = threadIdx.x;
-        const bool whole = begins && ends, live = r < nrow && r % a.GH < u.heads;
-        float* rec = a.work + (int64_t)(2 * c + (begins ? 1 : 0)) * Sh::REC;
-        if (n > 0) {
-          mbar_wait(&pvdone, (T - 1) & 1);
-          kt_fence_after();
-        }
-        const float scale = whole ? (l > 0.f ? 1.f / (KT_LIFT * l) : 0.f * l) : KA_LIFT / KT_LIFT;
-        const int64_t o0 = (int64_t)(u.row0 + r / a.GH) * a.ldo + (int64_t)(u.head0 + r % a.GH) * HD;
-        const bool wide_out = (((uintptr_t)a.out | (uintptr_t)(a.ldo * (WIDE ? 4 : 2))) & 15) == 0;
+      // results
+      const bool whole = w.begins && w.ends, live = r < nrow && r % a.GH < w.u.heads;
+      float* rec = a.work + (int64_t)(2 * c + (w.begins ? 1 : 0)) * Sh::REC;
+      if (w.n > 0) {
+        mbar_wait(&pvdone, (T - 1) & 1);
+        kt_fence_after();
+      }
+      const float scale = whole ? (l > 0.f ? 1.f / (KT_LIFT * l) : 0.f * l) : KA_LIFT / KT_LIFT;
+      const int64_t o0 = (int64_t)(w.u.row0 + r / a.GH) * a.ldo + (int64_t)(w.u.head0 + r % a.GH) * HD;
 #pragma unroll 1
-        for (int h = 0; h < HD / 32; ++h) {
-          float v[32];
-          if (n > 0) {
-            kt_ld32(tmem_o + ((uint32_t)(warp * 32) << 16) + h * 32, v);
+      for (int h = 0; h < HD / 32; ++h) {
+        float v[32];
+        if (w.n > 0) {
+          kt_ld32(tmem_o + lanes + h * 32, v);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] *= scale;
+        if (!whole) {
+          if (r < nrow) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+              *reinterpret_cast<float4*>(rec + r * HD + h * 32 + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+          }
+        } else if (live) {
+          if (WIDE && wide_out) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+              *reinterpret_cast<float4*>((float*)a.out + o0 + h * 32 + i) =
+                  make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
           } else {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = 0.f;
-          }
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] *= scale;
-          if (!whole) {
-            if (r < nrow) {
-#pragma unroll
-              for (int i = 0; i < 32; i += 4)
-                *reinterpret_cast<float4*>(rec + r * HD + h * 32 + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-            }
-          } else if (live) {
-            if (WIDE && wide_out) {
-#pragma unroll
-              for (int i = 0; i < 32; i += 4)
-                *reinterpret_cast<float4*>((float*)a.out + o0 + h * 32 + i) =
-                    make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-            } else {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) ka_store<WIDE>(a, o0 + h * 32 + i, v[i]);
-            }
+            for (int i = 0; i < 32; ++i) ka_store<WIDE>(a, o0 + h * 32 + i, v[i]);
           }
         }
-        if (!whole) {
-          rec[KT_ROWS * HD + r] = m;
-          rec[KT_ROWS * HD + KT_ROWS + r] = l;
-          if (threadIdx.x == 0)
-            a.work_meta[2 * c + (begins ? 1 : 0)] = make_int4(u.row0, u.head0, u.toks | u.heads << 16, ends);
-        }
-        kt_fence_before();
       }
-      __syncthreads();  // q and O are used again
-      kt_fence_after();
+      if (!whole) {
+        rec[KT_ROWS * HD + r] = m;
+        rec[KT_ROWS * HD + KT_ROWS + r] = l;
+        if (threadIdx.x == 0)
+          a.work_meta[2 * c + (w.begins ? 1 : 0)] =
+              make_int4(w.u.row0, w.u.head0, w.u.toks | w.u.heads << 16, w.ends);
+      }
+      kt_fence_before();
+      __syncwarp();  // s_fac is written again
     }
-    off = 0;
-    ++b;
+  } else if (warp < 8) {
+    // ---- codes to f16
+    constexpr int CPR = HD / 16, STEP = 128 / CPR, NI = KT_KEYS / STEP;
+    const int ct = threadIdx.x - 128, qd = ct % CPR, r0 = ct / CPR, ppb = a.kv.page / KV8_BLOCK;
+    while (w.next(a)) {
+      const int n = w.n;
+      if (n <= 0) continue;
+      const int32_t* trow = a.table + (int64_t)w.u.b * a.max_pages;
+      uint4 kc[NI], vc[NI];
+      // lanes 0-3: the block of a tile, by page column and block within the page
+      int blk = w.t0 * KT_BLOCKS + lane, col = blk / ppb, in = blk % ppb;
+      const int last = min(w.u.nblk, (w.t0 + n) * KT_BLOCKS);
+      auto look_up = [&]() { return lane < KT_BLOCKS && blk < last ? trow[col] : -1; };
+      auto step = [&]() {
+        blk += KT_BLOCKS;
+        in += KT_BLOCKS;
+        while (in >= ppb) in -= ppb, ++col;
+      };
+      auto id_of = [&](int e, int in_) {  // pool number, -1: no page
+        return e >= 0 && e < a.kv.num_pages ? (e * a.kv.n_kv + w.u.h) * ppb + in_ : -1;
+      };
+      auto load = [&](uint4 (&cs)[NI], const int8_t* codes, int ids) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          const int row = r0 + i * STEP, id = __shfl_sync(0xffffffffu, ids, row >> 4);
+          cs[i] = make_uint4(0u, 0u, 0u, 0u);
+          if (id >= 0)
+            cs[i] = __ldg(reinterpret_cast<const uint4*>(codes + (int64_t)id * (KV8_BLOCK * HD) + (row & 15) * HD +
+                                                         qd * 16));
+        }
+      };
+      auto put = [&](uint8_t* plane0, const uint4 (&cs)[NI]) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          const int row = r0 + i * STEP;
+          const uint32_t wd[4] = {cs[i].x ^ 0x80808080u, cs[i].y ^ 0x80808080u, cs[i].z ^ 0x80808080u,
+                                  cs[i].w ^ 0x80808080u};
+          uint4 x[2];
+          x[0] = make_uint4(ka_f16(wd[0], 0x5140), ka_f16(wd[0], 0x5342), ka_f16(wd[1], 0x5140), ka_f16(wd[1], 0x5342));
+          x[1] = make_uint4(ka_f16(wd[2], 0x5140), ka_f16(wd[2], 0x5342), ka_f16(wd[3], 0x5140), ka_f16(wd[3], 0x5342));
+          uint8_t* to = plane0 + (qd >> 2) * Sh::KP + row * 128;
+          const int c0 = (2 * qd) & 7, first = (qd >> 2) & 1;  // the planes' lanes take turns: no bank twice
+          *reinterpret_cast<uint4*>(to + (((c0 + first) ^ (row & 7)) << 4)) = first ? x[1] : x[0];
+          *reinterpret_cast<uint4*>(to + (((c0 + 1 - first) ^ (row & 7)) << 4)) = first ? x[0] : x[1];
+        }
+      };
+      // the fence holds up later loads: they are issued before it
+      auto done = [&](uint64_t* bar) {
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) kt_arrive(bar);
+      };
+      float sk = 0.f, sv = 0.f;
+      auto scales = [&](int id) {
+        if (warp != 4) return;
+        sk = id >= 0 ? a.kv.k_scale[id] : 0.f;
+        sv = id >= 0 ? a.kv.v_scale[id] : 0.f;
+      };
+      auto scales_out = [&](uint32_t t, int id) {
+        if (warp != 4) return;
+        if (lane < KT_BLOCKS)
+          s_sc[t & 3][lane] = make_float4(sk, sv * KT_LIFT, id >= 0 ? fmaxf(__log2f(sv), -100.f) : -INFINITY, 0.f);
+        __syncwarp();
+        if (lane == 0) kt_arrive(&scfull[t & 3]);
+      };
+      // of tiles j (V), j + 1 (K) and, by its table entry, j + 2
+      const int id0 = id_of(look_up(), in);
+      step();
+      int id1 = id_of(look_up(), in);
+      step();
+      int e2 = look_up(), in2 = in;
+      load(kc, a.kv.k, id0);
+      load(vc, a.kv.v, id0);
+      scales(id0);
+      mbar_wait(&kfree, (T & 1) ^ 1);  // K of the first tile
+      scales_out(T, id0);
+      put(sk_, kc);
+      load(kc, a.kv.k, id1);
+      scales(id1);
+      done(&kfull);
+      for (int j = 0; j < n; ++j) {  // K of tile j + 1, then V of tile j; their registers are loaded again at once
+        const uint32_t t = T + j;
+        const int id2 = id_of(e2, in2);
+        step();
+        in2 = in;
+        if (j + 1 < n) {
+          mbar_wait(&kfree, t & 1);
+          scales_out(t + 1, id1);
+          put(sk_, kc);
+          e2 = look_up();
+          load(kc, a.kv.k, id2);
+          scales(id2);
+          done(&kfull);
+        }
+        mbar_wait(&pvdone, (t & 1) ^ 1);
+        put(sv_, vc);
+        load(vc, a.kv.v, id1);
+        done(&vfull);
+        id1 = id2;
+      }
+      T += n;
+    }
+  } else {
+    // ---- products: f32 sums (bit 4), f16 operands, M = 128; V is MN-major (bit 16)
+    const uint32_t is = (1u << 4) | ((uint32_t)(KT_KEYS >> 3) << 17) | ((uint32_t)(KT_ROWS >> 4) << 24);
+    const uint32_t io = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(KT_ROWS >> 4) << 24);
+    const uint64_t dq = kt_desc(smem_u32(sq_), 16), dk = kt_desc(smem_u32(sk_), 16),
+                   dv = kt_desc(smem_u32(sv_), Sh::KP);
+    for (uint32_t U = 0; w.next(a);) {
+      const int n = w.n;
+      if (n <= 0) continue;
+      mbar_wait(&qfull, U & 1);
+      ++U;
+      for (int j = 0; j <= n; ++j) {
+        const uint32_t t = T + j;
+        if (j < n) {  // scores of tile j
+          mbar_wait(&kfull, t & 1);
+          kt_fence_after();
+          const uint32_t d = tmem + (t & 1) * KT_KEYS;
+          if (kt_elect()) {
+#pragma unroll
+            for (int x = 0; x < (WIDE ? 2 : 1); ++x)
+#pragma unroll
+              for (int k = 0; k < HD / 16; ++k)  // 16 dims: 32 bytes further inside the swizzle atom
+                kt_mma_ss(d, dq + (x * HALVES + (k >> 2)) * (Sh::QP >> 4) + (k & 3) * 2,
+                          dk + (k >> 2) * (Sh::KP >> 4) + (k & 3) * 2, is, (x | k) != 0);
+            kt_commit(&kfree);
+            kt_commit(&sfull[t & 1]);
+          }
+          __syncwarp();
+        }
+        if (j > 0) {  // outputs of the tile before
+          const uint32_t p = t - 1;
+          mbar_wait(&vfull, p & 1);
+          mbar_wait(&pfull[p & 1], (p >> 1) & 1);
+          kt_fence_after();
+          if (kt_elect()) {
+#pragma unroll
+            for (int x = 0; x < (WIDE ? 2 : 1); ++x)
+#pragma unroll
+              for (int k = 0; k < KT_KEYS / 16; ++k)  // 16 positions: two atoms further
+                kt_mma_ts(tmem_o, tmem + (p & 1) * KT_KEYS + (k >> 1) * 32 + x * 16 + (k & 1) * 8, dv + k * (2048 >> 4),
+                          io, (j != 1) | ((x | k) != 0));
+            kt_commit(&pvdone);
+          }
+          __syncwarp();
+        }
+      }
+      T += n;
+    }
   }
   kt_fence_before();
   __syncthreads();
