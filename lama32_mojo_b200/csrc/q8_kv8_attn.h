@@ -154,6 +154,7 @@ __device__ __forceinline__ int64_t ka_scan(int64_t v, int64_t* s, int64_t* total
 int kv8_attn_join(const Kv8AttnArgs& a, int ctas, int RMAX, cudaStream_t st);
 // Many rows per kv head (tcgen05): 128 rows to a group.
 constexpr int KT_ROWS = 128;
+constexpr int KV8_TILE = 4;  // blocks of a key tile
 int kv8_attn_tc_ctas();
 int kv8_attn_tc(const Kv8AttnArgs& a, int ctas, cudaStream_t st);
 

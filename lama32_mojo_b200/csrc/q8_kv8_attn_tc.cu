@@ -26,7 +26,7 @@
 
 namespace q8 {
 
-constexpr int KT_KEYS = 64, KT_BLOCKS = KT_KEYS / KV8_BLOCK;
+constexpr int KT_BLOCKS = KV8_TILE, KT_KEYS = KT_BLOCKS * KV8_BLOCK;
 constexpr int KT_THREADS = 288;
 constexpr float KT_LIFT = 16384.f;
 constexpr int KT_FIXED = 512;  // work of beginning and ending a unit, in positions
@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sq_ = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);  // q | k | v
   uint8_t *sk_ = sq_ + Sh::Q, *sv_ = sk_ + Sh::K;
-  __shared__ __align__(8) uint64_t qfull, kfull, kfree, vfull, pvdone, sfull[2], pfull[2], scfull[4];
+  __shared__ __align__(8) uint64_t qfull, kfull, kfree, vfull, pvdone[2], sfull[2], pfull[2], scfull[4];
   __shared__ uint32_t s_tmem;
   __shared__ float s_fac[KT_ROWS];
   __shared__ float4 s_sc[4][KT_BLOCKS];  // sk, lifted sv, log2 sv (-inf: no page)
@@ -263,8 +263,8 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
     mbar_init(&kfull, 4);
     mbar_init(&kfree, 1);
     mbar_init(&vfull, 4);
-    mbar_init(&pvdone, 1);
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&pvdone[i], 1);
       mbar_init(&sfull[i], 1);
       mbar_init(&pfull[i], 4);
     }
@@ -311,7 +311,9 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
   // T counts tiles, U units with tiles: the phases of all barriers.  No role waits for
   // another but through them; q's buffer is free once the scores of a unit's
   // last tile have been read, O once the softmax warps have taken it, before
-  // they announce the next unit's first weights.
+  // they announce the next unit's first weights.  A softmax warp may pass over
+  // pvdone of a tile: two barriers in turn keep it from taking the one before
+  // for the one that it waits for (the scores of tile t come after O of t - 2).
   uint32_t T = 0;
   if (warp < 4) {
     // ---- softmax, a thread per row
@@ -408,7 +410,7 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
           l *= alpha;
         }
         if (j > 0 && __any_sync(0xffffffffu, grew)) {
-          mbar_wait(&pvdone, (t & 1) ^ 1);  // O is up to date
+          mbar_wait(&pvdone[(t - 1) & 1], ((t - 1) >> 1) & 1);  // O is up to date
           kt_fence_after();
 #pragma unroll 1
           for (int h = 0; h < HD / 32; ++h) {
@@ -435,7 +437,7 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
       const bool whole = w.begins && w.ends, live = r < nrow && r % a.GH < w.u.heads;
       float* rec = a.work + (int64_t)(2 * c + (w.begins ? 1 : 0)) * Sh::REC;
       if (w.n > 0) {
-        mbar_wait(&pvdone, (T - 1) & 1);
+        mbar_wait(&pvdone[(T - 1) & 1], ((T - 1) >> 1) & 1);
         kt_fence_after();
       }
       const float scale = whole ? (l > 0.f ? 1.f / (KT_LIFT * l) : 0.f * l) : KA_LIFT / KT_LIFT;
@@ -573,7 +575,7 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
           scales(id2);
           done(&kfull);
         }
-        mbar_wait(&pvdone, (t & 1) ^ 1);
+        mbar_wait(&pvdone[(t - 1) & 1], ((t - 1) >> 1) & 1);
         put(sv_, vc);
         load(vc, a.kv.v, id1);
         done(&vfull);
@@ -622,7 +624,7 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
               for (int k = 0; k < KT_KEYS / 16; ++k)  // 16 positions: two atoms further
                 kt_mma_ts(tmem_o, tmem + (p & 1) * KT_KEYS + (k >> 1) * 32 + x * 16 + (k & 1) * 8, dv + k * (2048 >> 4),
                           io, (j != 1) | ((x | k) != 0));
-            kt_commit(&pvdone);
+            kt_commit(&pvdone[p & 1]);
           }
           __syncwarp();
         }

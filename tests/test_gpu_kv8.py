@@ -17,7 +17,9 @@ sum_d |q_d k_jd| / sqrt(hd) of the row,
     2^-25 / 2^14 = 2^-39 of the largest, however small it is, times a code of at
     most 127: positions * 2^-39 * 127 * max_j p_j sv_j.  (mag does not cover this
     where the positions that carry the weight have the code 0.)
-  * the result is rounded to its type: eps / 2 of its value.
+  * the result is rounded to its type: eps / 2 of its value, and below the
+    smallest normal number, where the grid stays smallest_normal * eps, half of
+    that (f16: 2^-14 * 2^-10 / 2 = 2^-25; an output of 2.2e-5 lies there).
 """
 import math
 
@@ -298,7 +300,8 @@ def run_case(cuda, kv, G, hd, page, ns, ctx, dtype="f32", seed=0, table=None, qs
     g = got.double().cpu().numpy().reshape(T, heads, hd)
     assert np.array_equal(g[used:], np.full_like(g[used:], 3.0)), "padding rows were written"
     eps = torch.finfo(DT[dtype]).eps / 2
-    tol = tol + (0 if dtype == "f32" else reference.tol16) + eps * np.abs(ref) + 1e-37
+    tol = tol + (0 if dtype == "f32" else reference.tol16) + eps * np.abs(ref)
+    tol += torch.finfo(DT[dtype]).smallest_normal * eps + 1e-37
     err = np.abs(g - ref)[:used]
     assert (err <= tol[:used]).all(), (err / tol[:used]).max()
     return g[:used], ref[:used]
@@ -400,6 +403,33 @@ def test_attention_offsets_past_32_bits(cuda):
     b = ops.kv8_attention(q, *args, small, i32([[0, 1, 2]], cuda))
     assert torch.equal(a, b)
     del pages
+
+
+@pytest.mark.parametrize("hd,page", [(128, 64), (64, 16)])
+@pytest.mark.parametrize("G,most,dtype", [(4, 1, "f32"), (4, 1, "bf16"), (2, 3, "f32"), (8, 24, "f32"),
+                                          (8, 24, "f16")])
+@pytest.mark.parametrize("width", [0, 500, 4000])
+def test_attention_many_sequences(cuda, hd, page, G, most, dtype, width):
+    """More sequences than threads of a CTA, empty ones among them; how the call is cut up goes
+    by the table's width, whatever the sequences' lengths are."""
+    rng = np.random.default_rng(G + most)
+    S = 401
+    ns = rng.integers(most > 1, most + 1, S)
+    ns[rng.integers(0, S, 30)] = 0
+    ctx = ns + rng.integers(0, 70, S)
+    ctx[ns == 0] //= 8
+    ctx[[7, 300, 399]] += 300
+    pages = make_pages(cuda, sum(-(-int(c) // page) for c in ctx), 2, page, hd, G)
+    table = make_table(ctx, page, pages.num_pages, G, width=max(width, -(-int(ctx.max()) // page)))
+    run_case(cuda, 2, G, hd, page, ns, ctx, dtype, G, table, pages=pages)
+
+
+@pytest.mark.parametrize("most", [1, 40])
+def test_attention_wide_tables_one_sequence(cuda, most):
+    """A table far wider than the one sequence, whose pages end inside a tile."""
+    for c in (most, 100, 1000):
+        pages = make_pages(cuda, 64, 1, 16, 128, c)
+        run_case(cuda, 1, 4, 128, 16, [most], [c], "f32", c, make_table([c], 16, 64, c, width=20000), pages=pages)
 
 
 def test_attention_repeats_and_streams(cuda):
