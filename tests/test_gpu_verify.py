@@ -307,3 +307,27 @@ def test_speculative_decoding_over_the_8_bit_cache(cuda):
         k = min(len(got[b]), len(want))
         assert got[b][:k] == want[:k], (b, got[b], want)
     assert np.array_equal(np.bincount(c.table[c.table >= 0].cpu().numpy(), minlength=20), c.refs.cpu().numpy())
+
+
+@pytest.mark.parametrize("kv,hd,normed", [(2, 64, False), (8, 128, True), (1, 128, False)])
+def test_rope_rotates_as_rope_kv_append(cuda, kv, hd, normed):
+    """The rotation alone, in place, has the bits of the one that writes the f32 cache; v and what
+    lies behind a row stay as they were."""
+    nh, T, page = 4 * kv, 21, 16
+    g = torch.Generator(device=cuda).manual_seed(hd)
+    w = (nh + 2 * kv) * hd
+    wide = torch.randn((T, w + 32), generator=g, device=cuda)
+    inv = 1.0 / 10000.0 ** (torch.arange(0, hd, 2, device=cuda) / hd)
+    pos = torch.randint(0, 64, (T,), generator=g, device=cuda, dtype=torch.int32)
+    qn, kn = ((torch.rand((hd,), generator=g, device=cuda) + 0.5).bfloat16() for _ in range(2)) if normed else (None, None)
+    a, b = wide.clone(), wide.clone()
+    ops.rope(a[:, :w], pos, nh, kv, hd, inv, qn, kn)
+    kp, vp = (torch.zeros((4 * T, kv, page, hd), device=cuda) for _ in range(2))
+    table = torch.arange(4 * T, device=cuda, dtype=torch.int32).view(T, 4)
+    ops.rope_kv_append(b[:, :w], pos, torch.arange(T, device=cuda, dtype=torch.int32), nh, kv, hd, inv, qn, kn, 1e-6,
+                       kp, vp, page, table)
+    assert torch.equal(a[:, :nh * hd], b[:, :nh * hd])
+    assert torch.equal(a[:, (nh + kv) * hd:], wide[:, (nh + kv) * hd:])
+    for t in range(T):
+        p = int(pos[t])
+        assert torch.equal(a[t, nh * hd:(nh + kv) * hd].view(kv, hd), kp[4 * t + p // page, :, p % page])
