@@ -265,8 +265,10 @@ int q8op_kv8_read(const q8_kv8_pages* kv, const int32_t* seq_start, const int32_
  * page is not there are masked (pages freed behind a window, say), and a row
  * that sees no position gives zeros.  Scores, softmax statistics and sums are
  * f32.  work: device scratch of q8op_kv8_attention_workspace() bytes, 16-byte
- * aligned (NULL where that is 0); calls that overlap need a scratch each. */
-size_t q8op_kv8_attention_workspace(int dtype, int64_t rows, int64_t S, int n_heads, int n_kv, int head_dim);
+ * aligned (NULL where that is 0), positions being max_pages * page; calls that
+ * overlap need a scratch each.  The device is the current one for both. */
+size_t q8op_kv8_attention_workspace(int dtype, int64_t rows, int64_t S, int n_heads, int n_kv, int head_dim,
+                                    int64_t positions);
 int q8op_kv8_attention(const void* q, int64_t ldq, int dtype, int64_t rows, const int32_t* seq_start,
                        const int32_t* ctx, int64_t S, int n_heads, const q8_kv8_pages* kv,
                        const int32_t* block_table, int max_pages, void* out, int64_t ldo, void* work,

@@ -74,7 +74,7 @@ SIGNATURES = {
     "q8op_kv8_append": [_P, _I64, _P, _I64, _I32, _I64, _P, _P, _I64, _P, _P, _I32, _P],
     "q8op_kv8_read": [_P, _P, _P, _I64, _P, _I32, _P, _P, _I64, _P],
     "q8op_kv8_attention": [_P, _I64, _I32, _I64, _P, _P, _I64, _I32, _P, _P, _I32, _P, _I64, _P, C.c_size_t, _P],
-    "q8op_kv8_attention_workspace": [_I32, _I64, _I64, _I32, _I32, _I32],
+    "q8op_kv8_attention_workspace": [_I32, _I64, _I64, _I32, _I32, _I32, _I64],
     "q8op_kv_truncate": [_P, _I64, _I32, _P, _P, _I64, _I32, _P, _P],
     "q8op_kv_fork": [_P, _I64, _I32, _P, _P, _I64, _I32, _P, _P, _I64, _P],
     "q8op_kv_reserve": [_P, _I64, _I32, _P, _P, _I64, _I32, _P, _P, _P, _P, _P, _P],

@@ -101,22 +101,26 @@ __device__ __forceinline__ int kv8_find(const int32_t* starts, int S, int rows, 
   return n - 1;
 }
 
+constexpr int ka_bpi(int nt) { return nt == 1 ? 2 : 1; }
+constexpr int ka_warps(int nt) { return nt <= 2 ? 12 : 8; }
+
 template <bool WIDE, int HD, int NT>  // WIDE: f32 rows, digits of q, halves of P
 struct KaShape {
   static constexpr int RPT = WIDE ? 4 : 8;      // rows per n-tile of the outputs
   static constexpr int RMAX = NT * RPT;
   static constexpr int RT = WIDE ? 1 : 2;       // rows per n-tile whose scores a lane holds
-  static constexpr int BPI = NT <= 2 ? 2 : 1;   // blocks per iteration
-  static constexpr int WARPS = NT == 1 ? 12 : 8;  // that an SM holds
+  static constexpr int BPI = ka_bpi(NT);        // blocks per iteration
+  static constexpr int WARPS = ka_warps(NT);     // that an SM holds
   static constexpr int QSMEM = NT == 1 ? 0 : NT * (HD / 16) * 32 * 8;
   static constexpr int REC = RMAX * (HD + 2);   // floats of a partial result: o, m, l
   static constexpr int smem(int warps) { return warps * REC * 4 + QSMEM + 3 * RMAX * 4; }
 };
 
-// Blocks [lo, hi) of a unit by the whole CTA.  Leaves the joined o in part
-// ([RMAX][HD], lifted by KA_LIFT), m and l in s_m, s_l.
-template <bool WIDE, int HD, int NT>
-__device__ __forceinline__ void ka_stretch(const Kv8AttnArgs& a, const KaUnit& un, int lo, int hi, uint8_t* smem) {
+// Blocks [lo, hi) of a unit by the whole CTA.  At the end a warp takes a row r at
+// a time: sink(r, x, m, l), x the lane's HD / 32 dims of the sum lifted by KA_LIFT.
+template <bool WIDE, int HD, int NT, typename Sink>
+__device__ __forceinline__ void ka_stretch(const Kv8AttnArgs& a, const KaUnit& un, int lo, int hi, uint8_t* smem,
+                                           Sink sink) {
   using Sh = KaShape<WIDE, HD, NT>;
   constexpr int RPT = Sh::RPT, RMAX = Sh::RMAX, RT = Sh::RT, BPI = Sh::BPI;
   constexpr int KW = HD / 16, VW = HD / 32, OT = HD / 16;  // words of a K quarter row, of a V eighth; output tiles
@@ -130,7 +134,6 @@ __device__ __forceinline__ void ka_stretch(const Kv8AttnArgs& a, const KaUnit& u
   float* pl = pm + warps * RMAX;                 // [warp][RMAX]
   uint2* qs = reinterpret_cast<uint2*>(pl + warps * RMAX);
   float* s_fac = reinterpret_cast<float*>(smem + warps * Sh::REC * 4 + Sh::QSMEM);
-  float *s_m = s_fac + RMAX, *s_l = s_m + RMAX;
 
   // A warp's iteration takes BPI neighbouring blocks.  Lane j keeps number in
   // the pool (-1: no page) and scales of the j-th of the next 32 blocks.
@@ -434,25 +437,41 @@ __device__ __forceinline__ void ka_stretch(const Kv8AttnArgs& a, const KaUnit& u
                       : make_float2(o[i][nt][j], o[i][nt][2 + j]);
     }
   __syncthreads();
-  // join the warps; the CTA's result replaces warp 0's
-  if (threadIdx.x < RMAX) {
-    float mx = -INFINITY, sum = 0.f;
-    for (int w = 0; w < warps; ++w) mx = fmaxf(mx, pm[w * RMAX + threadIdx.x]);
+  // join the warps
+  constexpr int D = HD / 32;
+  for (int r = warp; r < nrow; r += warps) {
+    float mx = -INFINITY, sum = 0.f, x[D];
+    for (int w = 0; w < warps; ++w) mx = fmaxf(mx, pm[w * RMAX + r]);
+    const float ref = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+    for (int e = 0; e < D; ++e) x[e] = 0.f;
     for (int w = 0; w < warps; ++w) {
-      const float mw = pm[w * RMAX + threadIdx.x];
-      const float x = mw == -INFINITY ? 0.f : exp2f(mw - mx);
-      sum += x * pl[w * RMAX + threadIdx.x];
-      pm[w * RMAX + threadIdx.x] = x;
+      const float f = exp2f(pm[w * RMAX + r] - ref);
+      const float* p = part + (w * RMAX + r) * HD + lane * D;
+      sum += f * pl[w * RMAX + r];
+#pragma unroll
+      for (int e = 0; e < D; ++e) x[e] += f * p[e];
     }
-    s_m[threadIdx.x] = mx;
-    s_l[threadIdx.x] = sum;
+    sink(r, x, mx, sum);
   }
-  __syncthreads();
-  for (int k = threadIdx.x; k < nrow * HD; k += blockDim.x) {
-    const int r = k / HD;
-    float x = 0.f;
-    for (int w = 0; w < warps; ++w) x += pm[w * RMAX + r] * part[w * RMAX * HD + k];
-    part[k] = x;
+}
+
+// The lane's dims of row r of a unit, from its lifted sums x and the sum of the weights.
+template <bool WIDE, int HD>
+__device__ __forceinline__ void ka_out(const Kv8AttnArgs& a, int row0, int head0, int heads, int r,
+                                       const float (&x)[HD / 32], float sum) {
+  constexpr int D = HD / 32;
+  if (r % a.GH >= heads) return;
+  const int64_t i = (int64_t)(row0 + r / a.GH) * a.ldo + (head0 + r % a.GH) * HD + (threadIdx.x & 31) * D;
+  float y[D];
+#pragma unroll
+  for (int e = 0; e < D; ++e)
+    y[e] = sum > 0.f ? x[e] * (1.f / KA_LIFT) / sum : 0.f * (x[e] + sum);  // no position: 0; NaN stays
+  if (WIDE && D == 4 && (((uintptr_t)a.out | (uintptr_t)(a.ldo * 4)) & 15) == 0) {
+    *reinterpret_cast<float4*>((float*)a.out + i) = make_float4(y[0], y[1], y[D - 2], y[D - 1]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < D; ++e) ka_store<WIDE>(a, i + e, y[e]);
   }
 }
 
@@ -476,42 +495,51 @@ __global__ void __launch_bounds__(KaShape<WIDE, HD, NT>::WARPS * 32, 1) k_kv8_at
   const KaUnit u = ka_unit(a, sq, blockIdx.y, i0);
   const int per = ((u.nblk + nsplit - 1) / nsplit + Sh::BPI - 1) / Sh::BPI * Sh::BPI;
   const int lo = min(u.nblk, split * per), hi = min(u.nblk, lo + per);
-  ka_stretch<WIDE, HD, NT>(a, u, lo, hi, smem);
-  const float* part = reinterpret_cast<float*>(smem);
-  const float* s_m = reinterpret_cast<float*>(smem + (blockDim.x >> 5) * Sh::REC * 4 + Sh::QSMEM) + RMAX;
-  const float* s_l = s_m + RMAX;
-  const int n = u.toks * a.GH * HD;
   if (nsplit == 1) {
-    for (int k = threadIdx.x; k < n; k += blockDim.x)
-      ka_write<WIDE, HD>(a, u.row0, u.head0, u.heads, k, part[k], s_l[k / HD]);
+    ka_stretch<WIDE, HD, NT>(a, u, lo, hi, smem, [&](int r, const float (&x)[HD / 32], float, float l) {
+      ka_out<WIDE, HD>(a, u.row0, u.head0, u.heads, r, x, l);
+    });
     return;
   }
-  cluster.sync();
-  for (int k = split * blockDim.x + threadIdx.x; k < n; k += nsplit * blockDim.x) {
-    const int r = k / HD;
-    float mx = -INFINITY;
-    for (int c = 0; c < nsplit; ++c) mx = fmaxf(mx, ka_remote(s_m + r, c));
-    float x = 0.f, sum = 0.f;
-    for (int c = 0; c < nsplit; ++c) {
-      const float mc = ka_remote(s_m + r, c);
-      const float w = mc == -INFINITY ? 0.f : exp2f(mc - mx);
-      x += w * ka_remote(part + k, c);
-      sum += w * ka_remote(s_l + r, c);
+  // the CTA's result takes warp 0's place
+  float* part = reinterpret_cast<float*>(smem);
+  float *s_m = reinterpret_cast<float*>(smem + (blockDim.x >> 5) * Sh::REC * 4 + Sh::QSMEM) + RMAX, *s_l = s_m + RMAX;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  ka_stretch<WIDE, HD, NT>(a, u, lo, hi, smem, [&](int r, const float (&x)[HD / 32], float m, float l) {
+#pragma unroll
+    for (int e = 0; e < HD / 32; ++e) part[r * HD + lane * (HD / 32) + e] = x[e];
+    if (lane == 0) {
+      s_m[r] = m;
+      s_l[r] = l;
     }
-    ka_write<WIDE, HD>(a, u.row0, u.head0, u.heads, k, x, sum);
+  });
+  cluster.sync();
+  // 32 elements to a warp, the clusters' warps in turn; lane c knows CTA c's m and l
+  const int n = u.toks * a.GH * HD;
+  for (int k0 = (warp * nsplit + split) * 32; k0 < n; k0 += (blockDim.x >> 5) * nsplit * 32) {
+    const int r = k0 / HD;
+    const float m = lane < nsplit ? ka_remote(s_m + r, lane) : -INFINITY;
+    const float l = lane < nsplit ? ka_remote(s_l + r, lane) : 0.f;
+    const float mx = warp_max(m), f = exp2f(m - (mx == -INFINITY ? 0.f : mx));
+    const float sum = warp_sum(f * l);
+    float x = 0.f;
+    for (int c = 0; c < nsplit; ++c) x += __shfl_sync(0xffffffffu, f, c) * ka_remote(part + k0 + lane, c);
+    ka_write<WIDE, HD>(a, u.row0, u.head0, u.heads, k0 + lane, x, sum);
   }
   cluster.sync();  // nobody leaves while its memory is read
 }
 
 // Many units: CTA c takes the c-th of gridDim.x equal stretches of all units'
 // work, units ordered by (sequence, group, kv head).  A unit's work is its
-// iterations (BPI blocks each) behind KA_FIXED more for its start and end.
-constexpr int KA_FIXED = 16;
+// iterations (BPI blocks each) behind some more for its start and end (7 us,
+// an iteration of a CTA's four warps taking 0.45 us with one n-tile and two
+// blocks, 0.3 us with two n-tiles and one).
+constexpr int ka_fixed(int nt) { return nt == 1 ? 14 : 28; }
 
 template <bool WIDE, int HD, int NT>
 __global__ void __launch_bounds__(128, KaShape<WIDE, HD, NT>::WARPS / 4) k_kv8_attn_many(Kv8AttnArgs a) {
   using Sh = KaShape<WIDE, HD, NT>;
-  constexpr int RMAX = Sh::RMAX, BPI = Sh::BPI;
+  constexpr int RMAX = Sh::RMAX, BPI = Sh::BPI, KA_FIXED = ka_fixed(NT);
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ int64_t s_scan[4];
   __shared__ int64_t s_at;
@@ -560,25 +588,27 @@ __global__ void __launch_bounds__(128, KaShape<WIDE, HD, NT>::WARPS / 4) k_kv8_a
       left -= take;
       if (u1 == 0 && !ends) continue;  // the next CTA begins it
       const KaUnit u = ka_unit(a, sq, (int)(k % H), (int)(k / H) * a.QT);
-      ka_stretch<WIDE, HD, NT>(a, u, min(u.nblk, u0 * BPI), min(u.nblk, u1 * BPI), smem);
-      const float* part = reinterpret_cast<float*>(smem);
-      const float* s_m = reinterpret_cast<float*>(smem + 4 * Sh::REC * 4 + Sh::QSMEM) + RMAX;
-      const float* s_l = s_m + RMAX;
-      const int n = u.toks * a.GH * HD;
-      if (begins && ends) {
-        for (int i = threadIdx.x; i < n; i += blockDim.x)
-          ka_write<WIDE, HD>(a, u.row0, u.head0, u.heads, i, part[i], s_l[i / HD]);
-      } else {
-        // record 1: a unit that begins here, record 0: one that goes on from the CTA before
-        const int rec = 2 * c + (begins ? 1 : 0);
-        float* to = a.work + (int64_t)rec * Sh::REC;
-        for (int i = threadIdx.x; i < n; i += blockDim.x) to[i] = part[i];
-        if (threadIdx.x < RMAX) {
-          to[RMAX * HD + threadIdx.x] = s_m[threadIdx.x];
-          to[RMAX * HD + RMAX + threadIdx.x] = s_l[threadIdx.x];
+      const int lo = min(u.nblk, u0 * BPI), hi = min(u.nblk, u1 * BPI);
+      // record 1: a unit that begins here, record 0: one that goes on from the CTA before
+      const bool whole = begins && ends;
+      const int rec = 2 * c + (begins ? 1 : 0), lane = threadIdx.x & 31;
+      float* to = a.work + (int64_t)rec * Sh::REC;
+      ka_stretch<WIDE, HD, NT>(a, u, lo, hi, smem, [&](int r, const float (&x)[HD / 32], float m, float l) {
+        if (whole) {
+          ka_out<WIDE, HD>(a, u.row0, u.head0, u.heads, r, x, l);
+          return;
         }
-        if (threadIdx.x == 0) a.work_meta[rec] = make_int4(u.row0, u.head0, u.toks | u.heads << 16, ends);
-      }
+        if constexpr (HD == 128)
+          *reinterpret_cast<float4*>(to + r * HD + lane * 4) = make_float4(x[0], x[1], x[HD / 32 - 2], x[HD / 32 - 1]);
+        else
+          *reinterpret_cast<float2*>(to + r * HD + lane * 2) = make_float2(x[0], x[1]);
+        if (lane == 0) {
+          to[RMAX * HD + r] = m;
+          to[RMAX * HD + RMAX + r] = l;
+        }
+      });
+      if (!whole && threadIdx.x == 0)
+        a.work_meta[rec] = make_int4(u.row0, u.head0, u.toks | u.heads << 16, ends);
       __syncthreads();  // shared memory is used again
     }
     off = 0;
@@ -618,9 +648,7 @@ __global__ void __launch_bounds__(256) k_kv8_attn_join(Kv8AttnArgs a, int RMAX) 
     for (int e = 0; e < E; ++e) x[e] = x[e] * f0 + v[e] * f1;
     mx = top;
   }
-#pragma unroll
-  for (int e = 0; e < E; ++e)
-    ka_write<WIDE, HD>(a, me.x, me.y, heads, r * HD + lane * E + e, x[e], sum);
+  ka_out<WIDE, HD>(a, me.x, me.y, heads, r, x, sum);
 }
 
 template <bool WIDE, int HD>
@@ -635,29 +663,90 @@ int kv8_attn_join(const Kv8AttnArgs& a, int ctas, int RMAX, cudaStream_t st) {
   return a.dtype == Q8_F32 ? join_run<true, 64>(a, ctas, RMAX, st) : join_run<false, 64>(a, ctas, RMAX, st);
 }
 
+// Clusters of c CTAs, each with an SM to itself, that the device holds at once.
+static int ka_clusters(int c) {
+  static int held[64][9];  // 0: not asked yet
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  int& n = held[dev & 63][c];
+  if (n == 0) {
+    auto kern = k_kv8_attn<true, 128, 1>;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim = {(unsigned)c, 1, 1};
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(c);
+    cfg.blockDim = dim3(KaShape<true, 128, 1>::WARPS * 32);
+    cfg.dynamicSmemBytes = KaShape<true, 128, 1>::smem(KaShape<true, 128, 1>::WARPS);
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int got = 0;
+    if (cudaOccupancyMaxActiveClusters(&got, kern, &cfg) != cudaSuccess) {
+      cudaGetLastError();
+      got = 0;
+    }
+    n = got > 0 ? got : -1;
+  }
+  return n > 0 ? n : 0;
+}
+
+// How a call is cut up.  Every sequence is taken to have rows / S rows and the
+// table's width of positions.  The three forms cost, fitted to 177 shapes of 1 to
+// 64 sequences, 600 to 20,000 positions, 1 to 24 rows a sequence (us, head size
+// 128; 64 in brackets):
+//   clusters  5 + 3 a wave + 1.25 (0.75) an iteration of a warp; 9 for 5 with 4
+//             n-tiles, whose results take longer to join
+//   many      14 (16 with 4 n-tiles) + 0.94 (0.56) an iteration: even stretches,
+//             a second launch
+//   tcgen05   28 + 1.2 (1.0) a tile of a CTA: pays when 128 rows share a reading
+// The form chosen so was within 1.6 % of the best one on average.  f32 rows, 8 kv
+// heads of 128, 32 heads, us for the three: 8 sequences of 4000 positions, 1 row,
+// 16.0, 21.7, 39.4; 16 of 8000, 39.4, 31.7, 90.1; 16 of 4500, 24 rows, 212, 187, 83.
 struct KaPlan {
-  bool tc;   // k_kv8_attn_tc
-  int nt, GH, hgroups, QT, ctas;  // ctas: stretches of k_kv8_attn_many, 0: clusters
-  int64_t slots, units;
+  bool tc;     // k_kv8_attn_tc
+  int nt, GH, hgroups, QT;
+  int ctas;    // stretches of k_kv8_attn_many or k_kv8_attn_tc, 0: clusters
+  int nsplit;  // CTAs of a cluster
+  int64_t slots;
   size_t meta, bytes;  // workspace
 };
 
-static KaPlan ka_plan(bool wide, int hd, int64_t rows, int64_t S, int n_heads, int n_kv) {
+static KaPlan ka_plan(bool wide, int hd, int64_t rows, int64_t S, int n_heads, int n_kv, int64_t positions) {
   KaPlan p{};
-  const int G = n_heads / n_kv;
-  const int64_t want = (rows + S - 1) / S * (int64_t)G;  // rows per kv head of an average sequence
+  const int G = n_heads / n_kv, sms = num_sms();
+  const int64_t avg = (rows + S - 1) / S, want = avg * G;  // rows per kv head of an average sequence
+  const int64_t blocks = (positions + KV8_BLOCK - 1) / KV8_BLOCK;
   const int cols = wide ? 2 : 1;
   p.nt = want * cols <= 8 ? 1 : want * cols <= 16 ? 2 : 4;
-  p.tc = want >= 64 && G <= KT_ROWS;
-  const int rmax = p.tc ? KT_ROWS : 8 * p.nt / cols;
-  p.GH = std::min(G, rmax);
-  p.hgroups = ceil_div(G, p.GH);
-  p.QT = rows <= S ? 1 : rmax / p.GH;
-  p.slots = p.QT > 1 ? rows / p.QT + S : rows;
-  p.units = p.slots * n_kv * p.hgroups;
-  // One n-tile: a unit is cheap to begin and its partial results are small.
-  if (p.tc || (p.nt == 1 && p.units > num_sms())) {
-    p.ctas = p.tc ? kv8_attn_tc_ctas() : 3 * num_sms();
+  // groups of a sequence on all kv heads: `rmax` rows each
+  auto cut = [&](int rmax) {
+    p.GH = std::min(G, rmax);
+    p.hgroups = ceil_div(G, p.GH);
+    p.QT = rows <= S ? 1 : rmax / p.GH;
+    return (avg + p.QT - 1) / p.QT * n_kv * p.hgroups;
+  };
+  int rmax = 8 * p.nt / cols;
+  const int64_t reg = S * cut(rmax), tc = S * cut(KT_ROWS);
+  const int per_it = ka_bpi(p.nt) * ka_warps(p.nt);
+  const int64_t most = (blocks + per_it - 1) / per_it;
+  p.nsplit = 1;
+  for (int c = 8; c > 1 && p.nsplit == 1; --c)
+    if (c <= most && reg <= ka_clusters(c)) p.nsplit = c;
+  const int64_t waves = (reg * p.nsplit + sms - 1) / sms, its = (most + p.nsplit - 1) / p.nsplit;
+  // at most 8 CTAs to a unit: their results are joined one after the other
+  const int many_ctas = (int)std::min<int64_t>(ka_warps(p.nt) / 4 * sms, reg * 8);
+  const int tc_ctas = (int)std::min<int64_t>(kv8_attn_tc_ctas(), tc * 8);
+  const double turn = hd == 128 ? 1.25 : 0.75;
+  const double t_cluster = (p.nt < 4 ? 5 : 9) + waves * (3 + turn * its);
+  const double t_many =
+      (p.nt < 4 ? 14 : 16) + 0.75 * turn * reg * blocks / (ka_bpi(p.nt) * 4.0 * many_ctas);
+  const double t_tc = 28 + (hd == 128 ? 1.2 : 1.0) * tc * ((blocks + KV8_TILE - 1) / KV8_TILE) / tc_ctas;
+  p.tc = p.nt == 4 && G <= KT_ROWS && t_tc < std::min(t_cluster, t_many);
+  if (p.tc || t_many < t_cluster) p.ctas = p.tc ? tc_ctas : many_ctas;
+  if (p.tc) rmax = KT_ROWS;
+  cut(rmax);
+  p.slots = p.QT > 1 ? rows / p.QT + S : rows;  // room for the groups, about half of it used where QT > 1
+  if (p.ctas) {
     p.meta = (size_t)p.ctas * 2 * rmax * (hd + 2) * 4;
     p.bytes = p.meta + (size_t)p.ctas * 2 * sizeof(int4);
   }
@@ -665,34 +754,30 @@ static KaPlan ka_plan(bool wide, int hd, int64_t rows, int64_t S, int n_heads, i
 }
 
 template <bool WIDE, int HD, int NT>
-static int attn_run(Kv8AttnArgs& a, const KaPlan& p, cudaStream_t st) {
+static int attn_run(const Kv8AttnArgs& a, const KaPlan& p, cudaStream_t st) {
   using Sh = KaShape<WIDE, HD, NT>;
   auto few = k_kv8_attn<WIDE, HD, NT>;
+  auto many = k_kv8_attn_many<WIDE, HD, NT>;
   static bool ready[64] = {false};
   int dev = 0;
   Q8_CUDA(cudaGetDevice(&dev));
   if (!ready[dev & 63]) {
     Q8_CUDA(cudaFuncSetAttribute(few, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::smem(Sh::WARPS)));
-    Q8_CUDA(cudaFuncSetAttribute(few, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    Q8_CUDA(cudaFuncSetAttribute(many, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::smem(4)));
     ready[dev & 63] = true;
   }
-  if constexpr (NT == 1) {
-    if (p.ctas) {
-      k_kv8_attn_many<WIDE, HD, NT><<<p.ctas, 128, Sh::smem(4), st>>>(a);
-      Q8_TRY(launch_check("k_kv8_attn_many"));
-      return kv8_attn_join(a, p.ctas, Sh::RMAX, st);
-    }
+  if (p.ctas) {
+    many<<<p.ctas, 128, Sh::smem(4), st>>>(a);
+    Q8_TRY(launch_check("k_kv8_attn_many"));
+    return kv8_attn_join(a, p.ctas, Sh::RMAX, st);
   }
-  // a cluster's CTAs: an SM each, but an iteration for every warp at the longest context
-  const int64_t most = ((int64_t)a.max_pages * a.kv.page / KV8_BLOCK + Sh::BPI * Sh::WARPS - 1) / (Sh::BPI * Sh::WARPS);
-  int nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({16, most, num_sms() / p.units}));
-  Q8_CHECK_ARG(p.slots * nsplit < ((int64_t)1 << 31) && (int64_t)a.kv.n_kv * a.hgroups <= 65535,
+  Q8_CHECK_ARG(p.slots * p.nsplit < ((int64_t)1 << 31) && (int64_t)a.kv.n_kv * a.hgroups <= 65535,
                "q8op_kv8_attention: too many rows or heads");
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim = {(unsigned)nsplit, 1, 1};
+  attr[0].val.clusterDim = {(unsigned)p.nsplit, 1, 1};
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(p.slots * nsplit), a.kv.n_kv * a.hgroups);
+  cfg.gridDim = dim3((unsigned)(p.slots * p.nsplit), a.kv.n_kv * a.hgroups);
   cfg.blockDim = dim3(Sh::WARPS * 32);
   cfg.dynamicSmemBytes = Sh::smem(Sh::WARPS);
   cfg.stream = st;
@@ -703,7 +788,7 @@ static int attn_run(Kv8AttnArgs& a, const KaPlan& p, cudaStream_t st) {
 }
 
 template <bool WIDE, int HD>
-static int attn_pick(Kv8AttnArgs& a, const KaPlan& p, cudaStream_t st) {
+static int attn_pick(const Kv8AttnArgs& a, const KaPlan& p, cudaStream_t st) {
   if (p.nt == 1) return attn_run<WIDE, HD, 1>(a, p, st);
   if (p.nt == 2) return attn_run<WIDE, HD, 2>(a, p, st);
   return attn_run<WIDE, HD, 4>(a, p, st);
@@ -713,10 +798,10 @@ static int attn_pick(Kv8AttnArgs& a, const KaPlan& p, cudaStream_t st) {
 
 using namespace q8;
 
-extern "C" size_t q8op_kv8_attention_workspace(int dtype, int64_t rows, int64_t S, int n_heads, int n_kv,
-                                               int head_dim) {
-  if (rows <= 0 || S <= 0 || n_kv <= 0 || n_heads <= 0 || n_heads % n_kv || head_dim <= 0) return 0;
-  return ka_plan(dtype == Q8_F32, head_dim, rows, S, n_heads, n_kv).bytes;
+extern "C" size_t q8op_kv8_attention_workspace(int dtype, int64_t rows, int64_t S, int n_heads, int n_kv, int head_dim,
+                                               int64_t positions) {
+  if (rows <= 0 || S <= 0 || n_kv <= 0 || n_heads <= 0 || n_heads % n_kv || head_dim <= 0 || positions < 0) return 0;
+  return ka_plan(dtype == Q8_F32, head_dim, rows, S, n_heads, n_kv, positions).bytes;
 }
 
 extern "C" int q8op_kv8_attention(const void* q, int64_t ldq, int dtype, int64_t rows, const int32_t* seq_start,
@@ -731,7 +816,7 @@ extern "C" int q8op_kv8_attention(const void* q, int64_t ldq, int dtype, int64_t
   const int64_t width = (int64_t)n_heads * kv->head_dim;
   Q8_CHECK_ARG(q && out && ldq >= width && ldo >= width, "q8op_kv8_attention: q and out rows need %lld elements",
                (long long)width);
-  const KaPlan p = ka_plan(dtype == Q8_F32, kv->head_dim, rows, S, n_heads, kv->n_kv);
+  const KaPlan p = ka_plan(dtype == Q8_F32, kv->head_dim, rows, S, n_heads, kv->n_kv, (int64_t)max_pages * kv->page);
   Q8_CHECK_ARG(p.bytes == 0 || (work && work_bytes >= p.bytes && ((uintptr_t)work & 15) == 0),
                "q8op_kv8_attention: workspace of %zu bytes (16-byte aligned), %zu needed", work ? work_bytes : (size_t)0,
                p.bytes);

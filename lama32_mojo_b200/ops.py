@@ -317,7 +317,8 @@ def kv8_attention(q, seq_start, ctx, n_heads: int, pages: KV8Pages, block_table,
         To, ldo = _rows_of(out, "kv8_attention: out", w, dev)
         if To != T or out.dtype != q.dtype:
             raise ValueError("kv8_attention: out must have q's rows and type")
-    nbytes = lib().q8op_kv8_attention_workspace(_DT[q.dtype], T, S, n_heads, pages.n_kv, pages.head_dim)
+    nbytes = lib().q8op_kv8_attention_workspace(_DT[q.dtype], T, S, n_heads, pages.n_kv, pages.head_dim,
+                                                width * pages.page)
     work = torch.empty(nbytes, dtype=torch.uint8, device=q.device).data_ptr() if nbytes else None
     _call(lib().q8op_kv8_attention, dev, q.data_ptr(), ldq, _DT[q.dtype], T, seq_start.data_ptr(), ctx.data_ptr(), S,
           n_heads, pages._ref, block_table.data_ptr(), width, out.data_ptr(), ldo, work, nbytes)
