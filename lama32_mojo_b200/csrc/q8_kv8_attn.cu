@@ -698,10 +698,11 @@ static int ka_clusters(int c) {
 //             n-tiles, whose results take longer to join
 //   many      14 (16 with 4 n-tiles) + 0.94 (0.56) an iteration: even stretches,
 //             a second launch
-//   tcgen05   28 + 1.2 (1.0) a tile of a CTA: pays when 128 rows share a reading
+//   tcgen05   28 + 1.2 (1.0) a tile of a CTA, a tenth more for f32 rows: pays when
+//             128 rows share a reading
 // The form chosen so was within 1.6 % of the best one on average.  f32 rows, 8 kv
 // heads of 128, 32 heads, us for the three: 8 sequences of 4000 positions, 1 row,
-// 16.0, 21.7, 39.4; 16 of 8000, 39.4, 31.7, 90.1; 16 of 4500, 24 rows, 212, 187, 83.
+// 16.0, 21.7, 39.4; 16 of 8000, 39.4, 31.7, 90.1; 16 of 4500, 24 rows, 212, 187, 88.
 struct KaPlan {
   bool tc;     // k_kv8_attn_tc
   int nt, GH, hgroups, QT;
@@ -740,14 +741,14 @@ static KaPlan ka_plan(bool wide, int hd, int64_t rows, int64_t S, int n_heads, i
   const double t_cluster = (p.nt < 4 ? 5 : 9) + waves * (3 + turn * its);
   const double t_many =
       (p.nt < 4 ? 14 : 16) + 0.75 * turn * reg * blocks / (ka_bpi(p.nt) * 4.0 * many_ctas);
-  const double t_tc = 28 + (hd == 128 ? 1.2 : 1.0) * tc * ((blocks + KV8_TILE - 1) / KV8_TILE) / tc_ctas;
+  const double t_tc = 28 + (hd == 128 ? 1.2 : 1.0) * (wide ? 1.1 : 1.0) * tc * ((blocks + KV8_TILE - 1) / KV8_TILE) / tc_ctas;
   p.tc = p.nt == 4 && G <= KT_ROWS && t_tc < std::min(t_cluster, t_many);
   if (p.tc || t_many < t_cluster) p.ctas = p.tc ? tc_ctas : many_ctas;
   if (p.tc) rmax = KT_ROWS;
   cut(rmax);
   p.slots = p.QT > 1 ? rows / p.QT + S : rows;  // room for the groups, about half of it used where QT > 1
   if (p.ctas) {
-    p.meta = (size_t)p.ctas * 2 * rmax * (hd + 2) * 4;
+    p.meta = (size_t)p.ctas * (p.tc && wide ? 3 : 2) * rmax * (hd + 2) * 4;  // tc: and a place for flushed sums
     p.bytes = p.meta + (size_t)p.ctas * 2 * sizeof(int4);
   }
   return p;

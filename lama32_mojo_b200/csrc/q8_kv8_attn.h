@@ -24,7 +24,7 @@ struct Kv8AttnArgs {
   void* out;
   int64_t ldo;
   int QT, GH, hgroups;  // tokens per group, heads per group, head groups per kv head
-  float* work;          // two partial results for every CTA
+  float* work;          // two partial results for every CTA, then k_kv8_attn_tc's flushed sums
   int4* work_meta;      // and what they are
 };
 
