@@ -515,8 +515,10 @@ __global__ void __launch_bounds__(KaShape<WIDE, HD, NT>::WARPS * 32, 1) k_kv8_at
   });
   cluster.sync();
   // 32 elements to a warp, the clusters' warps in turn; lane c knows CTA c's m and l
-  const int n = u.toks * a.GH * HD;
-  for (int k0 = (warp * nsplit + split) * 32; k0 < n; k0 += (blockDim.x >> 5) * nsplit * 32) {
+  const int n = u.toks * a.GH * HD, step = (blockDim.x >> 5) * nsplit * 32;
+  int k0 = (warp * nsplit + split) * 32;
+  if (k0 >= n) cluster_leave();
+  for (; k0 < n; k0 += step) {
     const int r = k0 / HD;
     const float m = lane < nsplit ? ka_remote(s_m + r, lane) : -INFINITY;
     const float l = lane < nsplit ? ka_remote(s_l + r, lane) : 0.f;
@@ -524,9 +526,10 @@ __global__ void __launch_bounds__(KaShape<WIDE, HD, NT>::WARPS * 32, 1) k_kv8_at
     const float sum = warp_sum(f * l);
     float x = 0.f;
     for (int c = 0; c < nsplit; ++c) x += __shfl_sync(0xffffffffu, f, c) * ka_remote(part + k0 + lane, c);
+    if (k0 + step >= n) cluster_leave();
     ka_write<WIDE, HD>(a, u.row0, u.head0, u.heads, k0 + lane, x, sum);
   }
-  cluster.sync();  // nobody leaves while its memory is read
+  cluster_left();  // nobody leaves while its memory is read
 }
 
 // Many units: CTA c takes the c-th of gridDim.x equal stretches of all units'

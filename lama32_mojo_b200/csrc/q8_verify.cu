@@ -24,7 +24,7 @@ constexpr int VF_THREADS = 512;
 constexpr int VF_WARPS = VF_THREADS / 32;
 constexpr int VF_MAX_CLUSTER = 16;
 constexpr int VF_Q = 10;                           // four-logit pieces that a thread of k_probs holds
-constexpr int VF_SLICE = VF_THREADS * 4 * VF_Q;    // logits of a row per CTA, at most
+constexpr int vf_slice(int threads) { return threads * 4 * VF_Q; }  // logits of a row per CTA of k_probs, at most
 
 __device__ __forceinline__ void vf_best(float& bv, int& bi, float ov, int oi) {
   if (ov > bv || (ov == bv && oi < bi)) {
@@ -68,24 +68,26 @@ __device__ __forceinline__ double vf_warp_sum(double v) {
 // (l - max) / temp log2(e) is taken as y + z, y the f32 product with c = ch + cl
 // and z what it lost, so that the exponent's rounding does not grow with it:
 // w = 2^y (1 + z ln 2).  Four weights are added in 32 bits, those sums in 64.
-__global__ void __launch_bounds__(VF_THREADS, 2) k_probs(const float* __restrict__ logits, int n, int64_t ld,
-                                                         float temp, float ch, float cl, float* __restrict__ out,
-                                                         int64_t ldo, int per) {
-  __shared__ float s_v[VF_WARPS], s_top;
-  __shared__ int s_i[VF_WARPS], s_arg;
-  __shared__ double s_d[VF_WARPS], s_sum;
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS)
+    k_probs(const float* __restrict__ logits, int rows, int n, int64_t ld, float temp, float ch, float cl,
+            float* __restrict__ out, int64_t ldo, int per, int ahead) {
+  constexpr int WARPS = THREADS / 32;
+  __shared__ float s_v[WARPS], s_top;
+  __shared__ int s_i[WARPS], s_arg;
+  __shared__ double s_d[WARPS], s_sum;
   const cg::cluster_group cluster = cg::this_cluster();
   const int nc = cluster.num_blocks(), rank = cluster.block_rank(), row = blockIdx.x / nc;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int lo = min(n, rank * per), cnt = min(n, lo + per) - lo;
   const float* src = logits + (int64_t)row * ld + lo;
   float* dst = out + (int64_t)row * ldo + lo;
-  const int at = threadIdx.x * 4;  // piece k: at + k * 4 * VF_THREADS
+  const int at = threadIdx.x * 4;  // piece k: at + k * 4 * THREADS
   const bool wide = ((uintptr_t)src & 15) == 0;
   float v[VF_Q][4];
 #pragma unroll
   for (int k = 0; k < VF_Q; ++k) {
-    const int i = at + k * 4 * VF_THREADS;
+    const int i = at + k * 4 * THREADS;
     if (wide && i + 4 <= cnt) {
       const float4 f = __ldcs(reinterpret_cast<const float4*>(src + i));
       v[k][0] = f.x, v[k][1] = f.y, v[k][2] = f.z, v[k][3] = f.w;
@@ -94,6 +96,8 @@ __global__ void __launch_bounds__(VF_THREADS, 2) k_probs(const float* __restrict
       for (int e = 0; e < 4; ++e) v[k][e] = i + e < cnt ? src[i + e] : -INFINITY;
     }
   }
+  if (threadIdx.x == 0 && row < rows - ahead && wide && (ld & 3) == 0 && cnt >= 4)
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src + ahead * ld), "r"((cnt & ~3) * 4));
   const bool greedy = !(temp > 0.f);
   float bv = -INFINITY;
   int bi = 0x7fffffff;
@@ -106,7 +110,7 @@ __global__ void __launch_bounds__(VF_THREADS, 2) k_probs(const float* __restrict
     for (int k = VF_Q - 1; k >= 0; --k)
 #pragma unroll
       for (int e = 3; e >= 0; --e)
-        if (v[k][e] == bv) bi = lo + at + k * 4 * VF_THREADS + e;
+        if (v[k][e] == bv) bi = lo + at + k * 4 * THREADS + e;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1)
@@ -117,10 +121,10 @@ __global__ void __launch_bounds__(VF_THREADS, 2) k_probs(const float* __restrict
   }
   __syncthreads();
   if (w == 0) {
-    bv = lane < VF_WARPS ? s_v[lane] : -INFINITY;
-    bi = lane < VF_WARPS ? s_i[lane] : 0x7fffffff;
+    bv = lane < WARPS ? s_v[lane] : -INFINITY;
+    bi = lane < WARPS ? s_i[lane] : 0x7fffffff;
 #pragma unroll
-    for (int o = VF_WARPS / 2; o > 0; o >>= 1)
+    for (int o = WARPS / 2; o > 0; o >>= 1)
       vf_best(bv, bi, __shfl_xor_sync(0xffffffffu, bv, o), __shfl_xor_sync(0xffffffffu, bi, o));
     if (lane == 0) {
       s_top = bv;
@@ -136,9 +140,10 @@ __global__ void __launch_bounds__(VF_THREADS, 2) k_probs(const float* __restrict
   bv = __shfl_sync(0xffffffffu, bv, 0);
   bi = __shfl_sync(0xffffffffu, bi, 0);
   if (greedy || bv == -INFINITY) {
+    cluster_leave();
     if (bi == 0x7fffffff) bi = 0;  // nothing above -inf: as q8op_argmax
-    for (int i = threadIdx.x; i < cnt; i += VF_THREADS) dst[i] = lo + i == bi ? 1.f : 0.f;
-    cluster.sync();
+    for (int i = threadIdx.x; i < cnt; i += THREADS) dst[i] = lo + i == bi ? 1.f : 0.f;
+    cluster_left();
     return;
   }
   const float low = bv - 16.f;
@@ -160,16 +165,17 @@ __global__ void __launch_bounds__(VF_THREADS, 2) k_probs(const float* __restrict
   __syncthreads();
   if (threadIdx.x == 0) {
     sum = 0.0;
-    for (int k = 0; k < VF_WARPS; ++k) sum += s_d[k];
+    for (int k = 0; k < WARPS; ++k) sum += s_d[k];
     s_sum = sum;
   }
   cluster.sync();
   sum = vf_warp_sum(lane < nc ? vf_peer(&s_sum, lane) : 0.0);
+  cluster_leave();
   const float inv = (float)(1.0 / sum);
   const bool wide_out = ((uintptr_t)dst & 15) == 0;
 #pragma unroll
   for (int k = 0; k < VF_Q; ++k) {
-    const int i = at + k * 4 * VF_THREADS;
+    const int i = at + k * 4 * THREADS;
     if (wide_out && i + 4 <= cnt) {
       __stcs(reinterpret_cast<float4*>(dst + i),
              make_float4(v[k][0] * inv, v[k][1] * inv, v[k][2] * inv, v[k][3] * inv));
@@ -179,7 +185,7 @@ __global__ void __launch_bounds__(VF_THREADS, 2) k_probs(const float* __restrict
         if (i + e < cnt) dst[i + e] = v[k][e] * inv;
     }
   }
-  cluster.sync();  // nobody leaves while its sum is read
+  cluster_left();  // nobody leaves while its sum is read
 }
 
 // A cluster of CTAs per sequence; all of them find the refused row, then each
@@ -307,6 +313,10 @@ __global__ void __launch_bounds__(VF_THREADS) k_verify(const float* __restrict__
     qr = nullptr;
     gone = -1;
   }
+  int tail = -1;  // the last index with a weight, for rank 0
+  if (rank == 0 && wid == 0) tail = __reduce_max_sync(0xffffffffu, lane < nc ? vf_peer(&s_last, lane) : -1);
+  __syncwarp();
+  cluster_leave();
   // the first index whose cumulative weight exceeds u total lies in the CTA
   // that reaches beyond it; if rounding leaves none, the last index with a weight
   const double r = (double)draw * total;
@@ -345,17 +355,14 @@ __global__ void __launch_bounds__(VF_THREADS) k_verify(const float* __restrict__
       last = __reduce_max_sync(0xffffffffu, last);
       if (lane == 0) tokens[stop] = first != 0x7fffffff ? first : last;
     }
-    if (rank == 0 && !(r < total)) {
-      const int last = __reduce_max_sync(0xffffffffu, lane < nc ? vf_peer(&s_last, lane) : -1);
-      if (lane == 0) tokens[stop] = max(last, 0);
-    }
+    if (rank == 0 && !(r < total) && lane == 0) tokens[stop] = max(tail, 0);
   }
   if (rank == nc - 1) {
     if (threadIdx.x == 0) taken[b] = stop - r0;
     for (int i = r0 + threadIdx.x; i < r1; i += VF_THREADS)
       if (i != stop) tokens[i] = i < stop ? ids[i + 1] : -1;
   }
-  cluster.sync();  // nobody leaves while its sums are read
+  cluster_left();  // nobody leaves while its sums are read
 }
 
 // CTAs per row: what `least` asks for, more while the GPU has room and a CTA keeps 2048 entries.
@@ -365,11 +372,10 @@ static int vf_cluster(int64_t rows, int64_t n, int64_t least, int64_t room) {
   return c;
 }
 
-template <typename... KArgs, typename... Args>
-static int vf_launch(const char* what, void (*kern)(KArgs...), int64_t rows, int c, size_t smem, int most,
-                     cudaStream_t st, Args... args) {
-  static_assert(sizeof...(KArgs) == sizeof...(Args), "a kernel of this file");
-  static bool ready[64] = {false};  // of this kernel: the two have parameters of their own
+template <auto kern, typename... Args>
+static int vf_launch(const char* what, int64_t rows, int c, int threads, size_t smem, int most, cudaStream_t st,
+                     Args... args) {
+  static bool ready[64] = {false};  // of this kernel
   int dev = 0;
   Q8_CUDA(cudaGetDevice(&dev));
   if (!ready[dev & 63]) {
@@ -382,7 +388,7 @@ static int vf_launch(const char* what, void (*kern)(KArgs...), int64_t rows, int
   attr[0].val.clusterDim = {(unsigned)c, 1, 1};
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(rows * c));
-  cfg.blockDim = dim3(VF_THREADS);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = attr;
@@ -399,7 +405,7 @@ static int vf_launch(const char* what, void (*kern)(KArgs...), int64_t rows, int
 
 using namespace q8;
 
-constexpr int64_t VF_PROBS_MAX = (int64_t)VF_MAX_CLUSTER * VF_SLICE;  // 327,680
+constexpr int64_t VF_PROBS_MAX = (int64_t)VF_MAX_CLUSTER * vf_slice(VF_THREADS);  // 327,680
 constexpr int64_t VF_VERIFY_MAX = (int64_t)VF_MAX_CLUSTER * 20000 * VF_SEG;
 
 extern "C" int q8op_probs(const float* logits, int64_t rows, int64_t n, int64_t ld, float temp, float* out,
@@ -410,12 +416,20 @@ extern "C" int q8op_probs(const float* logits, int64_t rows, int64_t n, int64_t 
   Q8_CHECK_ARG(!isnan(temp), "q8op_probs: temp must not be NaN");
   if (rows == 0) return Q8_OK;
   Q8_CHECK_ARG(logits && out, "q8op_probs: null pointer");
-  const int c = vf_cluster(rows, n, (n + VF_SLICE - 1) / VF_SLICE, 2 * num_sms());
+  // one round of small CTAs if they fit, else large ones
+  const int64_t c_fine = (n + vf_slice(256) - 1) / vf_slice(256);
+  const bool fine = c_fine <= VF_MAX_CLUSTER && rows * c_fine <= 4 * num_sms();
+  const int slice = vf_slice(fine ? 256 : VF_THREADS);
+  const int c = vf_cluster(rows, n, (n + slice - 1) / slice, 2 * num_sms());
   const int per = (int)((n + c - 1) / c + 3) & ~3;
+  const int ahead = 2 * num_sms() / c;
   const double scale = std::min(1.4426950408889634 / (double)temp, 3e38);  // a subnormal temp: still no 0 x infinity
   const float ch = (float)scale, cl = (float)(scale - (double)ch);
-  return vf_launch("k_probs", k_probs, rows, c, 0, 0, (cudaStream_t)stream, logits, (int)n, ld, temp, ch, cl, out,
-                   ldo, per);
+  cudaStream_t st = (cudaStream_t)stream;
+  return fine ? vf_launch<k_probs<256>>("k_probs", rows, c, 256, 0, 0, st, logits, (int)rows, (int)n, ld, temp, ch, cl,
+                                        out, ldo, per, ahead)
+              : vf_launch<k_probs<VF_THREADS>>("k_probs", rows, c, VF_THREADS, 0, 0, st, logits, (int)rows, (int)n, ld,
+                                               temp, ch, cl, out, ldo, per, ahead);
 }
 
 extern "C" int q8op_verify(const float* p, int64_t ldp, const float* q, int64_t ldq, int64_t q_rows,
@@ -428,6 +442,6 @@ extern "C" int q8op_verify(const float* p, int64_t ldp, const float* q, int64_t 
   Q8_CHECK_ARG(seq_start && n_accepted && (rows == 0 || (p && ids && u && tokens)), "q8op_verify: null pointer");
   const int c = vf_cluster(S, n, 1, 2 * num_sms());
   const int per = (int)(((n + c - 1) / c + VF_SEG - 1) / VF_SEG * VF_SEG);
-  return vf_launch("k_verify", k_verify, S, c, (size_t)(per / VF_SEG) * 8, 20001 * 8, (cudaStream_t)stream, p, ldp, q,
+  return vf_launch<k_verify>("k_verify", S, c, VF_THREADS, (size_t)(per / VF_SEG) * 8, 20001 * 8, (cudaStream_t)stream, p, ldp, q,
                    ldq, (int)q_rows, ids, seq_start, (int)rows, (int)n, u, n_accepted, tokens, per);
 }
