@@ -61,9 +61,21 @@ __device__ __forceinline__ double vf_warp_sum(double v) {
   return v;
 }
 
+__device__ __forceinline__ void vf_send(const float* p, int rank, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(vf_map(p, rank)), "f"(v) : "memory");
+}
+__device__ __forceinline__ void vf_send(const int* p, int rank, int v) {
+  asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(vf_map(p, rank)), "r"(v) : "memory");
+}
+__device__ __forceinline__ void vf_send(const double* p, int rank, double v) {
+  asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(vf_map(p, rank)), "d"(v) : "memory");
+}
+
 // A cluster of CTAs per row, each with a slice of it in registers: logits are
-// read once and probabilities written once (8 bytes a logit), the maximum and
-// the sum are exchanged through distributed shared memory.
+// read once and probabilities written once (8 bytes a logit).  Every warp sends
+// its maximum, then its sum, to all CTAs; each adds up all warps' numbers in the
+// same order.  Nobody reads from a peer, so that only the sums' barrier is waited
+// for at the end.
 //
 // (l - max) / temp log2(e) is taken as y + z, y the f32 product with c = ch + cl
 // and z what it lost, so that the exponent's rounding does not grow with it:
@@ -73,9 +85,10 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
     k_probs(const float* __restrict__ logits, int rows, int n, int64_t ld, float temp, float ch, float cl,
             float* __restrict__ out, int64_t ldo, int per, int ahead) {
   constexpr int WARPS = THREADS / 32;
-  __shared__ float s_v[WARPS], s_top;
-  __shared__ int s_i[WARPS], s_arg;
-  __shared__ double s_d[WARPS], s_sum;
+  __shared__ float s_v[VF_MAX_CLUSTER * WARPS];
+  __shared__ int s_i[VF_MAX_CLUSTER * WARPS];
+  __shared__ double s_d[VF_MAX_CLUSTER * WARPS];
+  cluster_leave();  // that all CTAs have begun
   const cg::cluster_group cluster = cg::this_cluster();
   const int nc = cluster.num_blocks(), rank = cluster.block_rank(), row = blockIdx.x / nc;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
@@ -96,81 +109,64 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
       for (int e = 0; e < 4; ++e) v[k][e] = i + e < cnt ? src[i + e] : -INFINITY;
     }
   }
+  // what a CTA of the next round reads
   if (threadIdx.x == 0 && row < rows - ahead && wide && (ld & 3) == 0 && cnt >= 4)
     asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src + ahead * ld), "r"((cnt & ~3) * 4));
-  const bool greedy = !(temp > 0.f);
   float bv = -INFINITY;
-  int bi = 0x7fffffff;
 #pragma unroll
   for (int k = 0; k < VF_Q; ++k)
 #pragma unroll
     for (int e = 0; e < 4; ++e) bv = fmaxf(bv, v[k][e]);  // a NaN is passed over
-  if (greedy && bv > -INFINITY) {
+  bv = warp_max(bv);
+  cluster_left();
+  if (lane < nc) vf_send(&s_v[rank * WARPS + w], lane, bv);
+  cluster.sync();
+  for (int k = lane; k < nc * WARPS; k += 32) bv = fmaxf(bv, s_v[k]);
+  bv = warp_max(bv);
+  if (!(temp > 0.f) || bv == -INFINITY) {
+    int bi = 0x7fffffff;
 #pragma unroll
     for (int k = VF_Q - 1; k >= 0; --k)
 #pragma unroll
       for (int e = 3; e >= 0; --e)
-        if (v[k][e] == bv) bi = lo + at + k * 4 * THREADS + e;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    vf_best(bv, bi, __shfl_xor_sync(0xffffffffu, bv, o), __shfl_xor_sync(0xffffffffu, bi, o));
-  if (lane == 0) {
-    s_v[w] = bv;
-    s_i[w] = bi;
-  }
-  __syncthreads();
-  if (w == 0) {
-    bv = lane < WARPS ? s_v[lane] : -INFINITY;
-    bi = lane < WARPS ? s_i[lane] : 0x7fffffff;
-#pragma unroll
-    for (int o = WARPS / 2; o > 0; o >>= 1)
-      vf_best(bv, bi, __shfl_xor_sync(0xffffffffu, bv, o), __shfl_xor_sync(0xffffffffu, bi, o));
-    if (lane == 0) {
-      s_top = bv;
-      s_arg = bi;
-    }
-  }
-  cluster.sync();
-  bv = lane < nc ? vf_peer(&s_top, lane) : -INFINITY;
-  bi = lane < nc ? vf_peer(&s_arg, lane) : 0x7fffffff;
-#pragma unroll
-  for (int o = VF_MAX_CLUSTER / 2; o > 0; o >>= 1)
-    vf_best(bv, bi, __shfl_xor_sync(0xffffffffu, bv, o), __shfl_xor_sync(0xffffffffu, bi, o));
-  bv = __shfl_sync(0xffffffffu, bv, 0);
-  bi = __shfl_sync(0xffffffffu, bi, 0);
-  if (greedy || bv == -INFINITY) {
-    cluster_leave();
+        if (v[k][e] == bv && bv > -INFINITY) bi = lo + at + k * 4 * THREADS + e;
+    bi = __reduce_min_sync(0xffffffffu, bi);
+    if (lane < nc) vf_send(&s_i[rank * WARPS + w], lane, bi);
+    cluster.sync();
+    for (int k = lane; k < nc * WARPS; k += 32) bi = min(bi, s_i[k]);
+    bi = __reduce_min_sync(0xffffffffu, bi);
     if (bi == 0x7fffffff) bi = 0;  // nothing above -inf: as q8op_argmax
     for (int i = threadIdx.x; i < cnt; i += THREADS) dst[i] = lo + i == bi ? 1.f : 0.f;
-    cluster_left();
     return;
   }
-  const float low = bv - 16.f;
   double sum = 0.0;
+  if (bv == INFINITY) {  // the infinite ones alone
 #pragma unroll
-  for (int k = 0; k < VF_Q; ++k) {
+    for (int k = 0; k < VF_Q; ++k) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float l = v[k][e], d = l == bv ? 0.f : l - bv;  // inf - inf is 0 here
-      const float y = d * ch, z = fmaf(d, cl, fmaf(d, ch, -y));
-      float p;
-      asm("ex2.approx.f32 %0, %1;" : "=f"(p) : "f"(y));
-      v[k][e] = l >= low && y > -160.f ? fmaf(p, z * 0.69314718f, p) : 0.f;  // below 2^-149; z is no number at -inf
+      for (int e = 0; e < 4; ++e) v[k][e] = v[k][e] == bv ? 1.f : 0.f;
+      sum += (double)((v[k][0] + v[k][1]) + (v[k][2] + v[k][3]));
     }
-    sum += (double)((v[k][0] + v[k][1]) + (v[k][2] + v[k][3]));
+  } else {
+    const float low = fmaxf(bv - 16.f, bv - 160.f / ch);  // 2^-160 is 0, and y stays finite
+#pragma unroll
+    for (int k = 0; k < VF_Q; ++k) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float d = v[k][e] - bv, y = d * ch, z = fmaf(d, cl, fmaf(d, ch, -y));
+        float p;
+        asm("ex2.approx.f32 %0, %1;" : "=f"(p) : "f"(y));
+        v[k][e] = v[k][e] >= low ? fmaf(p * 0.69314718f, z, p) : 0.f;
+      }
+      sum += (double)((v[k][0] + v[k][1]) + (v[k][2] + v[k][3]));
+    }
   }
   sum = vf_warp_sum(sum);
-  if (lane == 0) s_d[w] = sum;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    sum = 0.0;
-    for (int k = 0; k < WARPS; ++k) sum += s_d[k];
-    s_sum = sum;
-  }
+  if (lane < nc) vf_send(&s_d[rank * WARPS + w], lane, sum);
   cluster.sync();
-  sum = vf_warp_sum(lane < nc ? vf_peer(&s_sum, lane) : 0.0);
-  cluster_leave();
+  sum = 0.0;
+  for (int k = lane; k < nc * WARPS; k += 32) sum += s_d[k];
+  sum = vf_warp_sum(sum);
   const float inv = (float)(1.0 / sum);
   const bool wide_out = ((uintptr_t)dst & 15) == 0;
 #pragma unroll
@@ -185,7 +181,6 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
         if (i + e < cnt) dst[i + e] = v[k][e] * inv;
     }
   }
-  cluster_left();  // nobody leaves while its sum is read
 }
 
 // A cluster of CTAs per sequence; all of them find the refused row, then each
