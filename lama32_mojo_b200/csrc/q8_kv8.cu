@@ -203,33 +203,40 @@ __global__ void __launch_bounds__(128, 10) k_kv8_append(Kv8Rows kr, Kv8Rows vr, 
       }
     return;
   }
-  const float inv = 1.f / s;
-  const int half_up = __float_as_int(s * 0.5f) + 1;  // the next number above s / 2
+  const float inv = 1.f / s, half = s * 0.5f;
   const uint64_t inv2 = kv8_two(inv, inv), s2 = kv8_two(s, s), magic = kv8_two(12582912.f, 12582912.f),
                  minus = kv8_two(-1.f, -1.f);
 #pragma unroll 2
   for (int t = tk; t < cnt; t += RPI) {
     Piece v;
     load(v, t);
-    uint32_t w[E / 4];
+    uint64_t m[E / 2], d[E / 2];
+    bool near = false;
 #pragma unroll
-    for (int e = 0; e < E; e += 4) {
-      uint32_t c[4];
+    for (int e = 0; e < E / 2; ++e) {
+      const uint64_t a = kv8_two(kv8_f32(v.e[2 * e]), kv8_f32(v.e[2 * e + 1]));
+      m[e] = kv8_fma2(a, inv2, magic);
+      d[e] = kv8_fma2(kv8_fma2(m[e], minus, magic), s2, a);
+      near |= fabsf(__uint_as_float((uint32_t)d[e])) >= half || fabsf(__uint_as_float((uint32_t)(d[e] >> 32))) >= half;
+    }
+    if (near) {  // next to a tie
 #pragma unroll
-      for (int j = 0; j < 4; j += 2) {
-        const uint64_t a = kv8_two(kv8_f32(v.e[e + j]), kv8_f32(v.e[e + j + 1]));
-        const uint64_t m = kv8_fma2(a, inv2, magic), d = kv8_fma2(kv8_fma2(m, minus, magic), s2, a);
+      for (int e = 0; e < E / 2; ++e) {
+        float mi[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const float di = __uint_as_float((uint32_t)(d >> (32 * i)));
-          float mi = __uint_as_float((uint32_t)(m >> (32 * i)));
-          const float edge = __int_as_float(half_up - (__float_as_int(mi) & 1));
-          if (fabsf(di) >= edge) mi += copysignf(1.f, di);
-          c[j + i] = __float_as_uint(mi);
+          const float di = __uint_as_float((uint32_t)(d[e] >> (32 * i)));
+          mi[i] = __uint_as_float((uint32_t)(m[e] >> (32 * i)));
+          if (fabsf(di) > half || (fabsf(di) == half && (__float_as_int(mi[i]) & 1))) mi[i] += copysignf(1.f, di);
         }
+        m[e] = kv8_two(mi[0], mi[1]);
       }
-      w[e / 4] = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
     }
+    uint32_t w[E / 4];
+#pragma unroll
+    for (int e = 0; e < E / 4; ++e)
+      w[e] = __byte_perm(__byte_perm((uint32_t)m[2 * e], (uint32_t)(m[2 * e] >> 32), 0x0040),
+                         __byte_perm((uint32_t)m[2 * e + 1], (uint32_t)(m[2 * e + 1] >> 32), 0x0040), 0x5410);
     if constexpr (E == 8) *reinterpret_cast<uint2*>(codes + (in + t) * HD) = make_uint2(w[0], w[1]);
     else *reinterpret_cast<uint32_t*>(codes + (in + t) * HD) = w[0];
   }
