@@ -227,8 +227,8 @@ int q8op_sample(const float* logits, int64_t rows, int64_t n, int64_t ld, float 
  * padding: nothing is read or written for them.  Rows that would lie before
  * position 0 have no position.  block_table [S, max_pages] int32 holds the
  * page of each `page` positions; an entry outside [0, num_pages), or a position
- * past the table, is a page that is not there.  All of these are device
- * memory.  Nothing is allocated and no scratch is shared inside the library:
+ * past the table, is a page that is not there; max_pages * page is below
+ * 2^31.  All of these are device memory.  Nothing is allocated and no scratch is shared inside the library:
  * calls on different streams are independent as long as their tensors are. */
 #define Q8_KV8_BLOCK 16
 typedef struct q8_kv8_pages {
@@ -333,7 +333,8 @@ int q8op_kv_copy_pages(void* const* pools, const int64_t* page_bytes, int n_pool
  * src/sample.mojo:15-59): p = w / sum w, w = exp((l - max) / temp) where
  * l >= max - 16, else 0.  temp <= 0: 1 at the first maximum.  NaN and -inf
  * count as never; a row without any other logit gives 1 at index 0.  logits
- * [rows, ld] f32 with n used columns, out [rows, ldo] f32. */
+ * [rows, ld] f32 with n used columns, out [rows, ldo] f32; out may be logits
+ * (with ldo = ld). */
 int q8op_probs(const float* logits, int64_t rows, int64_t n, int64_t ld, float temp, float* out, int64_t ldo,
                void* stream);
 

@@ -25,6 +25,7 @@ int kv8_check(const char* what, const q8_kv8_pages* kv, const int32_t* seq_start
   Q8_CHECK_ARG(S >= 0 && S <= (1 << 20) && rows >= 0 && rows <= (1 << 24) && max_pages > 0,
                "%s: bad shape (%lld sequences, %lld rows, %d table columns)", what, (long long)S, (long long)rows,
                max_pages);
+  Q8_CHECK_ARG((int64_t)max_pages * kv->page <= INT32_MAX, "%s: the table has more than 2^31 - 1 positions", what);
   return Q8_OK;
 }
 

@@ -422,7 +422,7 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
       for (int j = 0; j < w.n; ++j) {
         const uint32_t t = T + j, at_s = tmem + lanes + (t & 1) * KT_KEYS;
         const int p0 = (w.t0 + j) * KT_KEYS, left = lim - p0;
-        const bool masked = p0 + KT_KEYS > seen;
+        const bool masked = p0 > seen - KT_KEYS;
         mbar_wait(&scfull[t & 3], (t >> 2) & 1);
         mbar_wait(&sfull[t & 1], (t >> 1) & 1);
         kt_fence_after();

@@ -18,6 +18,7 @@ there, and may be captured into CUDA graphs.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import torch
 
@@ -305,10 +306,18 @@ def kv8_read(seq_start, ctx, pages: KV8Pages, block_table, rows: int):
     return k, v
 
 
+@functools.lru_cache(maxsize=1024)
+def _kv8_scratch(dev, *shape) -> int:
+    return lib().q8op_kv8_attention_workspace(*shape)
+
+
 def kv8_attention(q, seq_start, ctx, n_heads: int, pages: KV8Pages, block_table, out=None) -> torch.Tensor:
     """Causal GQA attention of packed rows over the 8-bit cache (q8op_kv8_attention).  Returns
     [T, n_heads * head_dim] of q's type; ``out`` may be given (its padding rows are left alone)."""
     S, width, dev = _packed("kv8_attention", seq_start, ctx, pages, block_table)
+    if torch.cuda.current_device() != dev:  # the scratch's size goes by the device
+        with torch.cuda.device(dev):
+            return kv8_attention(q, seq_start, ctx, n_heads, pages, block_table, out)
     w = n_heads * pages.head_dim
     T, ldq = _rows_of(q, "kv8_attention: q", w, dev)
     if out is None:
@@ -317,8 +326,7 @@ def kv8_attention(q, seq_start, ctx, n_heads: int, pages: KV8Pages, block_table,
         To, ldo = _rows_of(out, "kv8_attention: out", w, dev)
         if To != T or out.dtype != q.dtype:
             raise ValueError("kv8_attention: out must have q's rows and type")
-    nbytes = lib().q8op_kv8_attention_workspace(_DT[q.dtype], T, S, n_heads, pages.n_kv, pages.head_dim,
-                                                width * pages.page)
+    nbytes = _kv8_scratch(dev, _DT[q.dtype], T, S, n_heads, pages.n_kv, pages.head_dim, width * pages.page)
     work = torch.empty(nbytes, dtype=torch.uint8, device=q.device).data_ptr() if nbytes else None
     _call(lib().q8op_kv8_attention, dev, q.data_ptr(), ldq, _DT[q.dtype], T, seq_start.data_ptr(), ctx.data_ptr(), S,
           n_heads, pages._ref, block_table.data_ptr(), width, out.data_ptr(), ldo, work, nbytes)
@@ -416,7 +424,7 @@ def _matrix(t, what, dev: int):
 
 
 def probs(logits: torch.Tensor, temp: float, out: torch.Tensor = None) -> torch.Tensor:
-    """The distributions that sampling at ``temp`` and top_p = 1 draws from (q8op_probs)."""
+    """The distributions that sampling at ``temp`` and top_p = 1 draws from (q8op_probs); ``out`` may be ``logits``."""
     dev = logits.get_device()
     rows, n, ld = _matrix(logits, "probs: logits", dev)
     if out is None:

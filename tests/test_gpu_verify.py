@@ -61,6 +61,22 @@ def test_probs_many_rows(cuda):
     check_probs((rng.standard_normal((700, 1003)) * 4).astype(np.float32), 0.7, cuda, pad=1)
 
 
+@pytest.mark.parametrize("rows,n", [(300, 30011), (5, 200001), (2, 327680)])
+@pytest.mark.parametrize("temp", [0.0, 0.9])
+def test_probs_large_slices(cuda, rows, n, temp):
+    """More rows than fit at once, and rows that take the larger CTAs; equal maxima in several of them."""
+    x = (np.random.default_rng(n).standard_normal((rows, n)) * 3).astype(np.float32)
+    x[1, [n - 1, 17, n // 2]] = 40.0
+    x[0, n // 3] = np.inf
+    check_probs(x, temp, cuda, pad=rows % 4)
+
+
+def test_probs_in_place(cuda):
+    x = torch.randn((40, 50000), device=cuda) * 4
+    want = ops.probs(x, 0.8)
+    assert ops.probs(x, 0.8, out=x) is x and torch.equal(x, want)
+
+
 def test_probs_special_rows(cuda):
     inf, nan, low = np.inf, np.nan, np.finfo(np.float32).min
     rows = np.zeros((9, 40), np.float32)

@@ -39,6 +39,8 @@ def test_kv8_entries_refuse():
     refused(append(rows=-1), "shape")
     refused(append(S=-1), "shape")
     refused(append(width=0), "shape")
+    refused(append(width=1 << 27), "positions")
+    refused(attend(width=1 << 27), "positions")
     for bad in (dict(page=24), dict(page=0), dict(head_dim=96), dict(num_pages=0), dict(n_kv=0), dict(k=None),
                 dict(v=None), dict(k_scale=None), dict(v_scale=None), dict(k=ONE + 8)):
         assert append(kv=pages(**bad)) == _lib.Q8_ERR_ARG
