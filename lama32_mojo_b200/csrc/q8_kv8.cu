@@ -77,16 +77,6 @@ __device__ __forceinline__ unsigned kv8_max(unsigned top, unsigned w) {
   }
 }
 
-// two floats in a register pair, and their packed fused multiply-add
-__device__ __forceinline__ uint64_t kv8_two(float a, float b) {
-  return (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a);
-}
-__device__ __forceinline__ uint64_t kv8_fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-
 // One warp per (block of 16 positions, kv head, k or v).  A lane takes 16 bytes
 // of a row, the warp as many rows as fit; the rows are read twice, for the
 // scale and for the codes (the second time from the caches), which takes half
@@ -205,8 +195,8 @@ __global__ void __launch_bounds__(128, 10) k_kv8_append(Kv8Rows kr, Kv8Rows vr, 
     return;
   }
   const float inv = 1.f / s, half = s * 0.5f;
-  const uint64_t inv2 = kv8_two(inv, inv), s2 = kv8_two(s, s), magic = kv8_two(12582912.f, 12582912.f),
-                 minus = kv8_two(-1.f, -1.f);
+  const uint64_t inv2 = f2_pack(inv, inv), s2 = f2_pack(s, s), magic = f2_pack(12582912.f, 12582912.f),
+                 minus = f2_pack(-1.f, -1.f);
 #pragma unroll 2
   for (int t = tk; t < cnt; t += RPI) {
     Piece v;
@@ -215,10 +205,10 @@ __global__ void __launch_bounds__(128, 10) k_kv8_append(Kv8Rows kr, Kv8Rows vr, 
     bool near = false;
 #pragma unroll
     for (int e = 0; e < E / 2; ++e) {
-      const uint64_t a = kv8_two(kv8_f32(v.e[2 * e]), kv8_f32(v.e[2 * e + 1]));
-      m[e] = kv8_fma2(a, inv2, magic);
-      d[e] = kv8_fma2(kv8_fma2(m[e], minus, magic), s2, a);
-      near |= fabsf(__uint_as_float((uint32_t)d[e])) >= half || fabsf(__uint_as_float((uint32_t)(d[e] >> 32))) >= half;
+      const uint64_t a = f2_pack(kv8_f32(v.e[2 * e]), kv8_f32(v.e[2 * e + 1]));
+      m[e] = f2_fma(a, inv2, magic);
+      d[e] = f2_fma(f2_fma(m[e], minus, magic), s2, a);
+      near |= fabsf(f2_lo(d[e])) >= half || fabsf(f2_hi(d[e])) >= half;
     }
     if (near) {  // next to a tie
 #pragma unroll
@@ -226,11 +216,11 @@ __global__ void __launch_bounds__(128, 10) k_kv8_append(Kv8Rows kr, Kv8Rows vr, 
         float mi[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const float di = __uint_as_float((uint32_t)(d[e] >> (32 * i)));
-          mi[i] = __uint_as_float((uint32_t)(m[e] >> (32 * i)));
+          const float di = i ? f2_hi(d[e]) : f2_lo(d[e]);
+          mi[i] = i ? f2_hi(m[e]) : f2_lo(m[e]);
           if (fabsf(di) > half || (fabsf(di) == half && (__float_as_int(mi[i]) & 1))) mi[i] += copysignf(1.f, di);
         }
-        m[e] = kv8_two(mi[0], mi[1]);
+        m[e] = f2_pack(mi[0], mi[1]);
       }
     }
     uint32_t w[E / 4];

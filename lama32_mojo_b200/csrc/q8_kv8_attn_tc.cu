@@ -108,28 +108,6 @@ __device__ __forceinline__ void kt_st16(uint32_t addr, const uint32_t (&r)[16]) 
 }
 __device__ __forceinline__ void kt_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// two floats in a register pair, and packed operations on them
-__device__ __forceinline__ uint64_t kt_two(float a, float b) {
-  return (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a);
-}
-__device__ __forceinline__ float kt_lo(uint64_t x) { return __uint_as_float((uint32_t)x); }
-__device__ __forceinline__ float kt_hi(uint64_t x) { return __uint_as_float((uint32_t)(x >> 32)); }
-__device__ __forceinline__ uint64_t kt_fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t kt_mul2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ uint64_t kt_add2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-
 // The largest score + log2(sv) of a row's tile; left: positions of the tile that the row sees.
 template <bool MASKED>
 __device__ __forceinline__ float kt_top(uint32_t addr, const float4* sc, float fac, int left) {
@@ -155,7 +133,7 @@ __device__ __forceinline__ float kt_top(uint32_t addr, const float4* sc, float f
 template <bool WIDE, bool MASKED>
 __device__ __forceinline__ float kt_weights(uint32_t addr, const float4* sc, float fac, float ref, int left) {
   uint64_t sum = 0ull;
-  const uint64_t minus = kt_two(-1.f, -1.f);
+  const uint64_t minus = f2_pack(-1.f, -1.f);
 #pragma unroll 1
   for (int h = 0; h < 2; ++h) {
     float v[32];
@@ -165,30 +143,30 @@ __device__ __forceinline__ float kt_weights(uint32_t addr, const float4* sc, flo
     for (int k = 0; k < 2; ++k) {
       const float4 s = sc[h * 2 + k];
       const float f = fac * s.x, b = s.z == -INFINITY ? -INFINITY : -ref;  // a missing page: 0 s - infinity
-      const uint64_t f2 = kt_two(f, f), b2 = kt_two(b, b), w2 = kt_two(s.y, s.y);
+      const uint64_t f2 = f2_pack(f, f), b2 = f2_pack(b, b), w2 = f2_pack(s.y, s.y);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int q = k * 16 + 2 * i;
-        const uint64_t x = kt_fma2(kt_two(v[q], v[q + 1]), f2, b2);
-        float e0 = ka_exp2(kt_lo(x)), e1 = ka_exp2(kt_hi(x));
+        const uint64_t x = f2_fma(f2_pack(v[q], v[q + 1]), f2, b2);
+        float e0 = ka_exp2(f2_lo(x)), e1 = ka_exp2(f2_hi(x));
         if (MASKED) {
           if (q >= left - h * 32) e0 = 0.f;
           if (q + 1 >= left - h * 32) e1 = 0.f;
         }
-        const uint64_t e = kt_two(e0, e1), p = kt_mul2(e, w2);
-        sum = kt_add2(sum, e);
-        hi[k * 8 + i] = ka_pack(kt_lo(p), kt_hi(p));
+        const uint64_t e = f2_pack(e0, e1), p = f2_mul(e, w2);
+        sum = f2_add(sum, e);
+        hi[k * 8 + i] = ka_pack(f2_lo(p), f2_hi(p));
         if (WIDE) {
           const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&hi[k * 8 + i]));
-          const uint64_t r = kt_fma2(kt_two(y.x, y.y), minus, p);
-          lo[k * 8 + i] = ka_pack(kt_lo(r), kt_hi(r));
+          const uint64_t r = f2_fma(f2_pack(y.x, y.y), minus, p);
+          lo[k * 8 + i] = ka_pack(f2_lo(r), f2_hi(r));
         }
       }
     }
     kt_st16(addr + h * 32, hi);
     if (WIDE) kt_st16(addr + h * 32 + 16, lo);
   }
-  return kt_lo(sum) + kt_hi(sum);
+  return f2_lo(sum) + f2_hi(sum);
 }
 
 // f32 rows: the tensor cores cut sums off where an f32 addition rounds, and O has

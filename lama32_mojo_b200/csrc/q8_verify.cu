@@ -77,9 +77,10 @@ __device__ __forceinline__ void vf_send(const double* p, int rank, double v) {
 // same order.  Nobody reads from a peer, so that only the sums' barrier is waited
 // for at the end.
 //
-// (l - max) / temp log2(e) is taken as y + z, y the f32 product with c = ch + cl
-// and z what it lost, so that the exponent's rounding does not grow with it:
-// w = 2^y (1 + z ln 2).  Four weights are added in 32 bits, those sums in 64.
+// (l - max) / temp log2(e) + 64 is taken as y + z, y the f32 multiply-add with
+// c = ch + cl and z what it lost, so that the exponent's rounding does not grow
+// with it: w = 2^y (1 + z ln 2).  The 64 keeps the weights that count, from 2^-96
+// to 2^64, among the normal numbers.  Four are added in 32 bits, those sums in 64.
 template <int THREADS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
     k_probs(const float* __restrict__ logits, int rows, int n, int64_t ld, float temp, float ch, float cl,
@@ -149,16 +150,26 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
     }
   } else {
     const float low = fmaxf(bv - 16.f, bv - 160.f / ch);  // 2^-160 is 0, and y stays finite
+    const uint64_t top2 = f2_pack(-bv, -bv), ch2 = f2_pack(ch, ch), cl2 = f2_pack(cl, cl), up = f2_pack(64.f, 64.f),
+                   minus = f2_pack(-1.f, -1.f), ln2 = f2_pack(0.69314718f, 0.69314718f);
 #pragma unroll
     for (int k = 0; k < VF_Q; ++k) {
+      uint64_t p[2];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float d = v[k][e] - bv, y = d * ch, z = fmaf(d, cl, fmaf(d, ch, -y));
-        float p;
-        asm("ex2.approx.f32 %0, %1;" : "=f"(p) : "f"(y));
-        v[k][e] = v[k][e] >= low ? fmaf(p * 0.69314718f, z, p) : 0.f;
+      for (int e = 0; e < 2; ++e) {
+        const float l0 = v[k][2 * e], l1 = v[k][2 * e + 1];
+        const uint64_t d = f2_add(f2_pack(l0, l1), top2), y = f2_fma(d, ch2, up);
+        const uint64_t z = f2_fma(d, cl2, f2_fma(d, ch2, f2_fma(y, minus, up)));  // y - 64 is exact
+        float p0, p1;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p0) : "f"(f2_lo(y)));
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p1) : "f"(f2_hi(y)));
+        p[e] = f2_pack(p0, p1);
+        p[e] = f2_fma(f2_mul(p[e], ln2), z, p[e]);
+        v[k][2 * e] = l0 >= low ? f2_lo(p[e]) : 0.f;
+        v[k][2 * e + 1] = l1 >= low ? f2_hi(p[e]) : 0.f;
       }
-      sum += (double)((v[k][0] + v[k][1]) + (v[k][2] + v[k][3]));
+      const uint64_t two = f2_add(f2_pack(v[k][0], v[k][1]), f2_pack(v[k][2], v[k][3]));
+      sum += (double)(f2_lo(two) + f2_hi(two));
     }
   }
   sum = vf_warp_sum(sum);
