@@ -86,8 +86,8 @@ const char* q8_status_string(int status);
 /* Library build string (arch, version). */
 const char* q8_version(void);
 /* Synchronizes the current device, then reports and clears a timeout that a
-   bounded barrier wait inside a tensor-core GEMM or the decode attention
-   recorded (Q8_ERR_TIMEOUT), else Q8_OK.  The model entry points (q8_forward,
+   bounded barrier wait inside a tensor-core GEMM, the decode attention or the
+   chunk attention over the 8-bit cache recorded (Q8_ERR_TIMEOUT), else Q8_OK.  The model entry points (q8_forward,
    q8_forward_hidden, q8_decode, q8_generate) read both words after every call,
    with the call's other results, and fail with Q8_ERR_TIMEOUT when one is set;
    op-level callers poll this when they synchronize.  No counterpart in the

@@ -18,6 +18,11 @@
 // M moves only when it has grown by more than 1, so that O in TMEM is scaled
 // seldom; weights stay below 2, lifted by 2^14.
 //
+// Bound.  2 x 1024 f32 rows of 32 heads on 8 of 128, 8000 positions: 385 us for
+// 258 GFLOP, 516 in f16 products (1.34 PFLOP/s, 0.81 of cuBLAS's bf16 rate).  The
+// tensor pipes are busy 40 % of the time, the issue slots 52 %: the chain from
+// scores to weights is what is waited for.
+//
 // Two CTAs an SM (256 TMEM columns each) cover one another's waits.  Their
 // number is fixed; each takes an equal stretch of all units' work and leaves
 // partial results where it begins or ends inside a unit (q8_kv8_attn.cu).

@@ -6,7 +6,10 @@
 // lengths, refs [num_pages] int32, the table entries that hold a page; 0 is
 // free.  There is no list of free pages: a page is taken by scanning refs, the
 // lowest number first, so equal states give equal results.  Sums into refs are
-// integer atomics; their order does not matter.
+// integer atomics; their order does not matter.  Tables are small: the kernels on
+// them wait for memory a few times in a row, which takes 3 to 11 us whatever
+// their sizes are (64 sequences of 16 pages: truncate 4, fork 7, reserve 11,
+// compact of 3000 pages 8 us with nothing in the caches).
 #include "q8_kernels.h"
 
 #include <algorithm>
@@ -291,7 +294,8 @@ struct PoolList {
 // order.  Every CTA marks the call's page numbers in bitmaps (sources,
 // destinations, destinations seen twice), lists the pairs that remain, and
 // takes its share of their 16 KB pieces: 64 bytes of a piece per thread, all
-// loaded before the first is stored.
+// loaded before the first is stored.  0.77 GB: 123 us, 6.3 TB/s or 0.96 of a
+// copy's rate; 50 MB: 10 us.
 constexpr int PG_COPY_THREADS = 256;
 constexpr int PG_PIECE = PG_COPY_THREADS * 64;
 constexpr int PG_LIST = 2048;  // pairs per pass
