@@ -266,8 +266,8 @@ __global__ void __launch_bounds__(256) k_kv8_read(int rows, const int32_t* __res
       k = make_float4(ck.x * sk, ck.y * sk, ck.z * sk, ck.w * sk);
       v = make_float4(cv.x * sv, cv.y * sv, cv.z * sv, cv.w * sv);
     }
-    *reinterpret_cast<float4*>(ko + o0 + i) = k;
-    *reinterpret_cast<float4*>(vo + o0 + i) = v;
+    __stcs(reinterpret_cast<float4*>(ko + o0 + i), k);
+    __stcs(reinterpret_cast<float4*>(vo + o0 + i), v);
   }
 }
 
