@@ -57,12 +57,24 @@ __device__ __forceinline__ int kv8_rescale(int c, float ratio, float s0, float s
 struct Kv8Rows {
   const void* x;
   int64_t ld;
-  bool aligned;  // to 16 bytes
 };
 
 __device__ __forceinline__ float kv8_f32(float x) { return x; }
 __device__ __forceinline__ float kv8_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float kv8_f32(__half x) { return __half2float(x); }
+
+// elements 2i and 2i + 1 of a 16-byte piece
+template <typename T>
+__device__ __forceinline__ uint64_t kv8_pair(const uint32_t (&u)[4], int i) {
+  if constexpr (sizeof(T) == 4) {
+    return (uint64_t)u[2 * i + 1] << 32 | u[2 * i];
+  } else if constexpr (std::is_same<T, __half>::value) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+    return f2_pack(f.x, f.y);
+  } else {
+    return (uint64_t)(u[i] & 0xffff0000u) << 32 | u[i] << 16;
+  }
+}
 
 // the larger of top and |w|, by pairs for 16-bit elements; NaN is the largest
 template <typename T>
@@ -93,7 +105,7 @@ __device__ __forceinline__ unsigned kv8_max(unsigned top, unsigned w) {
 // d = x - r s, which is exact, tells: r moves towards x where |d| > s / 2, or
 // where it is s / 2 and r odd (m's last bit).  Blocks with numbers that are not
 // finite, or scales far outside the usual ones, go the long way (kv8_code).
-template <typename T, int HD>
+template <typename T, int HD, bool ALIGNED>  // rows to 16 bytes; known when compiled: a branch at each load costs 4 us
 __global__ void __launch_bounds__(128, 10) k_kv8_append(Kv8Rows kr, Kv8Rows vr, int rows,
                                                         const int32_t* __restrict__ starts,
                                                         const int32_t* __restrict__ ctx, int S, q8_kv8_pages kv,
@@ -124,7 +136,7 @@ __global__ void __launch_bounds__(128, 10) k_kv8_append(Kv8Rows kr, Kv8Rows vr, 
     __device__ Piece() {}
   };
   auto load = [&](Piece& v, int t) {
-    if (src.aligned) {
+    if constexpr (ALIGNED) {
       v.w = *reinterpret_cast<const uint4*>(x + (int64_t)t * src.ld);
     } else {
 #pragma unroll
@@ -207,7 +219,7 @@ __global__ void __launch_bounds__(128, 10) k_kv8_append(Kv8Rows kr, Kv8Rows vr, 
     bool near = false;
 #pragma unroll
     for (int e = 0; e < E / 2; ++e) {
-      const uint64_t a = f2_pack(kv8_f32(v.e[2 * e]), kv8_f32(v.e[2 * e + 1]));
+      const uint64_t a = kv8_pair<T>(v.u, e);
       m[e] = f2_fma(a, inv2, magic);
       d[e] = f2_fma(f2_fma(m[e], minus, magic), s2, a);
       near |= fabsf(f2_lo(d[e])) >= half || fabsf(f2_hi(d[e])) >= half;
@@ -271,13 +283,21 @@ __global__ void __launch_bounds__(256) k_kv8_read(int rows, const int32_t* __res
   }
 }
 
-template <typename T>
+template <typename T, int HD>
 static int append_run(const Kv8Rows& k, const Kv8Rows& v, int rows, const int32_t* starts, const int32_t* ctx, int S,
                       const q8_kv8_pages& kv, const int32_t* table, int max_pages, cudaStream_t st) {
   const dim3 grid(rows / KV8_BLOCK + 2 * S, ceil_div(2 * kv.n_kv, 4));
-  if (kv.head_dim == 64) k_kv8_append<T, 64><<<grid, 128, 0, st>>>(k, v, rows, starts, ctx, S, kv, table, max_pages);
-  else k_kv8_append<T, 128><<<grid, 128, 0, st>>>(k, v, rows, starts, ctx, S, kv, table, max_pages);
+  const bool aligned = (((uintptr_t)k.x | (uintptr_t)v.x | (k.ld * sizeof(T)) | (v.ld * sizeof(T))) & 15) == 0;
+  auto kern = aligned ? k_kv8_append<T, HD, true> : k_kv8_append<T, HD, false>;
+  kern<<<grid, 128, 0, st>>>(k, v, rows, starts, ctx, S, kv, table, max_pages);
   return launch_check("k_kv8_append");
+}
+
+template <typename T>
+static int append_run(const Kv8Rows& k, const Kv8Rows& v, int rows, const int32_t* starts, const int32_t* ctx, int S,
+                      const q8_kv8_pages& kv, const int32_t* table, int max_pages, cudaStream_t st) {
+  return kv.head_dim == 64 ? append_run<T, 64>(k, v, rows, starts, ctx, S, kv, table, max_pages, st)
+                           : append_run<T, 128>(k, v, rows, starts, ctx, S, kv, table, max_pages, st);
 }
 
 }  // namespace q8
@@ -293,9 +313,7 @@ extern "C" int q8op_kv8_append(const void* k, int64_t ldk, const void* v, int64_
   const int64_t width = (int64_t)kv->n_kv * kv->head_dim;
   Q8_CHECK_ARG(k && v && ldk >= width && ldv >= width, "q8op_kv8_append: k and v rows need %lld elements",
                (long long)width);
-  const int64_t size = dtype == Q8_F32 ? 4 : 2;
-  const Kv8Rows kr{k, ldk, (((uintptr_t)k | (uintptr_t)(ldk * size)) & 15) == 0},
-      vr{v, ldv, (((uintptr_t)v | (uintptr_t)(ldv * size)) & 15) == 0};
+  const Kv8Rows kr{k, ldk}, vr{v, ldv};
   cudaStream_t st = (cudaStream_t)stream;
   if (dtype == Q8_F32)
     return append_run<float>(kr, vr, (int)rows, seq_start, ctx, (int)S, *kv, block_table, max_pages, st);

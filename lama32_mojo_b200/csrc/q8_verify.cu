@@ -86,7 +86,7 @@ __device__ __forceinline__ void vf_send(const double* p, int rank, double v) {
 // an SM take turns in loading, waiting for one another and storing.  One row of
 // 128,256: 5.8 us in CTAs of 256 threads, 8.1 in CTAs of 512.  Sending by st.async
 // instead (102 us) and clusters that stay and load a row ahead (107) were slower.
-template <int THREADS>
+template <int THREADS, bool WIDE>  // WIDE: rows to 16 bytes; loads behind a branch each would wait for one another
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
     k_probs(const float* __restrict__ logits, int rows, int n, int64_t ld, float temp, float ch, float cl,
             float* __restrict__ out, int64_t ldo, int per, int ahead) {
@@ -102,21 +102,34 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
   const float* src = logits + (int64_t)row * ld + lo;
   float* dst = out + (int64_t)row * ldo + lo;
   const int at = threadIdx.x * 4;  // piece k: at + k * 4 * THREADS
-  const bool wide = ((uintptr_t)src & 15) == 0;
   float v[VF_Q][4];
 #pragma unroll
   for (int k = 0; k < VF_Q; ++k) {
     const int i = at + k * 4 * THREADS;
-    if (wide && i + 4 <= cnt) {
-      const float4 f = __ldcs(reinterpret_cast<const float4*>(src + i));
-      v[k][0] = f.x, v[k][1] = f.y, v[k][2] = f.z, v[k][3] = f.w;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[k][e] = -INFINITY;
+    if constexpr (WIDE) {
+      if (i + 4 <= cnt) {
+        const float4 f = __ldcs(reinterpret_cast<const float4*>(src + i));
+        v[k][0] = f.x, v[k][1] = f.y, v[k][2] = f.z, v[k][3] = f.w;
+      }
     } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[k][e] = i + e < cnt ? src[i + e] : -INFINITY;
+      for (int e = 0; e < 4; ++e)
+        if (i + e < cnt) v[k][e] = src[i + e];
+    }
+  }
+  if (WIDE && (cnt & 3)) {
+#pragma unroll
+    for (int k = 0; k < VF_Q; ++k) {
+      const int i = at + k * 4 * THREADS;
+#pragma unroll
+      for (int e = 0; e < 3; ++e)
+        if (i + 4 > cnt && i + e < cnt) v[k][e] = src[i + e];
     }
   }
   // what a CTA of the next round reads
-  if (threadIdx.x == 0 && row < rows - ahead && wide && (ld & 3) == 0 && cnt >= 4)
+  if (WIDE && threadIdx.x == 0 && row < rows - ahead && cnt >= 4)
     asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src + ahead * ld), "r"((cnt & ~3) * 4));
   float bv = -INFINITY;
 #pragma unroll
@@ -184,11 +197,10 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
   for (int k = lane; k < nc * WARPS; k += 32) sum += s_d[k];
   sum = vf_warp_sum(sum);
   const float inv = (float)(1.0 / sum);
-  const bool wide_out = ((uintptr_t)dst & 15) == 0;
 #pragma unroll
   for (int k = 0; k < VF_Q; ++k) {
     const int i = at + k * 4 * THREADS;
-    if (wide_out && i + 4 <= cnt) {
+    if (WIDE && i + 4 <= cnt) {
       __stcs(reinterpret_cast<float4*>(dst + i),
              make_float4(v[k][0] * inv, v[k][1] * inv, v[k][2] * inv, v[k][3] * inv));
     } else {
@@ -385,6 +397,11 @@ static int vf_cluster(int64_t rows, int64_t n, int64_t least, int64_t room) {
   return c;
 }
 
+template <auto kern>
+struct VfKernel {
+  static constexpr auto value = kern;
+};
+
 template <auto kern, typename... Args>
 static int vf_launch(const char* what, int64_t rows, int c, int threads, size_t smem, int most, cudaStream_t st,
                      Args... args) {
@@ -439,10 +456,14 @@ extern "C" int q8op_probs(const float* logits, int64_t rows, int64_t n, int64_t 
   const double scale = std::min(1.4426950408889634 / (double)temp, 3e38);  // a subnormal temp: still no 0 x infinity
   const float ch = (float)scale, cl = (float)(scale - (double)ch);
   cudaStream_t st = (cudaStream_t)stream;
-  return fine ? vf_launch<k_probs<256>>("k_probs", rows, c, 256, 0, 0, st, logits, (int)rows, (int)n, ld, temp, ch, cl,
-                                        out, ldo, per, ahead)
-              : vf_launch<k_probs<VF_THREADS>>("k_probs", rows, c, VF_THREADS, 0, 0, st, logits, (int)rows, (int)n, ld,
-                                               temp, ch, cl, out, ldo, per, ahead);
+  const bool wide = (((uintptr_t)logits | (uintptr_t)out | (uintptr_t)(ld * 4) | (uintptr_t)(ldo * 4)) & 15) == 0;
+  auto go = [&](auto kernel, int threads) {
+    return vf_launch<decltype(kernel)::value>("k_probs", rows, c, threads, 0, 0, st, logits, (int)rows, (int)n, ld, temp,
+                                              ch, cl, out, ldo, per, ahead);
+  };
+  if (fine) return wide ? go(VfKernel<k_probs<256, true>>{}, 256) : go(VfKernel<k_probs<256, false>>{}, 256);
+  return wide ? go(VfKernel<k_probs<VF_THREADS, true>>{}, VF_THREADS)
+              : go(VfKernel<k_probs<VF_THREADS, false>>{}, VF_THREADS);
 }
 
 extern "C" int q8op_verify(const float* p, int64_t ldp, const float* q, int64_t ldq, int64_t q_rows,
