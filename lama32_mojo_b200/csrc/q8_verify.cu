@@ -15,6 +15,7 @@
 #include <algorithm>
 #include <cooperative_groups.h>
 #include <math.h>
+#include <type_traits>
 
 namespace cg = cooperative_groups;
 
@@ -84,12 +85,12 @@ __device__ __forceinline__ void vf_send(const double* p, int rank, double v) {
 //
 // 320 rows of 151,936: 91 us for 389 MB (4.3 TB/s, 0.65 of a copy's rate); two CTAs
 // an SM take turns in loading, waiting for one another and storing.  One row of
-// 128,256: 5.8 us in CTAs of 256 threads, 8.1 in CTAs of 512.  Sending by st.async
+// 128,256: 5.4 us in CTAs of 256 threads, 7.5 in CTAs of 512.  Sending by st.async
 // instead (102 us) and clusters that stay and load a row ahead (107) were slower.
 template <int THREADS, bool WIDE>  // WIDE: rows to 16 bytes; loads behind a branch each would wait for one another
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
-    k_probs(const float* __restrict__ logits, int rows, int n, int64_t ld, float temp, float ch, float cl,
-            float* __restrict__ out, int64_t ldo, int per, int ahead) {
+    k_probs(const float* __restrict__ logits, int n, int64_t ld, float temp, float ch, float cl,
+            float* __restrict__ out, int64_t ldo, int per) {
   constexpr int WARPS = THREADS / 32;
   __shared__ float s_v[VF_MAX_CLUSTER * WARPS];
   __shared__ int s_i[VF_MAX_CLUSTER * WARPS];
@@ -128,9 +129,6 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
         if (i + 4 > cnt && i + e < cnt) v[k][e] = src[i + e];
     }
   }
-  // what a CTA of the next round reads
-  if (WIDE && threadIdx.x == 0 && row < rows - ahead && cnt >= 4)
-    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src + ahead * ld), "r"((cnt & ~3) * 4));
   float bv = -INFINITY;
 #pragma unroll
   for (int k = 0; k < VF_Q; ++k)
@@ -268,14 +266,16 @@ __global__ void __launch_bounds__(VF_THREADS) k_verify(const float* __restrict__
   const int lo = min(n, rank * per), hi = min(n, lo + per);
   const int segs = (hi - lo + VF_SEG - 1) / VF_SEG;
   const bool wide = (((uintptr_t)pr | (uintptr_t)qr) & 15) == 0;  // lo is a multiple of VF_SEG
-  // the lane's four weights of a segment
-  auto weights = [&](int seg, double (&v)[4]) {
+  // the lane's four weights of a segment; HOW 0: p alone, 1: p - q, both by 16 bytes and the
+  // segment full, 2: any
+  auto weights_of = [&](auto how, int seg, double (&v)[4]) {
+    constexpr int HOW = decltype(how)::value;
     const int i = lo + seg * VF_SEG + lane * 4;
     float a[4] = {0.f, 0.f, 0.f, 0.f}, c[4] = {0.f, 0.f, 0.f, 0.f};
-    if (wide && i + 4 <= hi) {
+    if constexpr (HOW < 2) {
       const float4 f = *reinterpret_cast<const float4*>(pr + i);
       a[0] = f.x, a[1] = f.y, a[2] = f.z, a[3] = f.w;
-      if (qr) {
+      if constexpr (HOW == 1) {
         const float4 h = *reinterpret_cast<const float4*>(qr + i);
         c[0] = h.x, c[1] = h.y, c[2] = h.z, c[3] = h.w;
       }
@@ -293,19 +293,28 @@ __global__ void __launch_bounds__(VF_THREADS) k_verify(const float* __restrict__
       v[e] = d > 0.0 && i + e != gone ? d : 0.0;
     }
   };
+  const int plain = wide ? (hi - lo) / VF_SEG : 0;  // segments that loads of 16 bytes can take
   double total = 0.0, before = 0.0;
   for (;;) {
     int last = -1;
-#pragma unroll 4
-    for (int s = wid; s < segs; s += VF_WARPS) {
+    auto add_up = [&](auto how, int s) {
       double v[4];
-      weights(s, v);
+      weights_of(how, s, v);
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (v[e] > 0.0) last = lo + s * VF_SEG + lane * 4 + e;
       const double sum = vf_warp_sum((v[0] + v[1]) + (v[2] + v[3]));
       if (lane == 0) s_seg[s] = sum;
+    };
+    int s = wid;  // a branch around the loads, not one at each
+    if (qr) {
+#pragma unroll 4
+      for (; s < plain; s += VF_WARPS) add_up(std::integral_constant<int, 1>(), s);
+    } else {
+#pragma unroll 4
+      for (; s < plain; s += VF_WARPS) add_up(std::integral_constant<int, 0>(), s);
     }
+    for (; s < segs; s += VF_WARPS) add_up(std::integral_constant<int, 2>(), s);
     last = __reduce_max_sync(0xffffffffu, last);
     if (lane == 0 && last >= 0) atomicMax(&s_last, last);
     __syncthreads();
@@ -356,7 +365,7 @@ __global__ void __launch_bounds__(VF_THREADS) k_verify(const float* __restrict__
         else a = mid + 1;
       }
       double v[4], cum = 0.0;
-      weights(a, v);
+      weights_of(std::integral_constant<int, 2>(), a, v);
       cum = ((v[0] + v[1]) + v[2]) + v[3];
       double up = cum;
 #pragma unroll
@@ -452,14 +461,13 @@ extern "C" int q8op_probs(const float* logits, int64_t rows, int64_t n, int64_t 
   const int slice = vf_slice(fine ? 256 : VF_THREADS);
   const int c = vf_cluster(rows, n, (n + slice - 1) / slice, 2 * num_sms());
   const int per = (int)((n + c - 1) / c + 3) & ~3;
-  const int ahead = 2 * num_sms() / c;
   const double scale = std::min(1.4426950408889634 / (double)temp, 3e38);  // a subnormal temp: still no 0 x infinity
   const float ch = (float)scale, cl = (float)(scale - (double)ch);
   cudaStream_t st = (cudaStream_t)stream;
   const bool wide = (((uintptr_t)logits | (uintptr_t)out | (uintptr_t)(ld * 4) | (uintptr_t)(ldo * 4)) & 15) == 0;
   auto go = [&](auto kernel, int threads) {
-    return vf_launch<decltype(kernel)::value>("k_probs", rows, c, threads, 0, 0, st, logits, (int)rows, (int)n, ld, temp,
-                                              ch, cl, out, ldo, per, ahead);
+    return vf_launch<decltype(kernel)::value>("k_probs", rows, c, threads, 0, 0, st, logits, (int)n, ld, temp,
+                                              ch, cl, out, ldo, per);
   };
   if (fine) return wide ? go(VfKernel<k_probs<256, true>>{}, 256) : go(VfKernel<k_probs<256, false>>{}, 256);
   return wide ? go(VfKernel<k_probs<VF_THREADS, true>>{}, VF_THREADS)
