@@ -218,6 +218,22 @@ def test_append_quotients_next_to_a_tie(cuda):
     host.check(pages)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("hd,shift", [(128, 1), (64, 3)])
+def test_append_unaligned_rows(cuda, dtype, hd, shift):
+    """Rows that do not begin at a multiple of 16 bytes, k and v with strides of their own."""
+    kv, page, ns, ctx = 3, 32, np.array([21, 5, 40]), np.array([30, 5, 77])
+    T, w = int(ns.sum()), kv * hd
+    pages = make_pages(cuda, 8, kv, page, hd, shift)
+    host = HostCache(pages)
+    table = make_table(ctx, page, 8, shift)
+    k = torch.randn((T, w + 5), device=cuda).to(DT[dtype])[:, shift:shift + w]
+    v = torch.randn((T, w + 8), device=cuda).to(DT[dtype])[:, :w]
+    ops.kv8_append(k, v, i32(starts(ns), cuda), i32(ctx, cuda), pages, i32(table, cuda))
+    host.append(*(x.double().cpu().numpy().reshape(T, kv, hd) for x in (k, v)), ns, ctx, table)
+    host.check(pages)
+
+
 def test_append_leaves_out_what_has_no_page(cuda):
     kv, hd, page = 2, 64, 32
     pages = make_pages(cuda, 6, kv, page, hd)
@@ -375,6 +391,24 @@ def test_attention_scales_far_apart(cuda):
 def test_attention_query_sizes(cuda, qscale):
     """q far below and far above the 16-bit range; at 3e4 one position takes all the weight."""
     run_case(cuda, 2, 4, 64, 64, [1, 4], [150, 90], "f32", 11, qscale=qscale)
+
+
+@pytest.mark.parametrize("hd", [128, 64])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_attention_unaligned_rows(cuda, hd, dtype):
+    """q and out rows that do not begin at a multiple of 16 bytes, decode rows and chunks."""
+    kv, G, page, table_width = 2, 4, 64, 900
+    for ns, ctx in (([1, 1, 1], [500, 64, 3]), ([70, 130], [300, 130])):
+        ns, ctx = np.array(ns), np.array(ctx)
+        pages = make_pages(cuda, 16, kv, page, hd, hd)
+        table = make_table(ctx, page, 16, hd, width=table_width)
+        heads, T = kv * G, int(ns.sum())
+        w = heads * hd
+        q = torch.randn((T, w + 7), device=cuda).to(DT[dtype])[:, 3:3 + w]
+        args = i32(starts(ns), cuda), i32(ctx, cuda), heads, pages, i32(table, cuda)
+        want = ops.kv8_attention(q.contiguous(), *args)
+        out = torch.empty((T, w + 1), dtype=DT[dtype], device=cuda)[:, 1:]
+        assert torch.equal(ops.kv8_attention(q, *args, out=out), want)
 
 
 def test_attention_long_context_splits(cuda):
