@@ -355,10 +355,20 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
               for (int e = 0; e < E; ++e) x[i][e] = p[e];
             }
           } else {
+            const uint16_t* p = (const uint16_t*)a.q + at_q;
+            uint32_t u[E / 2];
+            if (E == 4 && aligned) {
+              const uint2 f = *reinterpret_cast<const uint2*>(p);
+              u[0] = f.x, u[E / 2 - 1] = f.y;
+            } else {
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-              const uint16_t h = ((const uint16_t*)a.q)[at_q + e];
-              x[i][e] = a.dtype == Q8_BF16 ? bf16_bits_to_f32(h) : __half2float(__ushort_as_half(h));
+              for (int e = 0; e < E / 2; ++e) u[e] = p[2 * e] | (uint32_t)p[2 * e + 1] << 16;
+            }
+#pragma unroll
+            for (int e = 0; e < E / 2; ++e) {
+              const float2 f = __half22float2(*reinterpret_cast<__half2*>(&u[e]));
+              x[i][2 * e] = a.dtype == Q8_BF16 ? __uint_as_float(u[e] << 16) : f.x;
+              x[i][2 * e + 1] = a.dtype == Q8_BF16 ? __uint_as_float(u[e] & 0xffff0000u) : f.y;
             }
           }
         }
@@ -510,6 +520,18 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
             for (int i = 0; i < 32; i += 4)
               *reinterpret_cast<float4*>((float*)a.out + o0 + h * 32 + i) =
                   make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+          } else if (!WIDE && wide_out) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+              uint32_t u[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const __nv_bfloat162 b2 = __floats2bfloat162_rn(v[i + 2 * k], v[i + 2 * k + 1]);
+                u[k] = a.dtype == Q8_BF16 ? *reinterpret_cast<const uint32_t*>(&b2)
+                                          : ka_pack(v[i + 2 * k], v[i + 2 * k + 1]);
+              }
+              *reinterpret_cast<uint4*>((uint16_t*)a.out + o0 + h * 32 + i) = make_uint4(u[0], u[1], u[2], u[3]);
+            }
           } else {
 #pragma unroll
             for (int i = 0; i < 32; ++i) ka_store<WIDE>(a, o0 + h * 32 + i, v[i]);
