@@ -96,8 +96,8 @@ __device__ __forceinline__ unsigned kv8_max(unsigned top, unsigned w) {
 // number the touched blocks: sequence b's start at starts[b]/16 + 2b, which
 // leaves room for the n/16 + 2 blocks that n rows can touch.  Bytes: the rows
 // once, a quarter or half of that in codes.  12,562 bf16 rows of 8 kv heads of
-// 128: 21.8 us for 77 MB (3.5 TB/s), bound by the chain from sequence to page to
-// rows and by 20 instructions an element (57 % of the issue slots).
+// 128: 17.4 us for 77 MB (4.4 TB/s), bound by the chain from sequence to page to
+// rows and by some 20 instructions an element.
 //
 // Codes, two at a time in packed f32 operations: m = fma(x, 1/s, 1.5 2^23) rounds to the whole number nearest to the
 // estimated quotient and holds it in its low byte; r = m - 1.5 2^23.  The
@@ -248,7 +248,8 @@ __global__ void __launch_bounds__(128, 10) k_kv8_append(Kv8Rows kr, Kv8Rows vr, 
 }
 
 // One warp per row of the call; rows without a page read as zeros.  12,599 rows
-// of 8 kv heads of 128: 27.6 us for 129 MB, four fifths of it written (4.7 TB/s).
+// of 8 kv heads of 128: 21.3 us for 129 MB (6.1 TB/s, 0.92 of a copy's rate); 27.6
+// without streaming stores, four fifths of the bytes being written.
 template <int HD>
 __global__ void __launch_bounds__(256) k_kv8_read(int rows, const int32_t* __restrict__ starts,
                                                   const int32_t* __restrict__ ctx, int S, q8_kv8_pages kv,

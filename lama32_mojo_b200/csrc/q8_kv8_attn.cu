@@ -700,18 +700,19 @@ static int ka_clusters(int c) {
 }
 
 // How a call is cut up.  Every sequence is taken to have rows / S rows and the
-// table's width of positions.  The three forms cost, fitted to 177 shapes of 1 to
+// table's width of positions.  The three forms cost, fitted to 531 shapes of 1 to
 // 64 sequences, 600 to 20,000 positions, 1 to 24 rows a sequence (us, head size
 // 128; 64 in brackets):
 //   clusters  5 + 3 a wave + 1.25 (0.75) an iteration of a warp; 9 for 5 with 4
 //             n-tiles, whose results take longer to join
 //   many      14 (16 with 4 n-tiles) + 0.94 (0.56) an iteration: even stretches,
 //             a second launch
-//   tcgen05   28 + 1.2 (1.0) a tile of a CTA, a tenth more for f32 rows: pays when
-//             128 rows share a reading
-// The form chosen so was within 1.6 % of the best one on average.  f32 rows, 8 kv
-// heads of 128, 32 heads, us for the three: 8 sequences of 4000 positions, 1 row,
-// 16.0, 21.7, 39.4; 16 of 8000, 39.4, 31.7, 90.1; 16 of 4500, 24 rows, 212, 187, 88.
+//   tcgen05   24 + 1.4 (1.2) a tile of a CTA for f32 rows, 1.0 (0.85) for 16-bit
+//             ones: pays when 128 rows share a reading
+// The form chosen so was within 1 % of the best one on average, 27 % at worst.
+// f32 rows, 32 heads on 8 of 128, us for the three: 8 sequences of 4000 positions,
+// 1 row, 16.0, 21.7, 39.4; 16 of 8000, 39.4, 31.7, 90.1; 16 of 4500, 24 rows, 212,
+// 187, 88.
 struct KaPlan {
   bool tc;     // k_kv8_attn_tc
   int nt, GH, hgroups, QT;
@@ -750,7 +751,7 @@ static KaPlan ka_plan(bool wide, int hd, int64_t rows, int64_t S, int n_heads, i
   const double t_cluster = (p.nt < 4 ? 5 : 9) + waves * (3 + turn * its);
   const double t_many =
       (p.nt < 4 ? 14 : 16) + 0.75 * turn * reg * blocks / (ka_bpi(p.nt) * 4.0 * many_ctas);
-  const double t_tc = 28 + (hd == 128 ? 1.2 : 1.0) * (wide ? 1.1 : 1.0) * tc * ((blocks + KV8_TILE - 1) / KV8_TILE) / tc_ctas;
+  const double t_tc = 24 + (hd == 128 ? 1.0 : 0.85) * (wide ? 1.4 : 1.0) * tc * ((blocks + KV8_TILE - 1) / KV8_TILE) / tc_ctas;
   p.tc = p.nt == 4 && G <= KT_ROWS && t_tc < std::min(t_cluster, t_many);
   if (p.tc || t_many < t_cluster) p.ctas = p.tc ? tc_ctas : many_ctas;
   if (p.tc) rmax = KT_ROWS;

@@ -21,7 +21,7 @@
 // Bound.  2 x 1024 f32 rows of 32 heads on 8 of 128, 8000 positions: 385 us for
 // 258 GFLOP, 516 in f16 products (1.34 PFLOP/s, 0.81 of cuBLAS's bf16 rate).  The
 // tensor pipes are busy 40 % of the time, the issue slots 52 %: the chain from
-// scores to weights is what is waited for.
+// scores to weights is what is waited for.  bf16 rows, one product each: 354 us.
 //
 // Two CTAs an SM (256 TMEM columns each) cover one another's waits.  Their
 // number is fixed; each takes an equal stretch of all units' work and leaves

@@ -83,10 +83,11 @@ __device__ __forceinline__ void vf_send(const double* p, int rank, double v) {
 // with it: w = 2^y (1 + z ln 2).  The 64 keeps the weights that count, from 2^-96
 // to 2^64, among the normal numbers.  Four are added in 32 bits, those sums in 64.
 //
-// 320 rows of 151,936: 91 us for 389 MB (4.3 TB/s, 0.65 of a copy's rate); two CTAs
+// 320 rows of 151,936: 92 us for 389 MB (4.2 TB/s, 0.64 of a copy's rate); two CTAs
 // an SM take turns in loading, waiting for one another and storing.  One row of
-// 128,256: 5.4 us in CTAs of 256 threads, 7.5 in CTAs of 512.  Sending by st.async
-// instead (102 us) and clusters that stay and load a row ahead (107) were slower.
+// 128,256: 5.4 us; CTAs of 256 threads took 6.0 where CTAs of 512 took 8.1.  At 98
+// us, sending by st.async took 102 and clusters that stay and load a row ahead 107;
+// three CTAs an SM of 13 a row took 109, one of 1024 threads 107 at 92.
 template <int THREADS, bool WIDE>  // WIDE: rows to 16 bytes; loads behind a branch each would wait for one another
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
     k_probs(const float* __restrict__ logits, int n, int64_t ld, float temp, float ch, float cl,
@@ -212,8 +213,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
 // A cluster of CTAs per sequence; all of them find the refused row, then each
 // adds up a slice of its weights, in segments of 128 per warp, so that the
 // drawn index is found in one segment: p and q rows are read once.  64 sequences,
-// 151,936 columns: 18.5 us for 78 MB (4.2 TB/s), the loads of a launch and four
-// steps that wait for one another; one sequence 8.0 us.  Segments of 512: 19.2.
+// 151,936 columns: 16.6 us for 78 MB (4.7 TB/s), a launch and four steps that wait
+// for one another; one sequence 7.2 us.  Segments of 512 took 19.2 at 18.5.
 constexpr int VF_SEG = 128;
 
 __global__ void __launch_bounds__(VF_THREADS) k_verify(const float* __restrict__ p, int64_t ldp,
