@@ -503,6 +503,46 @@ def test_attention_repeats_and_streams(cuda):
         assert torch.equal(eager[0], want[0]) and torch.equal(eager[1], want[1])
 
 
+@pytest.mark.parametrize("ns,ctx,width", [([300, 5, 200], [900, 70, 200], 0), ([1] * 40, list(range(1, 1600, 40)), 300),
+                                          ([40] * 20, list(range(40, 1640, 80)), 0)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_attention_forms_repeat_and_overlap(cuda, ns, ctx, width, dtype):
+    """Chunks, many sequences and short chunks: two graphs replayed on two streams at once,
+    next to calls on a third, give the bits of the first calls."""
+    kv, G, hd, page = 4, 4, 128, 16
+    ns, ctx = np.array(ns), np.array(ctx)
+    total = int(sum(-(-c // page) for c in ctx))
+    pages = make_pages(cuda, total, kv, page, hd, 31)
+    table = i32(make_table(ctx, page, total, 31, width=max(width, -(-int(ctx.max()) // page))), cuda)
+    st, cx = i32(starts(ns), cuda), i32(ctx, cuda)
+    T = int(ns.sum())
+    q = [torch.randn((T, kv * G * hd), device=cuda).to(DT[dtype]) for _ in range(3)]
+    want = [ops.kv8_attention(x, st, cx, kv * G, pages, table) for x in q]
+    graphs, outs = [], []
+    for x in q[:2]:
+        o, g = torch.empty_like(x), torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g):
+            ops.kv8_attention(x, st, cx, kv * G, pages, table, out=o)
+        graphs.append(g)
+        outs.append(o)
+    s = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for x, g in zip(s, graphs):
+            with torch.cuda.stream(x):
+                g.replay()
+        with torch.cuda.stream(s[2]):
+            third = [ops.kv8_attention(q[2], st, cx, kv * G, pages, table) for _ in range(2)]
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+        assert torch.equal(third[0], want[2]) and torch.equal(third[1], want[2])
+    ops.device_status()
+
+
 def test_attention_matches_the_f32_cache(cuda):
     """kv8_attention over appended rows against ops.attention over the values read back: the
     same numbers by two paths of the library, both f32 to about 1e-6."""
