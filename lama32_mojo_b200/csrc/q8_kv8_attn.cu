@@ -443,20 +443,29 @@ __device__ __forceinline__ void ka_stretch(const Kv8AttnArgs& a, const KaUnit& u
                       : make_float2(o[i][nt][j], o[i][nt][2 + j]);
     }
   __syncthreads();
-  // join the warps
+  // join the warps: lane w knows warp w's m and l
   constexpr int D = HD / 32;
   for (int r = warp; r < nrow; r += warps) {
-    float mx = -INFINITY, sum = 0.f, x[D];
-    for (int w = 0; w < warps; ++w) mx = fmaxf(mx, pm[w * RMAX + r]);
-    const float ref = mx == -INFINITY ? 0.f : mx;
+    const float mw = lane < warps ? pm[lane * RMAX + r] : -INFINITY, lw = lane < warps ? pl[lane * RMAX + r] : 0.f;
+    const float mx = warp_max(mw), f = exp2f(mw - (mx == -INFINITY ? 0.f : mx));
+    const float sum = warp_sum(f * lw);
+    float x[D];
 #pragma unroll
     for (int e = 0; e < D; ++e) x[e] = 0.f;
-    for (int w = 0; w < warps; ++w) {
-      const float f = exp2f(pm[w * RMAX + r] - ref);
-      const float* p = part + (w * RMAX + r) * HD + lane * D;
-      sum += f * pl[w * RMAX + r];
+    const float* p = part + r * HD + lane * D;
+#pragma unroll 4
+    for (int w = 0; w < warps; ++w, p += RMAX * HD) {
+      const float fw = __shfl_sync(0xffffffffu, f, w);
+      float y[D];
+      if constexpr (D == 4) {
+        const float4 v = *reinterpret_cast<const float4*>(p);
+        y[0] = v.x, y[1] = v.y, y[D - 2] = v.z, y[D - 1] = v.w;
+      } else {
+        const float2 v = *reinterpret_cast<const float2*>(p);
+        y[0] = v.x, y[1] = v.y;
+      }
 #pragma unroll
-      for (int e = 0; e < D; ++e) x[e] += f * p[e];
+      for (int e = 0; e < D; ++e) x[e] += fw * y[e];
     }
     sink(r, x, mx, sum);
   }
