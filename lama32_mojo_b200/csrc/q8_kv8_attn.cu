@@ -184,6 +184,17 @@ __device__ __forceinline__ void ka_stretch(const Kv8AttnArgs& a, const KaUnit& u
     ka_load(vr[j][2], p + 8 * HD);
     ka_load(vr[j][3], p + 9 * HD);
   };
+  // q: a lane's dims of its K quarter, of the rows of one n-tile (every warp's own
+  // copy where there is one n-tile).  Loaded before anything waits for the table.
+  const int mine = NT == 1 ? 0 : warp;
+  const int qr = mine * RPT + (WIDE ? g >> 1 : g);
+  const bool aligned = (((uintptr_t)a.q | (uintptr_t)(a.ldq * (WIDE ? 4 : 2))) & 15) == 0;
+  float x[HD / 4];
+#pragma unroll
+  for (int i = 0; i < HD / 4; ++i) x[i] = 0.f;
+  if (mine < NT && qr < nrow && qr % a.GH < un.heads)
+    ka_row<WIDE>(x, a.q, (int64_t)(un.row0 + qr / a.GH) * a.ldq + (un.head0 + qr % a.GH) * HD + t * (HD / 4), a.dtype,
+                 aligned);
   int id[BPI];
   look_up(0);
 #pragma unroll
@@ -193,20 +204,10 @@ __device__ __forceinline__ void ka_stretch(const Kv8AttnArgs& a, const KaUnit& u
     load_v(j, id[j]);
   }
 
-  // q: a lane holds its B column's words for the dims of its K quarter
+  // its B column's words
   uint2 qf[NT == 1 ? KW : 1];
-  const bool aligned = (((uintptr_t)a.q | (uintptr_t)(a.ldq * (WIDE ? 4 : 2))) & 15) == 0;
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    if (NT > 1 && nt % warps != warp) continue;
-    const int r = nt * RPT + (WIDE ? g >> 1 : g);
-    float x[HD / 4];
+  if (mine < NT) {
     float top = 0.f;
-#pragma unroll
-    for (int i = 0; i < HD / 4; ++i) x[i] = 0.f;
-    if (r < nrow && r % a.GH < un.heads)
-      ka_row<WIDE>(x, a.q, (int64_t)(un.row0 + r / a.GH) * a.ldq + (un.head0 + r % a.GH) * HD + t * (HD / 4), a.dtype,
-                   aligned);
     bool odd = false;  // NaN or infinite
 #pragma unroll
     for (int i = 0; i < HD / 4; ++i) {
@@ -233,7 +234,7 @@ __device__ __forceinline__ void ka_stretch(const Kv8AttnArgs& a, const KaUnit& u
           w1 |= ((uint32_t)((g & 1) ? 0 : d2) & 255u) << (8 * j);
         }
         if (NT == 1) qf[i] = make_uint2(w0, w1);
-        else qs[(nt * KW + i) * 32 + lane] = make_uint2(w0, w1);
+        else qs[(mine * KW + i) * 32 + lane] = make_uint2(w0, w1);
       }
       if (odd) fac = __int_as_float(0x7fc00000);  // NaN scores
     } else {
@@ -245,10 +246,10 @@ __device__ __forceinline__ void ka_stretch(const Kv8AttnArgs& a, const KaUnit& u
         const uint2 w = make_uint2(ka_pack(x[4 * i] * up, x[4 * i + 1] * up),
                                    ka_pack(x[4 * i + 2] * up, x[4 * i + 3] * up));
         if (NT == 1) qf[i] = w;
-        else qs[(nt * KW + i) * 32 + lane] = w;
+        else qs[(mine * KW + i) * 32 + lane] = w;
       }
     }
-    if (t == 0 && (!WIDE || (g & 1) == 0)) s_fac[r] = fac;
+    if (t == 0 && (!WIDE || (g & 1) == 0)) s_fac[qr] = fac;
   }
   __syncthreads();
   float fac[NT][RT], m[NT][RT], l[NT][RT], o[OT][NT][4];
@@ -476,17 +477,28 @@ template <bool WIDE, int HD>
 __device__ __forceinline__ void ka_out(const Kv8AttnArgs& a, int row0, int head0, int heads, int r,
                                        const float (&x)[HD / 32], float sum) {
   constexpr int D = HD / 32;
-  if (r % a.GH >= heads) return;
-  const int64_t i = (int64_t)(row0 + r / a.GH) * a.ldo + (head0 + r % a.GH) * HD + (threadIdx.x & 31) * D;
+  const int tok = r / a.GH, h = r - tok * a.GH;
+  if (h >= heads) return;
+  const int64_t i = (int64_t)(row0 + tok) * a.ldo + (head0 + h) * HD + (threadIdx.x & 31) * D;
+  const float inv = 1.f / (KA_LIFT * sum);
   float y[D];
 #pragma unroll
-  for (int e = 0; e < D; ++e)
-    y[e] = sum > 0.f ? x[e] * (1.f / KA_LIFT) / sum : 0.f * (x[e] + sum);  // no position: 0; NaN stays
-  if (WIDE && D == 4 && (((uintptr_t)a.out | (uintptr_t)(a.ldo * 4)) & 15) == 0) {
-    *reinterpret_cast<float4*>((float*)a.out + i) = make_float4(y[0], y[1], y[D - 2], y[D - 1]);
-  } else {
+  for (int e = 0; e < D; ++e) y[e] = sum > 0.f ? x[e] * inv : 0.f * (x[e] + sum);  // no position: 0; NaN stays
+  const bool aligned = (((uintptr_t)a.out | (uintptr_t)(a.ldo * (WIDE ? 4 : 2))) & (D * (WIDE ? 4 : 2) - 1)) == 0;
+  if (!aligned) {
 #pragma unroll
     for (int e = 0; e < D; ++e) ka_store<WIDE>(a, i + e, y[e]);
+  } else if constexpr (WIDE) {
+    float* to = (float*)a.out + i;
+    if constexpr (D == 4) *reinterpret_cast<float4*>(to) = make_float4(y[0], y[1], y[2], y[3]);
+    else *reinterpret_cast<float2*>(to) = make_float2(y[0], y[1]);
+  } else {
+    uint32_t u[D / 2];
+#pragma unroll
+    for (int k = 0; k < D / 2; ++k) u[k] = ka_pack16(a.dtype, y[2 * k], y[2 * k + 1]);
+    uint16_t* to = (uint16_t*)a.out + i;
+    if constexpr (D == 4) *reinterpret_cast<uint2*>(to) = make_uint2(u[0], u[1]);
+    else *reinterpret_cast<uint32_t*>(to) = u[0];
   }
 }
 

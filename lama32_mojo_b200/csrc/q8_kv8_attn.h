@@ -41,6 +41,12 @@ __device__ __forceinline__ uint32_t ka_pack(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// two floats as two bf16 or f16
+__device__ __forceinline__ uint32_t ka_pack16(int dtype, float lo, float hi) {
+  const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+  return dtype == Q8_BF16 ? *reinterpret_cast<const uint32_t*>(&b) : ka_pack(lo, hi);
+}
+
 __device__ __forceinline__ float ka_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

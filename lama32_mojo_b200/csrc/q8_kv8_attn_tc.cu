@@ -525,11 +525,7 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
             for (int i = 0; i < 32; i += 8) {
               uint32_t u[4];
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const __nv_bfloat162 b2 = __floats2bfloat162_rn(v[i + 2 * k], v[i + 2 * k + 1]);
-                u[k] = a.dtype == Q8_BF16 ? *reinterpret_cast<const uint32_t*>(&b2)
-                                          : ka_pack(v[i + 2 * k], v[i + 2 * k + 1]);
-              }
+              for (int k = 0; k < 4; ++k) u[k] = ka_pack16(a.dtype, v[i + 2 * k], v[i + 2 * k + 1]);
               *reinterpret_cast<uint4*>((uint16_t*)a.out + o0 + h * 32 + i) = make_uint4(u[0], u[1], u[2], u[3]);
             }
           } else {
