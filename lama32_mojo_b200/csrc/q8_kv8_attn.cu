@@ -47,6 +47,7 @@
 #include "q8_kv8_attn.h"
 
 #include <algorithm>
+#include <type_traits>
 #include <cooperative_groups.h>
 
 namespace cg = cooperative_groups;
@@ -117,21 +118,23 @@ struct KaShape {
   static constexpr int RT = WIDE ? 1 : 2;       // rows per n-tile whose scores a lane holds
   static constexpr int BPI = ka_bpi(NT);        // blocks per iteration
   static constexpr int WARPS = ka_warps(NT);     // that an SM holds
-  static constexpr int QSMEM = NT == 1 ? 0 : NT * (HD / 16) * 32 * 8;
+  static constexpr int QSMEM = NT * (HD / 16) * 32 * 8;
   static constexpr int REC = RMAX * (HD + 2);   // floats of a partial result: o, m, l
   static constexpr int smem(int warps) { return warps * REC * 4 + QSMEM + 3 * RMAX * 4; }
 };
 
 // Blocks [lo, hi) of a unit by the whole CTA.  At the end a warp takes a row r at
 // a time: sink(r, x, m, l), x the lane's HD / 32 dims of the sum lifted by KA_LIFT.
-template <bool WIDE, int HD, int NT, typename Sink>
+template <bool WIDE, int HD, int NT, int warps, typename Sink>
 __device__ __forceinline__ void ka_stretch(const Kv8AttnArgs& a, const KaUnit& un, int lo, int hi, uint8_t* smem,
                                            Sink sink) {
   using Sh = KaShape<WIDE, HD, NT>;
   constexpr int RPT = Sh::RPT, RMAX = Sh::RMAX, RT = Sh::RT, BPI = Sh::BPI;
   constexpr int KW = HD / 16, VW = HD / 32, OT = HD / 16;  // words of a K quarter row, of a V eighth; output tiles
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, g = lane >> 2, t = lane & 3;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int h = un.h, nrow = un.toks * a.GH;  // row r: token r / GH, head r % GH
+  const unsigned per_gh = (65535u + a.GH) / a.GH;
+  auto tok_of = [&](int r) { return (int)(r * per_gh >> 16); };  // exact: both are at most 128
   const int64_t room = (int64_t)a.max_pages * a.kv.page;
   const int32_t* trow = a.table + (int64_t)un.b * a.max_pages;
   const int ppb = a.kv.page / KV8_BLOCK;
@@ -184,17 +187,24 @@ __device__ __forceinline__ void ka_stretch(const Kv8AttnArgs& a, const KaUnit& u
     ka_load(vr[j][2], p + 8 * HD);
     ka_load(vr[j][3], p + 9 * HD);
   };
-  // q: a lane's dims of its K quarter, of the rows of one n-tile (every warp's own
-  // copy where there is one n-tile).  Loaded before anything waits for the table.
-  const int mine = NT == 1 ? 0 : warp;
-  const int qr = mine * RPT + (WIDE ? g >> 1 : g);
-  const bool aligned = (((uintptr_t)a.q | (uintptr_t)(a.ldq * (WIDE ? 4 : 2))) & 15) == 0;
-  float x[HD / 4];
+  // q: four dims a lane, a warp 128 / HD rows at a time.  Loaded before anything
+  // waits for the table.
+  constexpr int LPR = HD / 4, RPP = 32 / LPR, RPW = (RMAX + warps * RPP - 1) / (warps * RPP);
+  float x[RPW][4];
+  auto load_q = [&](auto by16) {
 #pragma unroll
-  for (int i = 0; i < HD / 4; ++i) x[i] = 0.f;
-  if (mine < NT && qr < nrow && qr % a.GH < un.heads)
-    ka_row<WIDE>(x, a.q, (int64_t)(un.row0 + qr / a.GH) * a.ldq + (un.head0 + qr % a.GH) * HD + t * (HD / 4), a.dtype,
-                 aligned);
+    for (int k = 0; k < RPW; ++k) {
+      const int r = (k * warps + warp) * RPP + lane / LPR;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[k][i] = 0.f;
+      const int tok = tok_of(r), head = r - tok * a.GH;
+      if (r < nrow && head < un.heads)
+        ka_four<WIDE, decltype(by16)::value>(
+            x[k], a.q, (int64_t)(un.row0 + tok) * a.ldq + (un.head0 + head) * HD + lane % LPR * 4, a.dtype);
+    }
+  };
+  if ((((uintptr_t)a.q | (uintptr_t)(a.ldq * (WIDE ? 4 : 2))) & 15) == 0) load_q(std::true_type());
+  else load_q(std::false_type());
   int id[BPI];
   look_up(0);
 #pragma unroll
@@ -204,54 +214,53 @@ __device__ __forceinline__ void ka_stretch(const Kv8AttnArgs& a, const KaUnit& u
     load_v(j, id[j]);
   }
 
-  // its B column's words
-  uint2 qf[NT == 1 ? KW : 1];
-  if (mine < NT) {
-    float top = 0.f;
-    bool odd = false;  // NaN or infinite
+  // the B columns' words, by lane: of lane (g, t) and word i, column g's codes of
+  // the dims t HD / 4 + 4 i .. + 3
 #pragma unroll
-    for (int i = 0; i < HD / 4; ++i) {
-      top = fmaxf(top, fabsf(x[i]));
-      odd |= !(fabsf(x[i]) < INFINITY);
-    }
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    odd = __ballot_sync(0xffffffffu, odd) >> (lane & ~3) & 15u;
+  for (int k = 0; k < RPW; ++k) {
+    const int r = (k * warps + warp) * RPP + lane / LPR, w = lane % LPR;
+    unsigned bits = 0u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bits = max(bits, __float_as_uint(x[k][i]) & 0x7fffffffu);
+#pragma unroll
+    for (int d = LPR / 2; d > 0; d >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, d));
+    if (r >= RMAX) continue;
+    const bool odd = bits >= 0x7f800000u;  // NaN or infinite
+    uint2* to = qs + (r / RPT * KW + w % KW) * 32 + w / KW;
     float fac = 1.4426950408889634f / sqrtf((float)HD);
     if constexpr (WIDE) {
+      const float top = __uint_as_float(bits);
       const float pre = top < 0x1p-60f ? 0x1p90f : 1.f;  // 127 65536 / top would overflow for a subnormal top
       const float up = top > 0.f ? 8323072.f / (top * pre) : 0.f;
       fac *= top / 8323072.f;
+      uint32_t d0 = 0u, d1 = 0u, d2 = 0u;  // digits
 #pragma unroll
-      for (int i = 0; i < KW; ++i) {
-        uint32_t w0 = 0u, w1 = 0u;  // digit 0 or 1, and digit 2
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int X = odd ? 0 : __float2int_rn(x[4 * i + j] * pre * up);
-          const int d2 = (int)(int8_t)X, X1 = (X - d2) >> 8;
-          const int d1 = (int)(int8_t)X1, d0 = (X1 - d1) >> 8;
-          w0 |= ((uint32_t)((g & 1) ? d1 : d0) & 255u) << (8 * j);
-          w1 |= ((uint32_t)((g & 1) ? 0 : d2) & 255u) << (8 * j);
-        }
-        if (NT == 1) qf[i] = make_uint2(w0, w1);
-        else qs[(mine * KW + i) * 32 + lane] = make_uint2(w0, w1);
+      for (int j = 0; j < 4; ++j) {
+        const int X = odd ? 0 : __float2int_rn(x[k][j] * pre * up);
+        const int c2 = (int)(int8_t)X, X1 = (X - c2) >> 8;
+        const int c1 = (int)(int8_t)X1, c0 = (X1 - c1) >> 8;
+        d0 |= ((uint32_t)c0 & 255u) << (8 * j);
+        d1 |= ((uint32_t)c1 & 255u) << (8 * j);
+        d2 |= ((uint32_t)c2 & 255u) << (8 * j);
       }
+      to[r % RPT * 8] = make_uint2(d0, d2);  // columns 2 r and 2 r + 1
+      to[r % RPT * 8 + 4] = make_uint2(d1, 0u);
       if (odd) fac = __int_as_float(0x7fc00000);  // NaN scores
     } else {
-      const int k = top > 0.f && top < INFINITY ? min(14 - ilogbf(top), 126) : 0;
-      const float up = scalbnf(1.f, k);
-      fac = scalbnf(fac, -k);
-#pragma unroll
-      for (int i = 0; i < KW; ++i) {
-        const uint2 w = make_uint2(ka_pack(x[4 * i] * up, x[4 * i + 1] * up),
-                                   ka_pack(x[4 * i + 2] * up, x[4 * i + 3] * up));
-        if (NT == 1) qf[i] = w;
-        else qs[(mine * KW + i) * 32 + lane] = w;
-      }
+      // the largest element into [2^14, 2^15)
+      const int sh = bits == 0u || odd ? 0 : min(141 - (int)(bits >> 23), 126);
+      const float up = __uint_as_float((unsigned)(127 + sh) << 23);
+      fac *= __uint_as_float((unsigned)(127 - sh) << 23);
+      to[r % RPT * 4] = make_uint2(ka_pack(x[k][0] * up, x[k][1] * up), ka_pack(x[k][2] * up, x[k][3] * up));
     }
-    if (t == 0 && (!WIDE || (g & 1) == 0)) s_fac[qr] = fac;
+    if (w == 0) s_fac[r] = fac;
   }
   __syncthreads();
+  uint2 qf[NT == 1 ? KW : 1];
+  if (NT == 1) {
+#pragma unroll
+    for (int i = 0; i < KW; ++i) qf[i] = qs[i * 32 + lane];
+  }
   float fac[NT][RT], m[NT][RT], l[NT][RT], o[OT][NT][4];
   int lim[NT][RT];  // positions that the lane's rows see
 #pragma unroll
@@ -260,7 +269,7 @@ __device__ __forceinline__ void ka_stretch(const Kv8AttnArgs& a, const KaUnit& u
     for (int j = 0; j < RT; ++j) {
       const int r = nt * RPT + t * RT + j;
       fac[nt][j] = s_fac[r];
-      lim[nt][j] = r < nrow ? (int)min(max(un.pos0 + r / a.GH + 1, (int64_t)0), room) : 0;
+      lim[nt][j] = r < nrow ? (int)min(max(un.pos0 + tok_of(r) + 1, (int64_t)0), room) : 0;
       m[nt][j] = -INFINITY;
       l[nt][j] = 0.f;
     }
@@ -523,7 +532,7 @@ __global__ void __launch_bounds__(KaShape<WIDE, HD, NT>::WARPS * 32, 1) k_kv8_at
   const int per = ((u.nblk + nsplit - 1) / nsplit + Sh::BPI - 1) / Sh::BPI * Sh::BPI;
   const int lo = min(u.nblk, split * per), hi = min(u.nblk, lo + per);
   if (nsplit == 1) {
-    ka_stretch<WIDE, HD, NT>(a, u, lo, hi, smem, [&](int r, const float (&x)[HD / 32], float, float l) {
+    ka_stretch<WIDE, HD, NT, Sh::WARPS>(a, u, lo, hi, smem, [&](int r, const float (&x)[HD / 32], float, float l) {
       ka_out<WIDE, HD>(a, u.row0, u.head0, u.heads, r, x, l);
     });
     return;
@@ -532,7 +541,7 @@ __global__ void __launch_bounds__(KaShape<WIDE, HD, NT>::WARPS * 32, 1) k_kv8_at
   float* part = reinterpret_cast<float*>(smem);
   float *s_m = reinterpret_cast<float*>(smem + (blockDim.x >> 5) * Sh::REC * 4 + Sh::QSMEM) + RMAX, *s_l = s_m + RMAX;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  ka_stretch<WIDE, HD, NT>(a, u, lo, hi, smem, [&](int r, const float (&x)[HD / 32], float m, float l) {
+  ka_stretch<WIDE, HD, NT, Sh::WARPS>(a, u, lo, hi, smem, [&](int r, const float (&x)[HD / 32], float m, float l) {
 #pragma unroll
     for (int e = 0; e < HD / 32; ++e) part[r * HD + lane * (HD / 32) + e] = x[e];
     if (lane == 0) {
@@ -623,7 +632,7 @@ __global__ void __launch_bounds__(128, KaShape<WIDE, HD, NT>::WARPS / 4) k_kv8_a
       const bool whole = begins && ends;
       const int rec = 2 * c + (begins ? 1 : 0), lane = threadIdx.x & 31;
       float* to = a.work + (int64_t)rec * Sh::REC;
-      ka_stretch<WIDE, HD, NT>(a, u, lo, hi, smem, [&](int r, const float (&x)[HD / 32], float m, float l) {
+      ka_stretch<WIDE, HD, NT, 4>(a, u, lo, hi, smem, [&](int r, const float (&x)[HD / 32], float m, float l) {
         if (whole) {
           ka_out<WIDE, HD>(a, u.row0, u.head0, u.heads, r, x, l);
           return;

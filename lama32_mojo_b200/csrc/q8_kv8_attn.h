@@ -53,36 +53,30 @@ __device__ __forceinline__ float ka_exp2(float x) {
   return y;
 }
 
-// N consecutive elements from element i0 on as floats
-template <bool WIDE, int N>
-__device__ __forceinline__ void ka_row(float (&v)[N], const void* base, int64_t i0, int dtype, bool aligned) {
+// four consecutive elements from element i0 on as floats
+template <bool WIDE, bool ALIGNED>
+__device__ __forceinline__ void ka_four(float (&v)[4], const void* base, int64_t i0, int dtype) {
   if constexpr (WIDE) {
     const float* p = (const float*)base + i0;
-    if (aligned) {
-#pragma unroll
-      for (int i = 0; i < N / 4; ++i) {
-        const float4 u = reinterpret_cast<const float4*>(p)[i];
-        v[4 * i] = u.x, v[4 * i + 1] = u.y, v[4 * i + 2] = u.z, v[4 * i + 3] = u.w;
-      }
+    if constexpr (ALIGNED) {
+      const float4 u = *reinterpret_cast<const float4*>(p);
+      v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
     } else {
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = p[i];
+      for (int i = 0; i < 4; ++i) v[i] = p[i];
     }
   } else {
     const uint16_t* p = (const uint16_t*)base + i0;
-    uint32_t w[N / 2];
-    if (aligned) {
-#pragma unroll
-      for (int i = 0; i < N / 8; ++i) {
-        const uint4 u = reinterpret_cast<const uint4*>(p)[i];
-        w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
-      }
+    uint32_t w[2];
+    if constexpr (ALIGNED) {
+      const uint2 u = *reinterpret_cast<const uint2*>(p);
+      w[0] = u.x, w[1] = u.y;
     } else {
 #pragma unroll
-      for (int i = 0; i < N / 2; ++i) w[i] = p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
+      for (int i = 0; i < 2; ++i) w[i] = p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
     }
 #pragma unroll
-    for (int i = 0; i < N / 2; ++i) {
+    for (int i = 0; i < 2; ++i) {
       const float2 f = __half22float2(*reinterpret_cast<__half2*>(&w[i]));
       v[2 * i] = dtype == Q8_BF16 ? __uint_as_float(w[i] << 16) : f.x;
       v[2 * i + 1] = dtype == Q8_BF16 ? __uint_as_float(w[i] & 0xffff0000u) : f.y;
