@@ -40,10 +40,11 @@
 // same bits every time.
 //
 // Bound.  64 f32 rows, one each for sequences up to 8192 positions, 32 heads on 8
-// of 128: 97.6 us for 557 MB, 5.7 TB/s or 0.87 of a copy's rate; 39 % of the issue
+// of 128: 94 us for 557 MB, 5.9 TB/s or 0.90 of a copy's rate; 39 % of the issue
 // slots, so the cache's rows are what it waits for.  80 bf16 rows of 16 sequences,
-// 24 heads: 32 us for 76 MB: launch, search and join take half.  One row and 523
-// positions, heads of 64: 6.7 us, a launch and a chain of dependent loads.
+// 24 heads: 33 us for 76 MB: launch, search and join take half.  One row and 523
+// positions, heads of 64: 5.9 us, a launch and a chain of dependent loads (6.8
+// before the warps shared the work on the query rows: 3000 of 8500 clocks).
 #include "q8_kv8_attn.h"
 
 #include <algorithm>
