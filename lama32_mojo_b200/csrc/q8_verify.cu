@@ -27,22 +27,10 @@ constexpr int VF_MAX_CLUSTER = 16;
 constexpr int VF_Q = 10;                           // four-logit pieces that a thread of k_probs holds
 constexpr int vf_slice(int threads) { return threads * 4 * VF_Q; }  // logits of a row per CTA of k_probs, at most
 
-__device__ __forceinline__ void vf_best(float& bv, int& bi, float ov, int oi) {
-  if (ov > bv || (ov == bv && oi < bi)) {
-    bv = ov;
-    bi = oi;
-  }
-}
-
 __device__ __forceinline__ uint32_t vf_map(const void* p, int rank) {
   uint32_t a;
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
   return a;
-}
-__device__ __forceinline__ float vf_peer(const float* p, int rank) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(vf_map(p, rank)) : "memory");
-  return v;
 }
 __device__ __forceinline__ int vf_peer(const int* p, int rank) {
   int v;
@@ -90,8 +78,8 @@ __device__ __forceinline__ void vf_send(const double* p, int rank, double v) {
 // three CTAs an SM of 13 a row took 109, one of 1024 threads 107 at 92.
 template <int THREADS, bool WIDE>  // WIDE: rows to 16 bytes; loads behind a branch each would wait for one another
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
-    k_probs(const float* __restrict__ logits, int n, int64_t ld, float temp, float ch, float cl,
-            float* __restrict__ out, int64_t ldo, int per) {
+    k_probs(const float* logits, int n, int64_t ld, float temp, float ch, float cl, float* out, int64_t ldo,
+            int per) {  // out may be logits
   constexpr int WARPS = THREADS / 32;
   __shared__ float s_v[VF_MAX_CLUSTER * WARPS];
   __shared__ int s_i[VF_MAX_CLUSTER * WARPS];
