@@ -339,6 +339,40 @@ def test_attention_several_tokens(cuda, kv, G, hd, page, dtype):
     run_case(cuda, kv, G, hd, page, [5, 0, 1, 17, 40, 2, 9], [200, 30, 1, 17, 131, 65, 70], dtype, seed=G, strided=True)
 
 
+@pytest.mark.parametrize("hd", [128, 64])
+@pytest.mark.parametrize("gone", [0, 12])
+def test_attention_long_chunks_in_one_stretch(cuda, hd, gone):
+    """330 times the same chunk, so that a CTA takes all of one: sums over many tiles, with scores
+    that grow along the context and, where pages are gone, none for the first tiles."""
+    kv, G, page, n, ctx, S = 1, 4, 64, 32, 2000, 330
+    pages = make_pages(cuda, 32, kv, page, hd, 5)
+    pages.k_scale.mul_(torch.linspace(0.2, 3.0, 32, device=cuda)[:, None, None])
+    row = np.arange(32, dtype=np.int32)
+    row[:gone] = -1
+    q = torch.randn((n, kv * G * hd), device=cuda, generator=torch.Generator(device=cuda).manual_seed(5))
+    got = ops.kv8_attention(q.repeat(S, 1), i32(starts([n] * S), cuda), i32([ctx] * S, cuda), kv * G, pages,
+                            i32(np.tile(row, (S, 1)), cuda)).view(S, n, G, hd)
+    host = HostCache(pages)
+    reference.tol16 = np.zeros((n, G, hd))
+    ref, tol = reference(host, q.double().cpu().numpy().reshape(n, G, hd), [n], [ctx], row[None], G)
+    tol = torch.from_numpy(tol + 2.0 ** -24 * np.abs(ref) + 1e-37).to(cuda)
+    err = (got.double() - torch.from_numpy(ref).to(cuda)).abs()
+    assert bool((err <= tol).all()), float((err / tol).max())
+    # and as a whole within twice an f32 sum's rounding of 2000 terms at random, 2000 ** 0.5 * 2 ** -24
+    assert float(err.norm() / (S ** 0.5 * np.linalg.norm(ref))) < 2 * 2000 ** 0.5 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("G,hd", [(3, 128), (5, 64), (7, 128), (71, 64), (128, 64), (130, 128)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("width", [0, 2500])
+def test_attention_chunks_of_odd_groups(cuda, G, hd, dtype, width):
+    """Head groups that do not fill a tile's rows, or need several tiles, in chunks; the table's
+    width decides how the call is cut up."""
+    ns, ctx, page = [33, 0, 50], [120, 7, 50], 16
+    pages = make_pages(cuda, 20, 1, page, hd, G)
+    run_case(cuda, 1, G, hd, page, ns, ctx, dtype, G, make_table(ctx, page, 20, G, width=max(8, width)), pages=pages)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "f16"])
 def test_attention_chunks(cuda, dtype):
     run_case(cuda, 2, 4, 128, 64, [130, 67], [515, 67], dtype, seed=3)
