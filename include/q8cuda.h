@@ -264,7 +264,7 @@ int q8op_kv8_read(const q8_kv8_pages* kv, const int32_t* seq_start, const int32_
  * row attends to the positions 0 .. its own of its sequence; positions whose
  * page is not there are masked (pages freed behind a window, say), and a row
  * that sees no position gives zeros.  Scores, softmax statistics and sums are
- * f32.  work: device scratch of q8op_kv8_attention_workspace() bytes, 16-byte
+ * f32, the weights have 22 bits in the products, whatever dtype is.  work: device scratch of q8op_kv8_attention_workspace() bytes, 16-byte
  * aligned (NULL where that is 0), positions being max_pages * page; calls that
  * overlap need a scratch each.  The device is the current one for both. */
 size_t q8op_kv8_attention_workspace(int dtype, int64_t rows, int64_t S, int n_heads, int n_kv, int head_dim,

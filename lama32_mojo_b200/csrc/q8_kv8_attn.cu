@@ -13,9 +13,10 @@
 // f32 rows: q becomes three signed 8-bit digits, q = s (65536 a + 256 b + c)
 // with s = max|q| / (127 65536) (23 bits of the row's largest element), one
 // column each, and the scores are exact integer products (m16n8k32) of the
-// codes as they are; P is split into two f16 halves (22 bits).  bf16 / f16 rows:
-// q scaled by a power of two to the top of the f16 range, one column, the codes
-// as f16 (exact); P is one f16.
+// codes as they are; the two f16 halves of P (22 bits) are two more columns.
+// bf16 / f16 rows: q scaled by a power of two to the top of the f16 range, one
+// column, the codes as f16 (exact); the halves of P are two products.  One f16
+// alone would move an f16 result by as much again as its own rounding.
 // The order of a dot product's terms is free, so lane (g, t) = (lane / 4,
 // lane % 4) reads its operand bytes straight from the cache rows: of K a
 // quarter of rows g and g + 8, of V the g-th eighth of rows 2t, 2t + 1, 2t + 8,
@@ -42,7 +43,7 @@
 // Bound.  64 f32 rows, one each for sequences up to 8192 positions, 32 heads on 8
 // of 128: 94 us for 557 MB, 5.9 TB/s or 0.90 of a copy's rate; 39 % of the issue
 // slots, so the cache's rows are what it waits for.  80 bf16 rows of 16 sequences,
-// 24 heads: 33 us for 76 MB: launch, search and join take half.  One row and 523
+// 24 heads: 37 us for 76 MB: launch, search and join take half (33 with one f16 a weight).  One row and 523
 // positions, heads of 64: 5.9 us, a launch and a chain of dependent loads (6.8
 // before the warps shared the work on the query rows: 3000 of 8500 clocks).
 #include "q8_kv8_attn.h"
@@ -352,7 +353,7 @@ __device__ __forceinline__ void ka_stretch(const Kv8AttnArgs& a, const KaUnit& u
     const int p0 = (lo + (warp + it * warps) * BPI) * KV8_BLOCK + g;
 #pragma unroll
     for (int j = 0; j < BPI; ++j) lsv[j] = fmaxf(__log2f(sv[j]), -100.f);
-    uint32_t pb[BPI][NT][2];
+    uint32_t pb[BPI][NT][2], pr[BPI][WIDE ? 1 : NT][2];  // pr: what the f16 of pb leave of the weights
     bool moved = false;
     float alpha[NT][RT];
 #pragma unroll
@@ -399,7 +400,10 @@ __device__ __forceinline__ void ka_stretch(const Kv8AttnArgs& a, const KaUnit& u
             const float ph = __half2float(__float2half_rn(p));
             x = ka_pack(ph, p - ph);
           } else {
-            x = ka_pack(p, s[j][nt][RT - 1][e] * w);
+            const float p1 = s[j][nt][RT - 1][e] * w;
+            x = ka_pack(p, p1);
+            const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&x));
+            pr[j][WIDE ? 0 : nt][e] = ka_transpose(ka_pack(p - h.x, p1 - h.y));
           }
           pb[j][nt][e] = ka_transpose(x);
         }
@@ -428,6 +432,10 @@ __device__ __forceinline__ void ka_stretch(const Kv8AttnArgs& a, const KaUnit& u
         for (int nt = 0; nt < NT; ++nt) {
           ka_mma(o[2 * w][nt], fa, pb[j][nt][0], pb[j][nt][1]);
           ka_mma(o[2 * w + 1][nt], fb, pb[j][nt][0], pb[j][nt][1]);
+          if constexpr (!WIDE) {
+            ka_mma(o[2 * w][nt], fa, pr[j][nt][0], pr[j][nt][1]);
+            ka_mma(o[2 * w + 1][nt], fb, pr[j][nt][0], pr[j][nt][1]);
+          }
         }
       }
       load_v(j, id[j]);  // of the next iteration
@@ -789,7 +797,7 @@ static KaPlan ka_plan(bool wide, int hd, int64_t rows, int64_t S, int n_heads, i
   cut(rmax);
   p.slots = p.QT > 1 ? rows / p.QT + S : rows;  // room for the groups, about half of it used where QT > 1
   if (p.ctas) {
-    p.meta = (size_t)p.ctas * (p.tc && wide ? 3 : 2) * rmax * (hd + 2) * 4;  // tc: and a place for flushed sums
+    p.meta = (size_t)p.ctas * (p.tc ? 3 : 2) * rmax * (hd + 2) * 4;  // tc: and a place for flushed sums
     p.bytes = p.meta + (size_t)p.ctas * 2 * sizeof(int4);
   }
   return p;

@@ -13,15 +13,15 @@
 //   warps 0-3  a thread per row: reads its 64 scores from TMEM, keeps M and l,
 //              writes P over them.  S / P have two buffers, so the next tile's
 //              scores are computed meanwhile.
-// f32 rows: q = qh + ql and p = ph + pl, two products each (22 bits; the codes
-// need one f16): 4 x 128 x 64 x hd multiply-adds a tile.  bf16 / f16 rows: one.
+// p = ph + pl, two products (22 bits; the codes need one f16); f32 rows: q = qh + ql
+// too.  4 x 128 x 64 x hd multiply-adds a tile, bf16 / f16 rows 3.
 // M moves only when it has grown by more than 1, so that O in TMEM is scaled
 // seldom; weights stay below 2, lifted by 2^14.
 //
 // Bound.  2 x 1024 f32 rows of 32 heads on 8 of 128, 8000 positions: 385 us for
 // 258 GFLOP, 516 in f16 products (1.34 PFLOP/s, 0.81 of cuBLAS's bf16 rate).  The
 // tensor pipes are busy 40 % of the time, the issue slots 52 %: the chain from
-// scores to weights is what is waited for.  bf16 rows, one product each: 354 us.
+// scores to weights is what is waited for.  bf16 rows: 391 us (356 with one f16 a weight).
 //
 // Two CTAs an SM (256 TMEM columns each) cover one another's waits.  Their
 // number is fixed; each takes an equal stretch of all units' work and leaves
@@ -135,7 +135,7 @@ __device__ __forceinline__ float kt_top(uint32_t addr, const float4* sc, float f
 }
 
 // Scores -> weights, in place; returns their sum before sv.
-template <bool WIDE, bool MASKED>
+template <bool MASKED>
 __device__ __forceinline__ float kt_weights(uint32_t addr, const float4* sc, float fac, float ref, int left) {
   uint64_t sum = 0ull;
   const uint64_t minus = f2_pack(-1.f, -1.f);
@@ -161,30 +161,30 @@ __device__ __forceinline__ float kt_weights(uint32_t addr, const float4* sc, flo
         const uint64_t e = f2_pack(e0, e1), p = f2_mul(e, w2);
         sum = f2_add(sum, e);
         hi[k * 8 + i] = ka_pack(f2_lo(p), f2_hi(p));
-        if (WIDE) {
-          const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&hi[k * 8 + i]));
-          const uint64_t r = f2_fma(f2_pack(y.x, y.y), minus, p);
-          lo[k * 8 + i] = ka_pack(f2_lo(r), f2_hi(r));
-        }
+        const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&hi[k * 8 + i]));
+        const uint64_t r = f2_fma(f2_pack(y.x, y.y), minus, p);
+        lo[k * 8 + i] = ka_pack(f2_lo(r), f2_hi(r));
       }
     }
     kt_st16(addr + h * 32, hi);
-    if (WIDE) kt_st16(addr + h * 32 + 16, lo);
+    kt_st16(addr + h * 32 + 16, lo);
   }
   return f2_lo(sum) + f2_hi(sum);
 }
 
-// f32 rows: the tensor cores cut sums off where an f32 addition rounds, and O has
+// The tensor cores cut sums off where an f32 addition rounds, and O has
 // eight additions a tile (four k-steps, two halves of P).  125 tiles in one go
 // came out 7.9e-6 too small (relative, least squares over all outputs, scores of
 // deviation 1.6).  So O goes into f32 sums in the workspace, which L2 holds, every
-// KT_FLUSH tiles: 2.1e-6, and what n tiles lose on average, (0.8 + 0.125 n) 1e-6,
-// is made good.  The error of the whole, 8.6e-6 before, is 1.2e-6 then, that of
+// KT_FLUSH tiles (f32 rows 8: 2.1e-6, and what n tiles lose on average, (0.8 + 0.125 n) 1e-6,
+// is made good).  The error of the whole, 8.6e-6 before, is 1.2e-6 then, that of
 // f32 sums in order 1.5e-6.  Where few positions carry a row less is lost and
 // that factor remains as an error of 1.8e-6 at most.
 // Cost, 2 x 1024 rows of 32 heads against 8000 positions: 355 -> 388 us (16
 // tiles: 370; adding in L2 by red.add instead of a load and a store: 481).
-constexpr int KT_FLUSH = 8;
+// 16-bit rows: every 64 tiles, 8.8e-6, a fiftieth of f16's rounding, at no cost to speak of.
+template <bool WIDE>
+constexpr int KT_FLUSH = WIDE ? 8 : 64;
 
 __device__ __forceinline__ float kt_lost(int n) { return fmaf((float)n, 0.125e-6f, 1.0000008f); }
 
@@ -195,7 +195,7 @@ struct KtShape {
   static constexpr int Q = QP * HALVES * (WIDE ? 2 : 1);
   static constexpr int KP = KT_KEYS * 128, K = KP * HALVES;
   static constexpr int SMEM = Q + 2 * K + 1024;     // + alignment
-  static constexpr int REC = KT_ROWS * (HD + 2);
+  static constexpr int REC = KT_ROWS * (HD + 2), FLUSH = KT_FLUSH<WIDE>;
 };
 
 // The units of a CTA's stretch, one after the other.  A unit (group of QT tokens,
@@ -428,14 +428,14 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
           m = top;
           l *= alpha;
         }
-        if (WIDE && j > 0 && j % KT_FLUSH == 0) {  // PV of this tile begins O anew
+        if (j > 0 && j % Sh::FLUSH == 0) {  // PV of this tile begins O anew
           float4* kept = reinterpret_cast<float4*>(a.work + (int64_t)(2 * gridDim.x + blockIdx.x) * Sh::REC) + r;
-          const bool add = j > KT_FLUSH;
+          const bool add = j > Sh::FLUSH;
           const float beta = add && s_ms[r] > -INFINITY ? ka_exp2(s_ms[r] - m) : 0.f;
           s_ms[r] = m;
           mbar_wait(&pvdone[(t - 1) & 1], ((t - 1) >> 1) & 1);
           kt_fence_after();
-          const float up = alpha * kt_lost(KT_FLUSH);
+          const float up = WIDE ? alpha * kt_lost(Sh::FLUSH) : alpha;
 #pragma unroll 1
           for (int h = 0; h < HD / 16; ++h, kept += 4 * KT_ROWS) {
             float4 y[4];
@@ -464,8 +464,8 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
           }
         }
         const float ref = m == -INFINITY ? 0.f : m;
-        l += masked ? kt_weights<WIDE, true>(at_s, s_sc[t & 3], fac, ref, left)
-                    : kt_weights<WIDE, false>(at_s, s_sc[t & 3], fac, ref, left);
+        l += masked ? kt_weights<true>(at_s, s_sc[t & 3], fac, ref, left)
+                    : kt_weights<false>(at_s, s_sc[t & 3], fac, ref, left);
         kt_wait_st();
         kt_fence_before();
         __syncwarp();
@@ -480,8 +480,8 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
         mbar_wait(&pvdone[(T - 1) & 1], ((T - 1) >> 1) & 1);
         kt_fence_after();
       }
-      const float beta = WIDE && w.n > KT_FLUSH && s_ms[r] > -INFINITY ? ka_exp2(s_ms[r] - m) : 0.f;
-      const float up = kt_lost((w.n - 1) % KT_FLUSH + 1);
+      const float beta = w.n > Sh::FLUSH && s_ms[r] > -INFINITY ? ka_exp2(s_ms[r] - m) : 0.f;
+      const float up = kt_lost((w.n - 1) % Sh::FLUSH + 1);
       const float4* kept = reinterpret_cast<const float4*>(a.work + (int64_t)(2 * nc + c) * Sh::REC) + r;
       const float scale = whole ? (l > 0.f ? 1.f / (KT_LIFT * l) : 0.f * l) : KA_LIFT / KT_LIFT;
       const int64_t o0 = (int64_t)(w.u.row0 + r / a.GH) * a.ldo + (int64_t)(w.u.head0 + r % a.GH) * HD;
@@ -498,7 +498,7 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[i] *= up;
         }
-        if (WIDE && w.n > KT_FLUSH) {
+        if (w.n > Sh::FLUSH) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const float4 y = __ldcg(kept + (h * 8 + i) * KT_ROWS);
@@ -682,11 +682,11 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
           kt_fence_after();
           if (kt_elect()) {
 #pragma unroll
-            for (int x = 0; x < (WIDE ? 2 : 1); ++x)
+            for (int x = 0; x < 2; ++x)
 #pragma unroll
               for (int k = 0; k < KT_KEYS / 16; ++k)  // 16 positions: two atoms further
                 kt_mma_ts(tmem_o, tmem + (p & 1) * KT_KEYS + (k >> 1) * 32 + x * 16 + (k & 1) * 8, dv + k * (2048 >> 4),
-                          io, (x | k) != 0 || (WIDE ? (j - 1) % KT_FLUSH != 0 : j != 1));
+                          io, (x | k) != 0 || (j - 1) % Sh::FLUSH != 0);
             kt_commit(&pvdone[p & 1]);
           }
           __syncwarp();

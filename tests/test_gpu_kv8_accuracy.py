@@ -1,0 +1,68 @@
+"""How exact kv8_attention is where its own tests leave room: rows of 16-bit types, rows that one
+position carries, chunks over many tiles.  The reference and the bound are those of test_gpu_kv8's
+docstring for f32 rows (weights in two 11-bit halves, sums in f32: 2^-18 of sum_j p_j |v_j|), for
+every type, and one rounding of the result to its type."""
+import numpy as np
+import pytest
+import torch
+
+import test_gpu_kv8 as base
+from test_gpu_kv8 import DT, HostCache, i32, make_pages, make_table, starts
+
+from lama32_mojo_b200 import ops
+
+pytestmark = pytest.mark.gpu
+
+
+def attend(cuda, kv, G, hd, page, ns, ctx, dtype, seed, width=None, pages=None):
+    """(outputs, reference, bound) of a call, f64 [T, heads, hd]."""
+    total = sum(-(-int(c) // page) for c in ctx) + 1
+    pages = pages or make_pages(cuda, total, kv, page, hd, seed)
+    table = make_table(ctx, page, pages.num_pages, seed, width)
+    heads, T = kv * G, int(sum(ns))
+    g = torch.Generator(device=cuda).manual_seed(seed)
+    q = torch.randn((T, heads * hd), device=cuda, generator=g).to(DT[dtype])
+    got = ops.kv8_attention(q, i32(starts(ns), cuda), i32(ctx, cuda), heads, pages, i32(table, cuda))
+    base.reference.tol16 = np.zeros((T, heads, hd))
+    ref, tol = base.reference(HostCache(pages), q.double().cpu().numpy().reshape(T, heads, hd), ns, ctx, table, heads)
+    info = torch.finfo(DT[dtype])
+    tol = tol + info.eps / 2 * np.abs(ref) + info.smallest_normal * info.eps / 2 + 1e-37
+    return got.double().cpu().numpy().reshape(T, heads, hd), ref, tol
+
+
+# every form: clusters, stretches, chunks on tcgen05 (the table's width decides)
+@pytest.mark.parametrize("kv,G,hd,page,ns,ctx,width", [
+    (2, 4, 128, 64, [1] * 6, [1, 2, 17, 64, 200, 301], None),
+    (2, 3, 64, 16, [1] * 40, list(range(1, 281, 7)), 900),
+    (2, 4, 128, 64, [5, 3, 4, 1], [5, 40, 130, 77], None),
+    (2, 12, 64, 32, [5] * 12, list(range(5, 245, 20)), 400),
+    (1, 4, 128, 64, [70, 33], [300, 33], 400),
+    (1, 4, 64, 64, [130, 64], [130, 500], 400),
+])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_rows_of_16_bit_types_are_rounded_once(cuda, kv, G, hd, page, ns, ctx, width, dtype):
+    got, ref, tol = attend(cuda, kv, G, hd, page, ns, ctx, dtype, G + hd, width)
+    assert (np.abs(got - ref) / tol).max() <= 1
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_long_chunks_of_16_bit_rows_in_one_stretch(cuda, dtype, hd):
+    """330 times a chunk against 6000 positions: single CTAs add up more than 64 tiles of 64 positions,
+    with scores that grow along the context."""
+    G, page, n, ctx, S = 4, 64, 32, 6000, 330
+    pages = make_pages(cuda, 94, 1, page, hd, 6)
+    pages.k_scale.mul_(torch.linspace(0.2, 3.0, 94, device=cuda)[:, None, None])
+    row = np.arange(94, dtype=np.int32)
+    q = torch.randn((n, G * hd), device=cuda, generator=torch.Generator(device=cuda).manual_seed(6)).to(DT[dtype])
+    got = ops.kv8_attention(q.repeat(S, 1), i32(starts([n] * S), cuda), i32([ctx] * S, cuda), G, pages,
+                            i32(np.tile(row, (S, 1)), cuda)).view(S, n, G, hd)
+    base.reference.tol16 = np.zeros((n, G, hd))
+    ref, tol = base.reference(HostCache(pages), q.double().cpu().numpy().reshape(n, G, hd), [n], [ctx], row[None], G)
+    info = torch.finfo(DT[dtype])
+    # sums of 64 tiles are cut off at the 24th bit some 8 times a tile: 64 * 8 * 2^-24 of sum_j p_j |v_j| at most,
+    # which is 8 times the docstring's 2^-18; tol holds that once already
+    mag = tol / 2.0 ** -18
+    tol = tol + mag * 64 * 8 * 2.0 ** -24 + info.eps / 2 * np.abs(ref) + info.smallest_normal * info.eps / 2
+    err = (got.double() - torch.from_numpy(ref).to(cuda)).abs()
+    assert float((err / torch.from_numpy(tol).to(cuda)).max()) <= 1
