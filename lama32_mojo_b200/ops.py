@@ -327,9 +327,11 @@ def kv8_attention(q, seq_start, ctx, n_heads: int, pages: KV8Pages, block_table,
         if To != T or out.dtype != q.dtype:
             raise ValueError("kv8_attention: out must have q's rows and type")
     nbytes = _kv8_scratch(dev, _DT[q.dtype], T, S, n_heads, pages.n_kv, pages.head_dim, width * pages.page)
-    work = torch.empty(nbytes, dtype=torch.uint8, device=q.device).data_ptr() if nbytes else None
+    # held until the kernels are in the stream: the allocator may give a free block to another thread before that
+    work = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
     _call(lib().q8op_kv8_attention, dev, q.data_ptr(), ldq, _DT[q.dtype], T, seq_start.data_ptr(), ctx.data_ptr(), S,
-          n_heads, pages._ref, block_table.data_ptr(), width, out.data_ptr(), ldo, work, nbytes)
+          n_heads, pages._ref, block_table.data_ptr(), width, out.data_ptr(), ldo,
+          None if work is None else work.data_ptr(), nbytes)
     return out
 
 

@@ -1,0 +1,72 @@
+"""How the Python entries of the paged-cache serving operators make their calls: what they hand to
+the library stays alive until the call has returned."""
+import gc
+import threading
+import types
+import weakref
+
+import numpy as np
+import pytest
+import torch
+
+from lama32_mojo_b200 import ops
+
+
+def test_attention_scratch_lives_through_the_call(monkeypatch):
+    """ctypes lets other threads run during the call: a scratch that is free by then may be theirs."""
+    made, seen, empty = [], [], torch.empty
+
+    def tracked(*a, **kw):
+        t = empty(*a, **kw)
+        made.append((weakref.ref(t), t.data_ptr()))
+        return t
+
+    def call(fn, dev, *args):
+        gc.collect()
+        seen.append([r() is not None and at in args for r, at in made])
+
+    pages = types.SimpleNamespace(head_dim=64, n_kv=1, page=64, _ref=0)
+    monkeypatch.setattr(ops, "_packed", lambda *a: (1, 4, 0))
+    monkeypatch.setattr(ops, "_kv8_scratch", lambda *a: 256)
+    monkeypatch.setattr(ops, "_rows_of", lambda t, *a: (t.shape[0], 64))
+    monkeypatch.setattr(ops, "_call", call)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    q, i = torch.zeros((1, 64)), torch.zeros(2, dtype=torch.int32)
+    monkeypatch.setattr(torch, "empty", tracked)
+    ops.kv8_attention(q, i, i, 1, pages, i)
+    assert seen == [[True]]
+
+
+@pytest.mark.gpu
+def test_attention_from_two_threads_on_one_stream(cuda):
+    """Two host threads on the default stream, each with calls that need a scratch and tensors of
+    its own in between: the bits of calls made alone."""
+    from test_gpu_kv8 import i32, make_pages, make_table, starts
+    kv, G, hd, page = 4, 4, 128, 16
+    work = []
+    for seed, ns, ctx, width in ((1, [1] * 40, list(range(1, 1600, 40)), 300), (2, [300, 5, 200], [900, 70, 200], 57)):
+        total = int(sum(-(-c // page) for c in ctx))
+        pages = make_pages(cuda, total, kv, page, hd, seed)
+        table = i32(make_table(ctx, page, total, seed, width=max(width, -(-max(ctx) // page))), cuda)
+        q = torch.randn((sum(ns), kv * G * hd), device=cuda)
+        args = q, i32(starts(np.array(ns)), cuda), i32(ctx, cuda), kv * G, pages, table
+        work.append((args, ops.kv8_attention(*args)))
+    torch.cuda.synchronize()
+    wrong, go = [], threading.Barrier(2)
+
+    def run(k):
+        args, want = work[k]
+        go.wait()
+        for _ in range(60):
+            got = ops.kv8_attention(*args)
+            other = [torch.full((1 << s,), float(k), device=cuda) for s in range(10, 22, 2)]
+            if not torch.equal(got, want):
+                wrong.append(k)
+            del other
+
+    threads = [threading.Thread(target=run, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
