@@ -172,21 +172,18 @@ __device__ __forceinline__ float kt_weights(uint32_t addr, const float4* sc, flo
   return f2_lo(sum) + f2_hi(sum);
 }
 
-// The tensor cores cut sums off where an f32 addition rounds, and O has
-// eight additions a tile (four k-steps, two halves of P).  125 tiles in one go
-// came out 7.9e-6 too small (relative, least squares over all outputs, scores of
-// deviation 1.6).  So O goes into f32 sums in the workspace, which L2 holds, every
-// KT_FLUSH tiles (f32 rows 8: 2.1e-6, and what n tiles lose on average, (0.8 + 0.125 n) 1e-6,
-// is made good).  The error of the whole, 8.6e-6 before, is 1.2e-6 then, that of
-// f32 sums in order 1.5e-6.  Where few positions carry a row less is lost and
-// that factor remains as an error of 1.8e-6 at most.
-// Cost, 2 x 1024 rows of 32 heads against 8000 positions: 355 -> 388 us (16
-// tiles: 370; adding in L2 by red.add instead of a load and a store: 481).
-// 16-bit rows: every 64 tiles, 8.8e-6, a fiftieth of f16's rounding, at no cost to speak of.
+// The tensor cores cut sums off where an f32 addition rounds, and O has eight
+// additions a tile (four k-steps, two halves of P).  125 tiles in one go came out
+// 7.9e-6 too small (relative, least squares over all outputs, scores of deviation
+// 1.6).  So O goes into f32 sums in the workspace, which L2 holds, every KT_FLUSH
+// tiles.  f32 rows, 8 tiles: errors of whole outputs against 8000 positions, q of
+// deviation 0.5, 2 and 8, are 0.8e-6, 2.5e-6 and 1.8e-6, those of elementary f32
+// operations 1.6e-6, 2.0e-6 and 1.8e-6; what is left comes from the scores.
+// 4 tiles: 0.5e-6, 2.0e-6, 1.8e-6 at 417 us for 383 (2 x 1024 rows of 32 heads,
+// 8000 and 2524 positions; no flush 355, adding in L2 by red.add 481).
+// 16-bit rows, 64 tiles: 8.8e-6, a fiftieth of f16's rounding, at no cost to speak of.
 template <bool WIDE>
 constexpr int KT_FLUSH = WIDE ? 8 : 64;
-
-__device__ __forceinline__ float kt_lost(int n) { return fmaf((float)n, 0.125e-6f, 1.0000008f); }
 
 template <bool WIDE, int HD>
 struct KtShape {
@@ -435,7 +432,6 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
           s_ms[r] = m;
           mbar_wait(&pvdone[(t - 1) & 1], ((t - 1) >> 1) & 1);
           kt_fence_after();
-          const float up = WIDE ? alpha * kt_lost(Sh::FLUSH) : alpha;
 #pragma unroll 1
           for (int h = 0; h < HD / 16; ++h, kept += 4 * KT_ROWS) {
             float4 y[4];
@@ -445,9 +441,9 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
             kt_ld16(tmem_o + lanes + h * 16, v);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              __stcg(kept + i * KT_ROWS, make_float4(fmaf(y[i].x, beta, v[4 * i] * up), fmaf(y[i].y, beta, v[4 * i + 1] * up),
-                                                     fmaf(y[i].z, beta, v[4 * i + 2] * up),
-                                                     fmaf(y[i].w, beta, v[4 * i + 3] * up)));
+              __stcg(kept + i * KT_ROWS, make_float4(fmaf(y[i].x, beta, v[4 * i] * alpha), fmaf(y[i].y, beta, v[4 * i + 1] * alpha),
+                                                     fmaf(y[i].z, beta, v[4 * i + 2] * alpha),
+                                                     fmaf(y[i].w, beta, v[4 * i + 3] * alpha)));
           }
         } else if (j > 0 && __any_sync(0xffffffffu, grew)) {
           mbar_wait(&pvdone[(t - 1) & 1], ((t - 1) >> 1) & 1);  // O is up to date
@@ -481,7 +477,6 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
         kt_fence_after();
       }
       const float beta = w.n > Sh::FLUSH && s_ms[r] > -INFINITY ? ka_exp2(s_ms[r] - m) : 0.f;
-      const float up = kt_lost((w.n - 1) % Sh::FLUSH + 1);
       const float4* kept = reinterpret_cast<const float4*>(a.work + (int64_t)(2 * nc + c) * Sh::REC) + r;
       const float scale = whole ? (l > 0.f ? 1.f / (KT_LIFT * l) : 0.f * l) : KA_LIFT / KT_LIFT;
       const int64_t o0 = (int64_t)(w.u.row0 + r / a.GH) * a.ldo + (int64_t)(w.u.head0 + r % a.GH) * HD;
@@ -493,10 +488,6 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
         } else {
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[i] = 0.f;
-        }
-        if (WIDE) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] *= up;
         }
         if (w.n > Sh::FLUSH) {
 #pragma unroll

@@ -66,3 +66,33 @@ def test_long_chunks_of_16_bit_rows_in_one_stretch(cuda, dtype, hd):
     tol = tol + mag * 64 * 8 * 2.0 ** -24 + info.eps / 2 * np.abs(ref) + info.smallest_normal * info.eps / 2
     err = (got.double() - torch.from_numpy(ref).to(cuda)).abs()
     assert float((err / torch.from_numpy(tol).to(cuda)).max()) <= 1
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("ctx", [40, 1000])
+def test_chunk_rows_that_one_position_carries(cuda, hd, ctx):
+    """f32 rows of chunks whose result is the value of one position: the first rows of fresh prompts
+    (ctx 40), and rows whose scores but one are so low that the other weights are 0 (ctx 1000, the
+    position in the first of 16 tiles).  The weight has 22 bits (2^-22), its two halves' products
+    are cut off at 24 bits (2 * 2^-23), l's quotient and the last product round (2^-24 each), and
+    exp2 of the row's largest score is one but for 2 ulps that weight and l share; 2^-24 more for
+    each of the scale and the reference's own rounding."""
+    G, kv, page, n, S = 4, 4, 64, 40, 64
+    per = -(-ctx // page)
+    pages = make_pages(cuda, per, kv, page, hd, hd)
+    g = torch.Generator(device=cuda).manual_seed(hd)
+    q = torch.rand((S * n, kv * G * hd), device=cuda, generator=g) + 0.5
+    if ctx > n:
+        pages.k.zero_()
+        pages.k[0, :, 5] = 127
+        pages.k_scale.fill_(1.0)
+    row = np.arange(per, dtype=np.int32)
+    got = ops.kv8_attention(q, i32(starts([n] * S), cuda), i32([ctx] * S, cuda), kv * G, pages,
+                            i32(np.tile(row, (S, 1)), cuda)).view(S, n, kv, G, hd).double()
+    at = 5 if ctx > n else 0
+    want = pages.v[0, :, at].double() * pages.v_scale[0, :, at // 16, None].double()  # [kv, hd]
+    if ctx == n:
+        got = got[:, :1]
+    err = (got - want[:, None]).abs() / want.abs().clamp(min=1e-30)[:, None]
+    err = err[torch.broadcast_to(want[:, None] != 0, err.shape)]
+    assert float(err.max()) <= 2.0 ** -22 + 2 * 2.0 ** -23 + 4 * 2.0 ** -24
