@@ -26,10 +26,10 @@
 // becomes the B operand by movmatrix.
 //
 // Softmax: base 2, running maximum M of s + log2(sv) rather than of s: the
-// weights that meet the codes are e sv, e = 2^(s - M), so they stay within
-// (0, 1] whatever the blocks' scales are, and l = sum e is kept against the same
-// M (a sv of 0 counts as 2^-100 in M).  They are lifted by 2^15 to the top of the
-// f16 range, whose smallest step, 2^-24, is then 2^-39 of the row's largest one.
+// weights that meet the codes are e sv, e = 2^(s - M), so they stay within one
+// range whatever the blocks' scales are, and l = sum e is kept against the same
+// M.  The largest is 2^15, at the top of the f16 range, whose smallest step,
+// 2^-24, is then 2^-39 of it.  How M is shifted for that: KA_DOWN.
 //
 // Joining.  The warps of a CTA join through shared memory.  Few units of work
 // (group x kv head): the CTAs that share a unit form a cluster and join through
@@ -352,7 +352,7 @@ __device__ __forceinline__ void ka_stretch(const Kv8AttnArgs& a, const KaUnit& u
     float lsv[BPI];
     const int p0 = (lo + (warp + it * warps) * BPI) * KV8_BLOCK + g;
 #pragma unroll
-    for (int j = 0; j < BPI; ++j) lsv[j] = fmaxf(__log2f(sv[j]), -100.f);
+    for (int j = 0; j < BPI; ++j) lsv[j] = fmaxf(__log2f(sv[j]), KA_LEAST) - KA_DOWN;
     uint32_t pb[BPI][NT][2], pr[BPI][WIDE ? 1 : NT][2];  // pr: what the f16 of pb leave of the weights
     bool moved = false;
     float alpha[NT][RT];
@@ -376,7 +376,7 @@ __device__ __forceinline__ void ka_stretch(const Kv8AttnArgs& a, const KaUnit& u
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
         const float mn = fmaxf(m[nt][r], top);
         const float ref = mn == -INFINITY ? 0.f : mn;
-        alpha[nt][r] = ka_exp2(m[nt][r] - ref);
+        alpha[nt][r] = ka_lower<false>(l[nt][r], m[nt][r] - ref);
         moved |= mn != m[nt][r];
         m[nt][r] = mn;
         float sum = 0.f;
@@ -387,7 +387,7 @@ __device__ __forceinline__ void ka_stretch(const Kv8AttnArgs& a, const KaUnit& u
             s[j][nt][r][e] = ka_exp2(s[j][nt][r][e] - ref);
             sum += s[j][nt][r][e];
           }
-        l[nt][r] = l[nt][r] * alpha[nt][r] + sum;
+        l[nt][r] += sum;
       }
 #pragma unroll
       for (int j = 0; j < BPI; ++j) {
@@ -465,9 +465,10 @@ __device__ __forceinline__ void ka_stretch(const Kv8AttnArgs& a, const KaUnit& u
   // join the warps: lane w knows warp w's m and l
   constexpr int D = HD / 32;
   for (int r = warp; r < nrow; r += warps) {
-    const float mw = lane < warps ? pm[lane * RMAX + r] : -INFINITY, lw = lane < warps ? pl[lane * RMAX + r] : 0.f;
-    const float mx = warp_max(mw), f = exp2f(mw - (mx == -INFINITY ? 0.f : mx));
-    const float sum = warp_sum(f * lw);
+    const float mw = lane < warps ? pm[lane * RMAX + r] : -INFINITY, mx = warp_max(mw);
+    float lw = lane < warps ? pl[lane * RMAX + r] : 0.f;
+    const float f = ka_lower<true>(lw, mw - (mx == -INFINITY ? 0.f : mx));
+    const float sum = warp_sum(lw);
     float x[D];
 #pragma unroll
     for (int e = 0; e < D; ++e) x[e] = 0.f;
@@ -566,9 +567,9 @@ __global__ void __launch_bounds__(KaShape<WIDE, HD, NT>::WARPS * 32, 1) k_kv8_at
   for (; k0 < n; k0 += step) {
     const int r = k0 / HD;
     const float m = lane < nsplit ? ka_remote(s_m + r, lane) : -INFINITY;
-    const float l = lane < nsplit ? ka_remote(s_l + r, lane) : 0.f;
-    const float mx = warp_max(m), f = exp2f(m - (mx == -INFINITY ? 0.f : mx));
-    const float sum = warp_sum(f * l);
+    float l = lane < nsplit ? ka_remote(s_l + r, lane) : 0.f;
+    const float mx = warp_max(m), f = ka_lower<true>(l, m - (mx == -INFINITY ? 0.f : mx));
+    const float sum = warp_sum(l);
     float x = 0.f;
     for (int c = 0; c < nsplit; ++c) x += __shfl_sync(0xffffffffu, f, c) * ka_remote(part + k0 + lane, c);
     if (k0 + step >= n) cluster_leave();
@@ -688,10 +689,11 @@ __global__ void __launch_bounds__(256) k_kv8_attn_join(Kv8AttnArgs a, int RMAX) 
     float v[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) v[e] = rec[r * HD + lane * E + e];
-    const float m = rec[RMAX * HD + r], l = rec[RMAX * HD + RMAX + r];
+    const float m = rec[RMAX * HD + r];
+    float l = rec[RMAX * HD + RMAX + r];
     const float top = fmaxf(mx, m), ref = top == -INFINITY ? 0.f : top;
-    const float f0 = exp2f(mx - ref), f1 = exp2f(m - ref);
-    sum = sum * f0 + l * f1;
+    const float f0 = ka_lower<true>(sum, mx - ref), f1 = ka_lower<true>(l, m - ref);
+    sum += l;
 #pragma unroll
     for (int e = 0; e < E; ++e) x[e] = x[e] * f0 + v[e] * f1;
     mx = top;

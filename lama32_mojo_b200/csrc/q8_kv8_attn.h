@@ -9,7 +9,11 @@
 
 namespace q8 {
 
-constexpr float KA_LIFT = 32768.f;
+// M of a block: s + log2(sv) less KA_DOWN, a sv below 2^KA_LEAST counting as that, so that e = 2^(s - M) is
+// between 2^(24 - 121) for the largest sv and 2^(24 + 72) for the least one: l = sum e of 2^31 positions
+// stays finite, and what e can lose below f32's smallest normal number is 2^-29 of the row's largest weight.
+constexpr float KA_DOWN = 24.f, KA_LEAST = -72.f;
+constexpr float KA_LIFT = 0x1p-9f;  // weights are e sv KA_LIFT: the largest is 2^15
 
 struct Kv8AttnArgs {
   const void* q;
@@ -51,6 +55,18 @@ __device__ __forceinline__ float ka_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// l 2^d and 2^d, d <= 0 the step of a running maximum.  Between blocks of the least and the largest scales d lies
+// below f32's exponents (-193 and the scores' difference), but l, 2^96 against 2^-97, does not.
+template <bool EXACT>
+__device__ __forceinline__ float ka_lower(float& l, float d) {
+  const bool far = d < -100.f;
+  const float e = far ? d + 96.f : d;
+  const float f = EXACT ? exp2f(e) : ka_exp2(e);
+  l *= f;
+  if (far) l *= 0x1p-96f;
+  return far ? 0.f : f;
 }
 
 // four consecutive elements from element i0 on as floats

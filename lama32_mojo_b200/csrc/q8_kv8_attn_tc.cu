@@ -16,7 +16,7 @@
 // p = ph + pl, two products (22 bits; the codes need one f16); f32 rows: q = qh + ql
 // too.  4 x 128 x 64 x hd multiply-adds a tile, bf16 / f16 rows 3.
 // M moves only when it has grown by more than 1, so that O in TMEM is scaled
-// seldom; weights stay below 2, lifted by 2^14.
+// seldom.
 //
 // Bound.  2 x 1024 f32 rows of 32 heads on 8 of 128, 8000 positions: 385 us for
 // 258 GFLOP, 516 in f16 products (1.34 PFLOP/s, 0.81 of cuBLAS's bf16 rate).  The
@@ -33,7 +33,7 @@ namespace q8 {
 
 constexpr int KT_BLOCKS = KV8_TILE, KT_KEYS = KT_BLOCKS * KV8_BLOCK;
 constexpr int KT_THREADS = 288;
-constexpr float KT_LIFT = 16384.f;
+constexpr float KT_LIFT = KA_LIFT / 2;  // M lags by up to 1: weights are 2^15 at most
 constexpr int KT_FIXED = 512;  // work of beginning and ending a unit, in positions
 
 __device__ __forceinline__ void kt_arrive(uint64_t* bar) {
@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
   __shared__ __align__(8) uint64_t qfull, kfull, kfree, vfull, pvdone[2], sfull[2], pfull[2], scfull[4];
   __shared__ uint32_t s_tmem;
   __shared__ float s_fac[KT_ROWS], s_ms[KT_ROWS];  // s_ms: M of the flushed sums, which lie as [dim / 4][row]
-  __shared__ float4 s_sc[4][KT_BLOCKS];  // sk, lifted sv, log2 sv (-inf: no page)
+  __shared__ float4 s_sc[4][KT_BLOCKS];  // sk, sv KT_LIFT, its part of M (-inf: no page)
   __shared__ int64_t s_scan[KT_THREADS / 32], s_at;
   __shared__ int s_b;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -421,9 +421,8 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
         float alpha = 1.f;
         const bool grew = top > m + 1.f || (m == -INFINITY && top > -INFINITY);
         if (grew) {
-          alpha = ka_exp2(m - top);
+          alpha = ka_lower<false>(l, m - top);
           m = top;
-          l *= alpha;
         }
         if (j > 0 && j % Sh::FLUSH == 0) {  // PV of this tile begins O anew
           float4* kept = reinterpret_cast<float4*>(a.work + (int64_t)(2 * gridDim.x + blockIdx.x) * Sh::REC) + r;
@@ -596,7 +595,7 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
       auto scales_out = [&](uint32_t t, int id) {
         if (warp != 4) return;
         if (lane < KT_BLOCKS)
-          s_sc[t & 3][lane] = make_float4(sk, sv * KT_LIFT, id >= 0 ? fmaxf(__log2f(sv), -100.f) : -INFINITY, 0.f);
+          s_sc[t & 3][lane] = make_float4(sk, sv * KT_LIFT, id >= 0 ? fmaxf(__log2f(sv), KA_LEAST) - KA_DOWN : -INFINITY, 0.f);
         __syncwarp();
         if (lane == 0) kt_arrive(&scfull[t & 3]);
       };

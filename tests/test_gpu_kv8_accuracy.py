@@ -96,3 +96,19 @@ def test_chunk_rows_that_one_position_carries(cuda, hd, ctx):
     err = (got - want[:, None]).abs() / want.abs().clamp(min=1e-30)[:, None]
     err = err[torch.broadcast_to(want[:, None] != 0, err.shape)]
     assert float(err.max()) <= 2.0 ** -22 + 2 * 2.0 ** -23 + 4 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("ns,ctx,width", [([1] * 6, [1, 2, 17, 64, 200, 301], None),
+                                          ([1] * 40, list(range(1, 281, 7)), 900),
+                                          ([5, 3, 4, 1], [5, 40, 130, 77], None), ([70, 130], [300, 130], 400)])
+@pytest.mark.parametrize("lo,hi", [(1.3e36, 2.6e36), (1e-25, 3e-25), (1e-25, 2e36)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_values_of_any_size(cuda, ns, ctx, width, lo, hi, dtype):
+    """Values up to f32's largest number (127 * 2.6e36), and small ones; every form."""
+    pages = make_pages(cuda, 20 if width is None else 110, 2, 64, 128, 3)
+    g = torch.Generator(device=cuda).manual_seed(3)
+    u = torch.rand(pages.v_scale.shape, generator=g, device=cuda, dtype=torch.float64)
+    pages.v_scale.copy_(torch.exp(np.log(lo) + u * (np.log(hi) - np.log(lo))))
+    got, ref, tol = attend(cuda, 2, 4, 128, 64, ns, ctx, dtype, 3, width, pages)
+    assert np.isfinite(got).all()
+    assert (np.abs(got - ref) / tol).max() <= 1
