@@ -131,10 +131,19 @@ __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)_
 
 // The last cluster barrier in two halves: a thread arrives once it has read what it needs of its
 // peers, stores its results, and waits at its end.  An arrival behind the stores would wait for them.
+// The aligned forms want their warps converged, which a branch or a loop by threads before them need not leave.
 __device__ __forceinline__ void cluster_leave() {
+  __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void cluster_left() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_left() {
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait_all() {
+  cluster_leave();
+  cluster_left();
+}
 
 __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");

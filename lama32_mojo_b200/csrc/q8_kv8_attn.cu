@@ -559,7 +559,7 @@ __global__ void __launch_bounds__(KaShape<WIDE, HD, NT>::WARPS * 32, 1) k_kv8_at
       s_l[r] = l;
     }
   });
-  cluster.sync();
+  cluster_wait_all();
   // 32 elements to a warp, the clusters' warps in turn; lane c knows CTA c's m and l
   const int n = u.toks * a.GH * HD, step = (blockDim.x >> 5) * nsplit * 32;
   int k0 = (warp * nsplit + split) * 32;

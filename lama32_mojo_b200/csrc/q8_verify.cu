@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
   bv = warp_max(bv);
   cluster_left();
   if (lane < nc) vf_send(&s_v[rank * WARPS + w], lane, bv);
-  cluster.sync();
+  cluster_wait_all();
   for (int k = lane; k < nc * WARPS; k += 32) bv = fmaxf(bv, s_v[k]);
   bv = warp_max(bv);
   if (!(temp > 0.f) || bv == -INFINITY) {
@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
         if (v[k][e] == bv && bv > -INFINITY) bi = lo + at + k * 4 * THREADS + e;
     bi = __reduce_min_sync(0xffffffffu, bi);
     if (lane < nc) vf_send(&s_i[rank * WARPS + w], lane, bi);
-    cluster.sync();
+    cluster_wait_all();
     for (int k = lane; k < nc * WARPS; k += 32) bi = min(bi, s_i[k]);
     bi = __reduce_min_sync(0xffffffffu, bi);
     if (bi == 0x7fffffff) bi = 0;  // nothing above -inf: as q8op_argmax
@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
   }
   sum = vf_warp_sum(sum);
   if (lane < nc) vf_send(&s_d[rank * WARPS + w], lane, sum);
-  cluster.sync();
+  cluster_wait_all();
   sum = 0.0;
   for (int k = lane; k < nc * WARPS; k += 32) sum += s_d[k];
   sum = vf_warp_sum(sum);
@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(VF_THREADS) k_verify(const float* __restrict__
       __syncwarp();
       if (lane == 0) s_sum = segs ? s_seg[segs - 1] : 0.0;
     }
-    cluster.sync();
+    cluster_wait_all();
     total = before = 0.0;
     for (int k = 0; k < nc; ++k) {
       if (k == rank) before = total;
@@ -332,7 +332,7 @@ __global__ void __launch_bounds__(VF_THREADS) k_verify(const float* __restrict__
     }
     if (total > 0.0 || !(qr || gone >= 0)) break;
     // p <= q everywhere: the refusal was a rounding's, p itself is drawn from
-    cluster.sync();
+    cluster_wait_all();
     qr = nullptr;
     gone = -1;
   }

@@ -1,0 +1,30 @@
+"""verify and probs where their own tests do not go: sequences that fill the last warp in part,
+weights that are not probabilities, vocabularies beyond a CTA's share, rows behind the last
+sequence.  The restatement is test_gpu_verify's; tokens and counts have to be equal."""
+import numpy as np
+import pytest
+
+from test_gpu_verify import check_verify, rows_of
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("n,drafts", [(9000, [33, 0, 65, 1, 31, 700]), (33000, [513]), (70000, [1, 40])])
+@pytest.mark.parametrize("certain", [False, True])
+def test_sequences_of_odd_lengths_over_clusters(cuda, n, drafts, certain):
+    """Rows that do not fill the warps that store them, several CTAs a sequence."""
+    rng = np.random.default_rng(n)
+    starts = np.concatenate([[0], np.cumsum([d + 1 for d in drafts])])
+    rows = int(starts[-1])
+    p = rows_of(rng, rows, n)
+    last = set(starts[1:] - 1)
+    body = [r for r in range(rows) if r not in last]
+    q = p[body]
+    ids = np.zeros(rows, np.int64)
+    for r in body:
+        ids[r + 1] = p[r].argmax()
+    u = (rng.random(rows) * 0.9).astype(np.float32)
+    for b in range(len(drafts)):  # a refused draft somewhere in each
+        if drafts[b]:
+            u[starts[b] + rng.integers(drafts[b])] = 1.0
+    check_verify(p, None if certain else q, ids, starts, u, cuda)
