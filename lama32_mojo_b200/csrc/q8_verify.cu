@@ -434,7 +434,9 @@ static int vf_launch(const char* what, int64_t rows, int c, int threads, size_t 
 using namespace q8;
 
 constexpr int64_t VF_PROBS_MAX = (int64_t)VF_MAX_CLUSTER * vf_slice(VF_THREADS);  // 327,680
-constexpr int64_t VF_VERIFY_MAX = (int64_t)VF_MAX_CLUSTER * 20000 * VF_SEG;
+constexpr int VF_SEGS = 20000;                         // sums that a CTA of k_verify holds
+constexpr int64_t VF_SLICE = (int64_t)VF_SEGS * VF_SEG;  // and the columns of them
+constexpr int64_t VF_VERIFY_MAX = VF_MAX_CLUSTER * VF_SLICE;
 
 extern "C" int q8op_probs(const float* logits, int64_t rows, int64_t n, int64_t ld, float temp, float* out,
                           int64_t ldo, void* stream) {
@@ -471,8 +473,8 @@ extern "C" int q8op_verify(const float* p, int64_t ldp, const float* q, int64_t 
                "q8op_verify: bad shape");
   if (S == 0) return Q8_OK;
   Q8_CHECK_ARG(seq_start && n_accepted && (rows == 0 || (p && ids && u && tokens)), "q8op_verify: null pointer");
-  const int c = vf_cluster(S, n, 1, 2 * num_sms());
+  const int c = vf_cluster(S, n, (n + VF_SLICE - 1) / VF_SLICE, 2 * num_sms());
   const int per = (int)(((n + c - 1) / c + VF_SEG - 1) / VF_SEG * VF_SEG);
-  return vf_launch<k_verify>("k_verify", S, c, VF_THREADS, (size_t)(per / VF_SEG) * 8, 20001 * 8, (cudaStream_t)stream, p, ldp, q,
+  return vf_launch<k_verify>("k_verify", S, c, VF_THREADS, (size_t)(per / VF_SEG) * 8, VF_SEGS * 8, (cudaStream_t)stream, p, ldp, q,
                    ldq, (int)q_rows, ids, seq_start, (int)rows, (int)n, u, n_accepted, tokens, per);
 }

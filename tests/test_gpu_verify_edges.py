@@ -3,8 +3,11 @@ weights that are not probabilities, vocabularies beyond a CTA's share, rows behi
 sequence.  The restatement is test_gpu_verify's; tokens and counts have to be equal."""
 import numpy as np
 import pytest
+import torch
 
-from test_gpu_verify import check_verify, rows_of
+from test_gpu_verify import check_verify, i32, rows_of
+
+from lama32_mojo_b200 import ops
 
 pytestmark = pytest.mark.gpu
 
@@ -28,3 +31,14 @@ def test_sequences_of_odd_lengths_over_clusters(cuda, n, drafts, certain):
         if drafts[b]:
             u[starts[b] + rng.integers(drafts[b])] = 1.0
     check_verify(p, None if certain else q, ids, starts, u, cuda)
+
+
+@pytest.mark.parametrize("S,n", [(149, 2_700_001), (1, 40_960_000)])
+def test_columns_beyond_what_one_cta_holds(cuda, S, n):
+    """Many sequences get few CTAs each, but never fewer than their columns need; the most columns."""
+    p = torch.zeros((S, n), device=cuda)
+    at = torch.arange(S, device=cuda) * ((n - 1) // max(S - 1, 1))
+    at[-1] = n - 1
+    p[torch.arange(S, device=cuda), at] = 1.0
+    a, t = ops.verify(p, None, i32(np.zeros(S), cuda), i32(np.arange(S + 1), cuda), torch.full((S,), 0.5, device=cuda))
+    assert t.tolist() == at.tolist() and not a.any()
