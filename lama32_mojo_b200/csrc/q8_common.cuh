@@ -22,10 +22,13 @@ namespace q8 {
 void set_error(const char* fmt, ...);
 const char* get_error();
 
+// A call that fails leaves its error behind for the next reader (launch_check, or the caller's
+// own framework): it is taken back here, once it is reported.
 #define Q8_CUDA(call)                                                              \
   do {                                                                             \
     cudaError_t _e = (call);                                                       \
     if (_e != cudaSuccess) {                                                       \
+      cudaGetLastError();                                                          \
       ::q8::set_error("%s:%d %s: %s", __FILE__, __LINE__, #call,                   \
                       cudaGetErrorString(_e));                                     \
       return Q8_ERR_CUDA;                                                          \
@@ -46,14 +49,16 @@ const char* get_error();
     if (_s != Q8_OK) return _s;                                                    \
   } while (0)
 
-static inline int launch_check(const char* what) {
-  cudaError_t e = cudaGetLastError();
+static inline int launch_status(const char* what, cudaError_t e) {
   if (e != cudaSuccess) {
+    cudaGetLastError();
     set_error("launch %s: %s", what, cudaGetErrorString(e));
     return Q8_ERR_CUDA;
   }
   return Q8_OK;
 }
+
+static inline int launch_check(const char* what) { return launch_status(what, cudaGetLastError()); }
 
 // ------------------------------------------------------------------ layout helpers
 __host__ __device__ inline int64_t q8_row_bytes(int64_t k) { return k / 32 + k; }
@@ -224,12 +229,7 @@ inline int launch_pdl(const char* what, void (*kern)(KArgs...), dim3 grid, dim3 
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = pdl_enabled() ? 1 : 0;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
-  if (e != cudaSuccess) {
-    set_error("launch %s: %s", what, cudaGetErrorString(e));
-    return Q8_ERR_CUDA;
-  }
-  return Q8_OK;
+  return launch_status(what, cudaLaunchKernelEx(&cfg, kern, args...));
 }
 
 int num_sms();

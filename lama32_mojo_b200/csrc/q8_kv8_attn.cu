@@ -835,8 +835,7 @@ static int attn_run(const Kv8AttnArgs& a, const KaPlan& p, cudaStream_t st) {
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  Q8_CUDA(cudaLaunchKernelEx(&cfg, few, a));
-  return Q8_OK;
+  return launch_status("k_kv8_attn", cudaLaunchKernelEx(&cfg, few, a));
 }
 
 template <bool WIDE, int HD>

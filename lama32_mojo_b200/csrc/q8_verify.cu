@@ -421,12 +421,7 @@ static int vf_launch(const char* what, int64_t rows, int c, int threads, size_t 
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
-  if (e != cudaSuccess) {
-    set_error("launch %s: %s", what, cudaGetErrorString(e));
-    return Q8_ERR_CUDA;
-  }
-  return Q8_OK;
+  return launch_status(what, cudaLaunchKernelEx(&cfg, kern, args...));
 }
 
 }  // namespace q8

@@ -9,7 +9,7 @@ import numpy as np
 import pytest
 import torch
 
-from lama32_mojo_b200 import ops
+from lama32_mojo_b200 import _lib, ops
 
 
 def test_attention_scratch_lives_through_the_call(monkeypatch):
@@ -70,3 +70,17 @@ def test_attention_from_two_threads_on_one_stream(cuda):
     for t in threads:
         t.join()
     assert not wrong
+
+
+@pytest.mark.gpu
+def test_a_refused_launch_is_not_blamed_on_the_next_call(cuda):
+    """More blocks than a grid has (2^33, which an int counts as 0: nothing can run): the call says
+    so, and neither torch nor the library's next call sees its error."""
+    L, x = _lib.lib(), torch.randn((1, 256), device=cuda)
+    pos, inv = torch.zeros(1, dtype=torch.int32, device=cuda), torch.ones(32, device=cuda)
+    at = x.data_ptr()
+    status = L.q8op_rope_kv_append(at, 256, 2 ** 35, pos.data_ptr(), None, 1, 1, 64, inv.data_ptr(), None, None, 1e-6,
+                                   None, None, 0, None, 0, None)
+    assert status == _lib.Q8_ERR_CUDA and "k_rope_kv" in _lib.last_error()
+    assert int(ops.argmax(x)) == int(x.argmax())
+    assert float(torch.zeros(3, device=cuda).sum()) == 0.0
