@@ -350,9 +350,10 @@ int q8op_probs(const float* logits, int64_t rows, int64_t n, int64_t ld, float t
  * cumulative weight exceeds u[last row] times the whole (from p itself when
  * max(p - q, 0) is all zero).  n_accepted [S]: drafts kept.  tokens [rows]:
  * the kept drafts, the next token, then -1, from seq_start[b] on.  Sums are 64
- * bits.  NaN and negative weights count as 0; a draft outside [0, n), or
- * whose row of q is not among the q_rows, is refused; a row without any weight
- * gives token 0.  Rows from seq_start[S] on
+ * bits.  Negative weights, and NaN in p, count as 0.  A draft outside [0, n), or
+ * whose weight in q is NaN, or whose row of q is not among the q_rows, is
+ * refused; max(p - q, 0) is 0 where q is NaN, and p where its row is not there.
+ * A row without any weight gives token 0.  Rows from seq_start[S] on
  * are left as they are.  No counterpart in the reference. */
 int q8op_verify(const float* p, int64_t ldp, const float* q, int64_t ldq, int64_t q_rows, const int32_t* ids,
                 const int32_t* seq_start, int64_t rows, int64_t S, int64_t n, const float* u, int32_t* n_accepted,

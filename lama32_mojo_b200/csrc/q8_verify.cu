@@ -242,8 +242,8 @@ __global__ void __launch_bounds__(VF_THREADS) k_verify(const float* __restrict__
     const int x = ids[r + 1];
     bool keep = false;
     if (x >= 0 && x < n && (!q || r + q0 < q_rows)) {
-      const double qx = q ? (double)q[(int64_t)(r + q0) * ldq + x] : 1.0;
-      keep = (double)u[r] * qx < (double)p[(int64_t)r * ldp + x];
+      const double w = q ? (double)q[(int64_t)(r + q0) * ldq + x] : 1.0, qx = w < 0.0 ? 0.0 : w;
+      keep = (double)u[r] * qx < (double)p[(int64_t)r * ldp + x];  // never with a NaN
     }
     if (!keep) atomicMin(&s_stop, r);
   }
@@ -278,7 +278,7 @@ __global__ void __launch_bounds__(VF_THREADS) k_verify(const float* __restrict__
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const double d = (double)a[e] - (double)c[e];
+      const double d = (double)a[e] - (c[e] < 0.f ? 0.0 : (double)c[e]);
       v[e] = d > 0.0 && i + e != gone ? d : 0.0;
     }
   };

@@ -42,3 +42,23 @@ def test_columns_beyond_what_one_cta_holds(cuda, S, n):
     p[torch.arange(S, device=cuda), at] = 1.0
     a, t = ops.verify(p, None, i32(np.zeros(S), cuda), i32(np.arange(S + 1), cuda), torch.full((S,), 0.5, device=cuda))
     assert t.tolist() == at.tolist() and not a.any()
+
+
+def test_negative_and_nan_weights_of_q(cuda):
+    """A negative q counts as 0: it neither keeps a draft that p gives no weight, nor adds to the
+    next token's weights.  A NaN refuses its draft and takes its index out."""
+    n = 300
+    p = np.full((8, n), 1.0 / 128, np.float32)
+    p[:, 128:] = 0.0
+    q = np.full((4, n), 1.0 / 256, np.float32)
+    starts, ids, u = np.array([0, 2, 4, 6, 8]), np.zeros(8, np.int64), np.full(8, 0.5, np.float32)
+    ids[1], q[0, 200] = 200, -0.5  # p is 0: refused; index 200 must not be drawn
+    ids[3], q[1, 5] = 5, -3.0      # p is not 0: kept, as with q = 0
+    ids[5], q[2, 7] = 7, np.nan    # refused
+    ids[7], q[3, 9] = 250, -1e30   # refused; index 9 weighs p(9), no more
+    a, t = ops.verify(*(torch.from_numpy(x).to(cuda) for x in (p, q)), i32(ids, cuda), i32(starts, cuda),
+                      torch.from_numpy(u).to(cuda))
+    # 128 weights of 1/256: index i ends i + 1 of them, the first beyond half of them is 64; 127 without
+    # index 7: i > 63.5, 64; 129 with index 9 twice: i + 2 > 64.5, 63
+    assert a.tolist() == [0, 1, 0, 0]
+    assert t.tolist() == [64, -1, 5, 64, 64, -1, 63, -1]
