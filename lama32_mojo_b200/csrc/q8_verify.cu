@@ -342,7 +342,7 @@ __global__ void __launch_bounds__(VF_THREADS) k_verify(const float* __restrict__
   cluster_leave();
   // the first index whose cumulative weight exceeds u total lies in the CTA
   // that reaches beyond it; if rounding leaves none, the last index with a weight
-  const double r = (double)draw * total;
+  const double r = fmax((double)draw * total, 0.0);  // a draw that is none gives the first weight
   if (wid == 0) {
     const bool mine = before <= r && before + s_sum > r;
     if (mine) {
@@ -353,9 +353,14 @@ __global__ void __launch_bounds__(VF_THREADS) k_verify(const float* __restrict__
         if (before + s_seg[mid] > r) z = mid;
         else a = mid + 1;
       }
-      double v[4], cum = 0.0;
-      weights_of(std::integral_constant<int, 2>(), a, v);
-      cum = ((v[0] + v[1]) + v[2]) + v[3];
+      // the lanes of the running sums add in different orders, so a segment without a weight can begin beyond r by a
+      // rounding: the weights that got there lie before it
+      double v[4], cum;
+      for (;; --a) {
+        weights_of(std::integral_constant<int, 2>(), a, v);
+        cum = ((v[0] + v[1]) + v[2]) + v[3];
+        if (a == 0 || __any_sync(0xffffffffu, cum > 0.0)) break;
+      }
       double up = cum;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {

@@ -62,3 +62,18 @@ def test_negative_and_nan_weights_of_q(cuda):
     # index 7: i > 63.5, 64; 129 with index 9 twice: i + 2 > 64.5, 63
     assert a.tolist() == [0, 1, 0, 0]
     assert t.tolist() == [64, -1, 5, 64, 64, -1, 63, -1]
+
+
+def test_a_drawn_token_has_a_weight(cuda):
+    """Segments of 128 columns, one each for the lanes that add them up: 1 + 2^-53 + 2^-53 is 1 in the order
+    of the columns and 1 + 2^-52 in a tree, so that the empty fifth segment seems to begin beyond u times
+    the whole, 1 of 2.  The exact draw is the third weight, a sequential one the fourth.  And draws that
+    are none (negative, NaN) give tokens with a weight."""
+    n = 4096
+    p = np.zeros((3, n), np.float32)
+    p[:, 0] = p[:, 5 * 128] = 1.0
+    p[:, 2 * 128] = p[:, 3 * 128] = 2.0 ** -53
+    a, t = ops.verify(torch.from_numpy(p).to(cuda), None, i32(np.zeros(3), cuda), i32(np.arange(4), cuda),
+                      torch.tensor([0.5, -0.25, float("nan")], device=cuda))
+    assert int(t[0]) in (3 * 128, 5 * 128)
+    assert int(t[1]) == 0 and int(t[2]) in (0, 5 * 128)
