@@ -9,7 +9,7 @@ Names follow the reference kernels they replace: ``pack_q8`` (quantize.py:31),
 device memory and the stream); every kernel is in libq8cuda.so.
 
 Without a counterpart in the reference: the 8-bit paged cache (``KV8Pages``,
-``kv8_append``, ``kv8_read``, ``kv8_attention``), the page tables of either cache
+``rope``, ``kv8_append``, ``kv8_read``, ``kv8_attention``), the page tables of either cache
 (``kv_truncate``, ``kv_fork``, ``kv_reserve``, ``kv_compact``, ``kv_copy_pages``) and
 speculative decoding (``probs``, ``verify``).  include/q8cuda.h says what each
 does; these run on the device of their tensors, on torch's current stream
@@ -138,11 +138,19 @@ def rope_inv_freq(cfg) -> torch.Tensor:
 
 
 def rope(qkv, pos, n_heads, n_kv, hd, inv_freq, q_norm=None, k_norm=None, eps=1e-6):
-    """(QK-norm and) RoPE of the q and k heads of q|k|v rows, in place, without an append."""
-    _need_cuda(qkv, pos, inv_freq, q_norm, k_norm)
-    check(lib().q8op_rope_kv_append(_p(qkv), qkv.stride(0), qkv.shape[0], _p(pos), None, n_heads, n_kv, hd,
-                                    _p(inv_freq), _p(q_norm), _p(k_norm), eps, None, None, 0, None, 0,
-                                    _stream(qkv)))
+    """(QK-norm and) RoPE of the q and k heads of q|k|v rows (f32), in place, without an append."""
+    dev = qkv.get_device()
+    rows, width, ld = _matrix(qkv, "rope: qkv", dev)
+    if width < (n_heads + 2 * n_kv) * hd:
+        raise ValueError(f"rope: qkv rows of {n_heads} + 2 x {n_kv} heads of {hd} wanted, got {width} columns")
+    _tensor(pos, "rope: pos", torch.int32, (rows,), dev)
+    _tensor(inv_freq, "rope: inv_freq", torch.float32, (hd // 2,), dev)
+    for t, what in ((q_norm, "rope: q_norm"), (k_norm, "rope: k_norm")):
+        if t is not None:
+            _tensor(t, what, torch.bfloat16, (hd,), dev)
+    if rows:
+        _call(lib().q8op_rope_kv_append, dev, qkv.data_ptr(), ld, rows, pos.data_ptr(), None, n_heads, n_kv, hd,
+              inv_freq.data_ptr(), _p(q_norm), _p(k_norm), eps, None, None, 0, None, 0)
 
 
 def rope_kv_append(qkv, pos, seq, n_heads, n_kv, hd, inv_freq, q_norm, k_norm, eps, k_pages, v_pages, page,

@@ -84,3 +84,26 @@ def test_a_refused_launch_is_not_blamed_on_the_next_call(cuda):
     assert status == _lib.Q8_ERR_CUDA and "k_rope_kv" in _lib.last_error()
     assert int(ops.argmax(x)) == int(x.argmax())
     assert float(torch.zeros(3, device=cuda).sum()) == 0.0
+
+
+@pytest.mark.gpu
+def test_rope_refuses_what_its_kernel_would_misread(cuda):
+    """Rows, positions and frequencies of other types or lengths reach behind their tensors."""
+    nh, kv, hd, T = 4, 2, 64, 3
+    w = (nh + 2 * kv) * hd
+    qkv, pos = torch.randn((T, w), device=cuda), torch.arange(T, device=cuda, dtype=torch.int32)
+    inv, norm = torch.rand(hd // 2, device=cuda), torch.ones(hd, device=cuda, dtype=torch.bfloat16)
+    was = qkv.clone()
+    for bad in (lambda: ops.rope(qkv.bfloat16(), pos, nh, kv, hd, inv), lambda: ops.rope(qkv[:, 1:], pos, nh, kv, hd, inv),
+                lambda: ops.rope(qkv.t(), pos, nh, kv, hd, inv), lambda: ops.rope(qkv, pos.long(), nh, kv, hd, inv),
+                lambda: ops.rope(qkv, pos[:2], nh, kv, hd, inv), lambda: ops.rope(qkv, pos, nh, kv, hd, inv[:-1]),
+                lambda: ops.rope(qkv, pos, nh, kv, hd, inv.double()), lambda: ops.rope(qkv, pos, nh, kv, hd, inv, norm.float()),
+                lambda: ops.rope(qkv, pos, nh, kv, hd, inv, norm, norm[:32]), lambda: ops.rope(qkv, pos.cpu(), nh, kv, hd, inv)):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(_lib.Q8Error):
+        ops.rope(qkv, pos, 8, 4, 32, inv[:16])
+    assert torch.equal(qkv, was)
+    ops.rope(qkv[:0], pos[:0], nh, kv, hd, inv)  # no rows: nothing to do
+    ops.rope(qkv, pos, nh, kv, hd, inv, norm, norm)
+    assert not torch.equal(qkv, was) and torch.equal(qkv[:, (nh + kv) * hd:], was[:, (nh + kv) * hd:])
