@@ -242,6 +242,11 @@ class KV8Pages:
         self._ref = C.addressof(self._c)
         self._dev = dev
 
+    def __setattr__(self, name, value):
+        if hasattr(self, "_dev"):  # set last: the calls go by the addresses taken here
+            raise AttributeError(f"KV8Pages: {name} cannot be replaced, make another KV8Pages")
+        super().__setattr__(name, value)
+
     @classmethod
     def empty(cls, num_pages: int, n_kv: int, page: int = 64, head_dim: int = 128, device="cuda") -> "KV8Pages":
         """Zeroed pages."""

@@ -107,3 +107,15 @@ def test_rope_refuses_what_its_kernel_would_misread(cuda):
     ops.rope(qkv[:0], pos[:0], nh, kv, hd, inv)  # no rows: nothing to do
     ops.rope(qkv, pos, nh, kv, hd, inv, norm, norm)
     assert not torch.equal(qkv, was) and torch.equal(qkv[:, (nh + kv) * hd:], was[:, (nh + kv) * hd:])
+
+
+@pytest.mark.gpu
+def test_pages_keep_the_tensors_that_they_were_made_of(cuda):
+    """The calls read the addresses of the first tensors: a replaced one would be read after it is free."""
+    pages = ops.KV8Pages.empty(2, 1, 16, 64, cuda)
+    k = pages.k
+    for name in ("k", "v", "k_scale", "v_scale", "num_pages", "page"):
+        with pytest.raises(AttributeError):
+            setattr(pages, name, getattr(pages, name))
+    pages.k[1] = 3
+    assert pages.k is k and pages.tensors()[0] is k and int(k.sum()) == 3 * 16 * 64
