@@ -303,7 +303,8 @@ int q8op_kv_fork(int32_t* block_table, int64_t S, int max_pages, int32_t* ctx, i
  * copy (q8op_kv_copy_pages; -1: none).  When all sharers of a page write, the
  * first of them keeps it.  Requests are served in the order of (sequence,
  * position).  ctx grows by n_new.  All or nothing: when the pool or a table row
- * is too small, nothing changes, and src / dst are -1.  status [3]: Q8_OK or
+ * is too small, nothing changes, and src / dst are -1: rows that are appended
+ * all the same would replace the last positions.  status [3]: Q8_OK or
  * Q8_ERR_KV_FULL, pages wanted (of the rows that fit their table), pages free
  * after the call.  src, dst [S], status and work [num_pages] are int32 device
  * memory, work being scratch. */

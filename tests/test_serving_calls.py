@@ -1,6 +1,9 @@
 """How the Python entries of the paged-cache serving operators make their calls: what they hand to
 the library stays alive until the call has returned."""
 import gc
+import os
+import re
+import textwrap
 import threading
 import types
 import weakref
@@ -119,3 +122,46 @@ def test_pages_keep_the_tensors_that_they_were_made_of(cuda):
             setattr(pages, name, getattr(pages, name))
     pages.k[1] = 3
     assert pages.k is k and pages.tensors()[0] is k and int(k.sum()) == 3 * 16 * 64
+
+
+def documented_step():
+    """The Python blocks of INTEGRATION.md's section on the serving operators: set-up, one step."""
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "INTEGRATION.md")
+    with open(path) as f:
+        text = f.read().split("## Serving operators on a paged cache")[1].split("\n## ")[0]
+    return [textwrap.dedent(b) for b in re.findall(r"```python\n(.*?)```", text, re.S)]
+
+
+@pytest.mark.gpu
+def test_the_documented_step_and_a_full_pool(cuda):
+    """The step as INTEGRATION.md shows it: drafts verified, refused positions given back.  Where the
+    pool is full it leaves lengths, pages and their content as they are."""
+    setup, step = documented_step()
+    S, V, n = 2, 50, 3
+    env = dict(torch=torch, num_pages=3, n_kv=1, head_dim=64, n_heads=2, layers=2, temp=0.0)
+    env["table"] = torch.full((S, 4), -1, dtype=torch.int32, device=cuda)
+    env["ctx"], env["refs"] = (torch.zeros(k, dtype=torch.int32, device=cuda) for k in (S, 3))
+    exec(setup, env)
+    g = torch.Generator(device=cuda).manual_seed(0)
+    env["inv_freq"] = torch.rand(32, generator=g, device=cuda)
+    used = 0
+    for _ in range(60):
+        qkv = torch.randn((S * n, 4 * 64), generator=g, device=cuda)
+        env.update(qkv=qkv, q=qkv[:, :128], k=qkv[:, 128:192], v=qkv[:, 192:], n_new=env["ctx"] * 0 + n,
+                   pos=(env["ctx"][:, None] + torch.arange(n, device=cuda)).flatten().int().contiguous(),
+                   seq_start=torch.arange(0, S * n + 1, n, dtype=torch.int32, device=cuda), q_drafts=None,
+                   logits=torch.randn((S * n, V), generator=g, device=cuda),
+                   u=torch.rand(S * n, generator=g, device=cuda))
+        ids = env["logits"].argmax(-1).int().roll(1)  # the first draft of each is the target's choice, the second is not
+        ids[2::n] = (ids[2::n] + 1) % V
+        env["ids"] = ids
+        was = [t.clone() for t in (env["ctx"], env["refs"], env["table"])] + \
+            [t.clone() for p in env["pages"] for t in p.tensors()]
+        exec(step, env)
+        now = [env["ctx"], env["refs"], env["table"]] + [t for p in env["pages"] for t in p.tensors()]
+        if int(env["status"][0]) != 0:
+            assert all(torch.equal(a, b) for a, b in zip(was, now))
+            break
+        assert env["n_accepted"].tolist() == [1, 1] and (env["ctx"] - was[0]).tolist() == [2, 2]
+        used += 1
+    assert int(env["status"][0]) == _lib.Q8_ERR_KV_FULL and used > 20
