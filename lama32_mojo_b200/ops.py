@@ -326,7 +326,7 @@ def _kv8_scratch(dev, *shape) -> int:
 
 def kv8_attention(q, seq_start, ctx, n_heads: int, pages: KV8Pages, block_table, out=None) -> torch.Tensor:
     """Causal GQA attention of packed rows over the 8-bit cache (q8op_kv8_attention).  Returns
-    [T, n_heads * head_dim] of q's type; ``out`` may be given (its padding rows are left alone)."""
+    [T, n_heads * head_dim] of q's type; ``out`` may be given (rows behind the last sequence are not written)."""
     S, width, dev = _packed("kv8_attention", seq_start, ctx, pages, block_table)
     if torch.cuda.current_device() != dev:  # the scratch's size goes by the device
         with torch.cuda.device(dev):
@@ -455,7 +455,8 @@ def probs(logits: torch.Tensor, temp: float, out: torch.Tensor = None) -> torch.
 def verify(p, q, ids, seq_start, u):
     """Verify drafted tokens against the target's distributions p [T, n] (q8op_verify): q is the
     drafts' [drafts, n] or None (certain drafts), ids [T] the tokens fed, u [T] uniform draws.
-    Returns (n_accepted [S], tokens [T]: kept drafts, the next token, -1)."""
+    Returns (n_accepted [S], tokens [T]: kept drafts, the next token, -1; rows behind the last sequence are
+    not written)."""
     dev = p.get_device()
     rows, n, ldp = _matrix(p, "verify: p", dev)
     S = seq_start.numel() - 1

@@ -165,3 +165,42 @@ def test_the_documented_step_and_a_full_pool(cuda):
         assert env["n_accepted"].tolist() == [1, 1] and (env["ctx"] - was[0]).tolist() == [2, 2]
         used += 1
     assert int(env["status"][0]) == _lib.Q8_ERR_KV_FULL and used > 20
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv,hd", [(2, 64), (8, 128), (3, 128)])
+def test_read_leaves_rows_behind_the_last_sequence(cuda, kv, hd):
+    from test_gpu_kv8 import i32, make_pages
+    page, ns, ctx, tail = 32, [3, 0, 9], [40, 5, 9], 7
+    pages = make_pages(cuda, 6, kv, page, hd)
+    args = i32([0, 3, 3, 12], cuda), i32(ctx, cuda), pages, i32([[0, 1], [2, -1], [3, 4]], cuda)
+    want = ops.kv8_read(*args, 12)
+    T = 12 + tail
+    k, v = (torch.full((T, kv, hd), 7.0, device=cuda) for _ in range(2))
+    L, stream = _lib.lib(), torch.cuda.current_stream().cuda_stream
+    _lib.check(L.q8op_kv8_read(pages._ref, args[0].data_ptr(), args[1].data_ptr(), 3, args[3].data_ptr(), 2,
+                               k.data_ptr(), v.data_ptr(), T, stream))
+    for got, w in zip((k, v), want):
+        assert torch.equal(got[:12], w) and bool((got[12:] == 7.0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [50, 20000])
+@pytest.mark.parametrize("certain", [False, True])
+def test_verify_leaves_rows_behind_the_last_sequence(cuda, n, certain):
+    """Tokens from seq_start[S] on keep what they were, and a sequence without rows touches none."""
+    from test_gpu_kv8 import i32
+    S, T, used = 4, 15, 9
+    g = torch.Generator(device=cuda).manual_seed(n)
+    p = torch.rand((T, n), generator=g, device=cuda)
+    q = None if certain else p[:used - 3].clone()
+    ids = p.argmax(-1).int().roll(1)
+    starts, u = i32([0, 4, 4, 5, 9], cuda), torch.rand(T, generator=g, device=cuda)
+    a, t = ops.verify(p[:used], q, ids[:used], starts, u[:used])
+    taken = torch.full((S + 2,), -9, dtype=torch.int32, device=cuda)
+    tokens = torch.full((T,), -9, dtype=torch.int32, device=cuda)
+    _lib.check(_lib.lib().q8op_verify(p.data_ptr(), n, None if certain else q.data_ptr(), n, 0 if certain else used - 3,
+                                      ids.data_ptr(), starts.data_ptr(), T, S, n, u.data_ptr(), taken.data_ptr(),
+                                      tokens.data_ptr(), torch.cuda.current_stream().cuda_stream))
+    assert torch.equal(taken[:S], a) and taken[S:].tolist() == [-9, -9]
+    assert torch.equal(tokens[:used], t) and tokens[used:].tolist() == [-9] * (T - used)
