@@ -177,10 +177,11 @@ __device__ __forceinline__ float kt_weights(uint32_t addr, const float4* sc, flo
 // 7.9e-6 too small (relative, least squares over all outputs, scores of deviation
 // 1.6).  So O goes into f32 sums in the workspace, which L2 holds, every KT_FLUSH
 // tiles.  f32 rows, 8 tiles: errors of whole outputs against 8000 positions, q of
-// deviation 0.5, 2 and 8, are 0.8e-6, 2.5e-6 and 1.8e-6, those of elementary f32
-// operations 1.6e-6, 2.0e-6 and 1.8e-6; what is left comes from the scores.
-// 4 tiles: 0.5e-6, 2.0e-6, 1.8e-6 at 417 us for 383 (2 x 1024 rows of 32 heads,
-// 8000 and 2524 positions; no flush 355, adding in L2 by red.add 481).
+// deviation 0.5, 2 and 8, are 0.8e-6, 1.5e-6 and 0.6e-6, those of elementary f32
+// operations 1.6e-6, 2.0e-6 and 1.8e-6.  Scores add the products with ql first: the
+// other way round all of them were cut off at the scores' size, 2.5e-6 for q of
+// deviation 2.  4 tiles: 417 us for 383 (2 x 1024 rows of 32 heads, 8000 and 2524
+// positions; no flush 355, adding in L2 by red.add 481).
 // 16-bit rows, 64 tiles: 8.8e-6, a fiftieth of f16's rounding, at no cost to speak of.
 template <bool WIDE>
 constexpr int KT_FLUSH = WIDE ? 8 : 64;
@@ -655,11 +656,11 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
           const uint32_t d = tmem + (t & 1) * KT_KEYS;
           if (kt_elect()) {
 #pragma unroll
-            for (int x = 0; x < (WIDE ? 2 : 1); ++x)
+            for (int x = WIDE ? 1 : 0; x >= 0; --x)  // the small halves first: little of their sums is cut off
 #pragma unroll
               for (int k = 0; k < HD / 16; ++k)  // 16 dims: 32 bytes further inside the swizzle atom
                 kt_mma_ss(d, dq + (x * HALVES + (k >> 2)) * (Sh::QP >> 4) + (k & 3) * 2,
-                          dk + (k >> 2) * (Sh::KP >> 4) + (k & 3) * 2, is, (x | k) != 0);
+                          dk + (k >> 2) * (Sh::KP >> 4) + (k & 3) * 2, is, x != (WIDE ? 1 : 0) || k != 0);
             kt_commit(&kfree);
             kt_commit(&sfull[t & 1]);
           }
@@ -672,11 +673,11 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
           kt_fence_after();
           if (kt_elect()) {
 #pragma unroll
-            for (int x = 0; x < 2; ++x)
+            for (int x = 1; x >= 0; --x)
 #pragma unroll
               for (int k = 0; k < KT_KEYS / 16; ++k)  // 16 positions: two atoms further
                 kt_mma_ts(tmem_o, tmem + (p & 1) * KT_KEYS + (k >> 1) * 32 + x * 16 + (k & 1) * 8, dv + k * (2048 >> 4),
-                          io, (x | k) != 0 || (j - 1) % Sh::FLUSH != 0);
+                          io, x == 0 || k != 0 || (j - 1) % Sh::FLUSH != 0);
             kt_commit(&pvdone[p & 1]);
           }
           __syncwarp();

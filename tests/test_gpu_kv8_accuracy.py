@@ -112,3 +112,39 @@ def test_values_of_any_size(cuda, ns, ctx, width, lo, hi, dtype):
     got, ref, tol = attend(cuda, 2, 4, 128, 64, ns, ctx, dtype, 3, width, pages)
     assert np.isfinite(got).all()
     assert (np.abs(got - ref) / tol).max() <= 1
+
+
+@pytest.mark.parametrize("deviation", [0.5, 2.0, 8.0])
+def test_long_chunks_are_as_exact_as_f32_operations(cuda, deviation):
+    """f32 chunks against 8000 positions, as a whole: not further from 64 bits than the same formula in
+    elementary f32 operations, which round every sum where the tensor cores cut theirs off."""
+    ctx, n, S, kv, G, hd, page = 8000, 256, 8, 8, 4, 128, 64
+    g = torch.Generator(device=cuda).manual_seed(3)
+    per = ctx // page
+    shape = per, kv, page, hd
+
+    def codes():
+        return torch.randn(shape, generator=g, device=cuda).mul_(36).round_().clamp_(-127, 127).to(torch.int8)
+
+    def scales():
+        return torch.rand((per, kv, page // 16), generator=g, device=cuda) * 0.02 + 0.01
+
+    pages = ops.KV8Pages(codes(), codes(), scales(), scales())
+    q = torch.randn((n, kv * G * hd), generator=g, device=cuda) * deviation
+    row = np.arange(per, dtype=np.int32)
+    got = ops.kv8_attention(q.repeat(S, 1), i32(starts([n] * S), cuda), i32([ctx] * S, cuda), kv * G, pages,
+                            i32(np.tile(row, (S, 1)), cuda))[:n]
+    later = torch.arange(ctx, device=cuda)[None] > (ctx - n + torch.arange(n, device=cuda))[:, None]
+
+    def plain(dtype):
+        def values(c, s):
+            return (c.to(dtype) * s.to(dtype).repeat_interleave(16, 2)[..., None]).transpose(1, 2).reshape(ctx, kv, hd)
+        s = torch.einsum("nkgd,pkd->kgnp", q.to(dtype).view(n, kv, G, hd), values(pages.k, pages.k_scale)) / hd ** 0.5
+        p = s.masked_fill_(later, float("-inf")).softmax(-1)
+        return torch.einsum("kgnp,pkd->nkgd", p, values(pages.v, pages.v_scale)).reshape(n, -1).double()
+
+    was = torch.backends.cuda.matmul.allow_tf32
+    torch.backends.cuda.matmul.allow_tf32 = False
+    exact, near = plain(torch.float64), plain(torch.float32)
+    torch.backends.cuda.matmul.allow_tf32 = was
+    assert float((got.double() - exact).norm()) <= float((near - exact).norm())
