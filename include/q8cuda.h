@@ -246,9 +246,14 @@ typedef struct q8_kv8_pages {
  * the block has earlier tokens and their scale is larger; codes that stay
  * become round(code * old / new), new ones round(x / scale), both of the exact
  * quotient, ties to even, within +-127.  A block whose first token is new
- * starts over.  NaN is stored as 0; infinities as +-127, and they do not
- * enter the scale.  Rows whose page is not there are left out.  The table may
- * not lead two of the call's rows to the same place. */
+ * starts over.  Otherwise its scale only grows, and every growth rounds the
+ * codes that stay once more (half a step of the new scale): 15 times at most
+ * while a block fills, and again for each drafted token that is refused and
+ * given back (q8op_kv_truncate), whose scale stays.  So decoding with drafts
+ * does not leave the codes that decoding without them leaves.  NaN is stored as
+ * 0; infinities as +-127, and they do not enter the scale.  Rows whose page is
+ * not there are left out.  The table may not lead two of the call's rows to the
+ * same place. */
 int q8op_kv8_append(const void* k, int64_t ldk, const void* v, int64_t ldv, int dtype, int64_t rows,
                     const int32_t* seq_start, const int32_t* ctx, int64_t S, const q8_kv8_pages* kv,
                     const int32_t* block_table, int max_pages, void* stream);

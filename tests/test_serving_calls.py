@@ -204,3 +204,21 @@ def test_verify_leaves_rows_behind_the_last_sequence(cuda, n, certain):
                                       tokens.data_ptr(), torch.cuda.current_stream().cuda_stream))
     assert torch.equal(taken[:S], a) and taken[S:].tolist() == [-9, -9]
     assert torch.equal(tokens[:used], t) and tokens[used:].tolist() == [-9] * (T - used)
+
+
+@pytest.mark.gpu
+def test_a_refused_draft_leaves_its_scale(cuda):
+    """As documented: giving positions back does not shrink their block's scale, a new block starts over."""
+    from test_gpu_kv8 import i32
+    pages = ops.KV8Pages.empty(2, 1, 16, 64, cuda)
+    table, refs, ctx, start = i32([[0, 1]], cuda), i32([1, 1], cuda), i32([3], cuda), i32([0, 3], cuda)
+    x = torch.ones((3, 64), device=cuda)
+    x[2] = 100.0
+    ops.kv8_append(x, x, start, ctx, pages, table)
+    ops.kv_truncate(table, ctx, refs, 16, i32([2], cuda))
+    ctx += 15
+    ops.kv8_append(x[:1].expand(15, 64).contiguous(), x[:1].expand(15, 64).contiguous(), i32([0, 15], cuda), ctx, pages,
+                   i32([[0, 1]], cuda))
+    s = pages.k_scale.flatten()
+    assert float(s[0]) == float(np.float32(100) / np.float32(127)) and float(s[1]) == float(np.float32(1) / np.float32(127))
+    assert pages.k[0, 0].unique().tolist() == [1]  # 1 / (100 / 127) rounds to 1
