@@ -96,8 +96,9 @@ __device__ __forceinline__ unsigned kv8_max(unsigned top, unsigned w) {
 // number the touched blocks: sequence b's start at starts[b]/16 + 2b, which
 // leaves room for the n/16 + 2 blocks that n rows can touch.  Bytes: the rows
 // once, a quarter or half of that in codes.  12,562 bf16 rows of 8 kv heads of
-// 128: 17.4 us for 77 MB (4.4 TB/s), bound by the chain from sequence to page to
-// rows and by some 20 instructions an element.
+// 128, 77 MB: 17.4 us with the rows in the L2, 28.7 (under ncu) with nothing there,
+// bound by some 20 instructions an element and by the chain from sequence to page
+// to rows (no row is loaded before the table has answered, though it could be).
 //
 // Codes, two at a time in packed f32 operations: m = fma(x, 1/s, 1.5 2^23) rounds to the whole number nearest to the
 // estimated quotient and holds it in its low byte; r = m - 1.5 2^23.  The

@@ -750,7 +750,11 @@ static int ka_clusters(int c) {
 //             a second launch
 //   tcgen05   24 + 1.4 (1.2) a tile of a CTA for f32 rows, 1.0 (0.85) for 16-bit
 //             ones: pays when 128 rows share a reading
-// The form chosen so was within 1 % of the best one on average, 27 % at worst.
+// The form chosen so was within 1 % of the best one on average, 27 % at worst, with
+// tables as wide as the longest sequence.  Wider ones mislead it: 8 sequences of 512
+// positions take 7.9 us, 12.3 with 2048 columns of 64; 5 rows each 13.6 and 26.0.
+// (16-bit rows: fitted when a weight was one f16, which made all forms 5 to 12 %
+// faster.)
 // f32 rows, 32 heads on 8 of 128, us for the three: 8 sequences of 4000 positions,
 // 1 row, 16.0, 21.7, 39.4; 16 of 8000, 39.4, 31.7, 90.1; 16 of 4500, 24 rows, 212,
 // 187, 88.

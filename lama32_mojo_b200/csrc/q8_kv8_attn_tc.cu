@@ -18,10 +18,12 @@
 // M moves only when it has grown by more than 1, so that O in TMEM is scaled
 // seldom.
 //
-// Bound.  2 x 1024 f32 rows of 32 heads on 8 of 128, 8000 positions: 385 us for
-// 258 GFLOP, 516 in f16 products (1.34 PFLOP/s, 0.81 of cuBLAS's bf16 rate).  The
-// tensor pipes are busy 40 % of the time, the issue slots 52 %: the chain from
-// scores to weights is what is waited for.  bf16 rows: 391 us (356 with one f16 a weight).
+// Bound.  2 x 1024 f32 rows of 32 heads on 8 of 128, 8000 and 2524 positions: 380 us
+// for 159 GFLOP, 319 in f16 products (0.84 PFLOP/s, 0.50 of cuBLAS's bf16 rate, at
+// which they take 192 us).  The tensor pipes are busy 40 % of the time, the issue
+// slots 52 %: the chain of a tile, codes to f16 to scores to weights to product, is
+// what is waited for, with one buffer each for K and V.  bf16 rows, 239 GFLOP in
+// products: 383 us (356 with one f16 a weight).
 //
 // Two CTAs an SM (256 TMEM columns each) cover one another's waits.  Their
 // number is fixed; each takes an equal stretch of all units' work and leaves

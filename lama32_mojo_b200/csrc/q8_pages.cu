@@ -6,10 +6,17 @@
 // lengths, refs [num_pages] int32, the table entries that hold a page; 0 is
 // free.  There is no list of free pages: a page is taken by scanning refs, the
 // lowest number first, so equal states give equal results.  Sums into refs are
-// integer atomics; their order does not matter.  Tables are small: the kernels on
-// them wait for memory a few times in a row, which takes 3 to 11 us whatever
-// their sizes are (64 sequences of 16 pages: truncate 4, fork 7, reserve 11,
-// compact of 3000 pages 8 us with nothing in the caches).
+// integer atomics; their order does not matter.
+//
+// Bound: chains of loads and barriers, not bytes.  64 sequences, 17 columns, 389
+// pages, everything in the caches: truncate 1.8, fork 4.9, reserve 3.7, compact
+// 4.5 us (3.6, 7.0, 10.9 and, of 3000 pages, 8.3 with nothing there).  Truncate has
+// a CTA for each sequence (2048 columns: 3.5 us); the others are one CTA each and
+// grow:  fork with the table's columns, a strip of 4 to 32 after the other whatever
+// the lengths are (2048 columns: 112 us; 1024 sequences 1.3 ms);  reserve and compact
+// with the pool, 1024 counts in a round of three barriers, compact three times (16,384
+// pages: 12.6 and 25 us, 262,144: 149 and 375);  reserve also compares every
+// sequence that writes into a shared page with all sequences.
 #include "q8_kernels.h"
 
 #include <algorithm>

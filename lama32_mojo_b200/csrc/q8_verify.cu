@@ -164,7 +164,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
       for (int e = 0; e < 2; ++e) {
         const float l0 = v[k][2 * e], l1 = v[k][2 * e + 1];
         const uint64_t d = f2_add(f2_pack(l0, l1), top2), y = f2_fma(d, ch2, up);
-        const uint64_t z = f2_fma(d, cl2, f2_fma(d, ch2, f2_fma(y, minus, up)));  // y - 64 is exact
+        // y - 64 is exact for y >= 32; below, weights under 2^-32 of the largest are off by up to 1.3e-6
+        const uint64_t z = f2_fma(d, cl2, f2_fma(d, ch2, f2_fma(y, minus, up)));
         float p0, p1;
         asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p0) : "f"(f2_lo(y)));
         asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p1) : "f"(f2_hi(y)));
@@ -201,8 +202,9 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
 // A cluster of CTAs per sequence; all of them find the refused row, then each
 // adds up a slice of its weights, in segments of 128 per warp, so that the
 // drawn index is found in one segment: p and q rows are read once.  64 sequences,
-// 151,936 columns: 16.6 us for 78 MB (4.7 TB/s), a launch and four steps that wait
-// for one another; one sequence 7.2 us.  Segments of 512 took 19.2 at 18.5.
+// 151,936 columns, 78 MB: 16.1 us from the L2, 24 from memory (3.2 TB/s), a launch
+// and four steps that wait for one another; one sequence 7.0 us.  Segments of 512
+// took 19.2 at 18.5.
 constexpr int VF_SEG = 128;
 
 __global__ void __launch_bounds__(VF_THREADS) k_verify(const float* __restrict__ p, int64_t ldp,
