@@ -598,7 +598,8 @@ __global__ void __launch_bounds__(KT_THREADS, 2) k_kv8_attn_tc(Kv8AttnArgs a) {
       auto scales_out = [&](uint32_t t, int id) {
         if (warp != 4) return;
         if (lane < KT_BLOCKS)
-          s_sc[t & 3][lane] = make_float4(sk, sv * KT_LIFT, id >= 0 ? fmaxf(__log2f(sv), KA_LEAST) - KA_DOWN : -INFINITY, 0.f);
+          s_sc[t & 3][lane] = make_float4(sk, sv * KT_LIFT,
+                                          id >= 0 ? fmaxf(__log2f(sv), KA_LEAST) - KA_DOWN : -INFINITY, 0.f);
         __syncwarp();
         if (lane == 0) kt_arrive(&scfull[t & 3]);
       };

@@ -125,7 +125,7 @@ def test_pages_keep_the_tensors_that_they_were_made_of(cuda):
 
 
 def documented_step():
-    """The Python blocks of INTEGRATION.md's section on the serving operators: set-up, one step."""
+    """The Python blocks of the integration notes on the serving operators: set-up, one step."""
     path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "INTEGRATION.md")
     with open(path) as f:
         text = f.read().split("## Serving operators on a paged cache")[1].split("\n## ")[0]
@@ -134,7 +134,7 @@ def documented_step():
 
 @pytest.mark.gpu
 def test_the_documented_step_and_a_full_pool(cuda):
-    """The step as INTEGRATION.md shows it: drafts verified, refused positions given back.  Where the
+    """The step as the integration notes show it: drafts verified, refused positions given back.  Where the
     pool is full it leaves lengths, pages and their content as they are."""
     setup, step = documented_step()
     S, V, n = 2, 50, 3
